@@ -32,6 +32,7 @@ from .cache import (  # noqa: F401
     RoleAwareAsymKVCache,
     load_per_layer_bits_from_policy,
 )
+from .paged import append_paged, decode_attn_paged, evict_paged, prefill_attn_window  # noqa: F401
 from .patch import (  # noqa: F401
     INT8CacheWrapper,
     INT8CacheWrapperContainer,
@@ -61,6 +62,10 @@ __all__ = [
     "decode_attn_int4_kivi",
     "decode_attn_int4_asym_v2",
     "decode_attn_int4_asym_gqa",
+    "append_paged",
+    "decode_attn_paged",
+    "prefill_attn_window",
+    "evict_paged",
     "INT8CacheWrapper",
     "INT8CacheWrapperContainer",
     "apply_int8_fused_patch",

@@ -33,6 +33,10 @@ KVQ_FMT_INT4_KIVI = 4
 KVQ_FMT_INT8_KIVI = 5
 KVQ_FMT_FP16 = 6
 
+KVQ_PAGED_F16 = 0
+KVQ_PAGED_BF16 = 1
+KVQ_PAGED_INT8 = 2
+
 KVQ_LAYOUT_ROWS = 0
 KVQ_LAYOUT_TILE32 = 1
 
@@ -122,6 +126,76 @@ class AppendParams(ctypes.Structure):
     ]
 
 
+class PagedCache(ctypes.Structure):
+    """kvq_paged_cache (include/kvq_paged.h)."""
+    _fields_ = [
+        ("k", c_vp), ("v", c_vp),
+        ("k_stride_p", c_i64), ("k_stride_h", c_i64), ("k_stride_t", c_i64),
+        ("v_stride_p", c_i64), ("v_stride_h", c_i64), ("v_stride_t", c_i64),
+        ("k_scale", c_vp), ("v_scale", c_vp),
+        ("ks_stride_p", c_i64), ("ks_stride_h", c_i64), ("vs_stride_p", c_i64), ("vs_stride_h", c_i64),
+        ("table", c_vp), ("table_stride", c_i64),
+        ("num_pages", c_i32), ("max_pages", c_i32), ("page_size", c_i32), ("format", c_i32),
+        ("group_size", c_i32), ("batch", c_i32), ("kv_heads", c_i32), ("reserved", c_i32),
+    ]
+
+
+class PagedAppendParams(ctypes.Structure):
+    _fields_ = [
+        ("cache", PagedCache),
+        ("k", c_vp), ("v", c_vp),
+        ("k_stride_b", c_i64), ("k_stride_h", c_i64), ("k_stride_s", c_i64),
+        ("v_stride_b", c_i64), ("v_stride_h", c_i64), ("v_stride_s", c_i64),
+        ("write_pos", c_vp), ("new_lens", c_vp),
+        ("seq_new", c_i32), ("x_type", c_i32),
+    ]
+
+
+class PagedDecodeParams(ctypes.Structure):
+    _fields_ = [
+        ("cache", PagedCache),
+        ("q", c_vp), ("q_stride_b", c_i64), ("q_stride_h", c_i64), ("out", c_vp),
+        ("context_lens", c_vp), ("inv_tau", c_vp),
+        ("weights", c_vp), ("w_stride_b", c_i64), ("w_stride_h", c_i64),
+        ("workspace", c_vp), ("workspace_bytes", c_i64),
+        ("sm_scale", c_f32), ("window", c_i32), ("sinks", c_i32), ("q_heads", c_i32), ("q_type", c_i32),
+        ("reserved", c_i32),
+    ]
+
+
+class PrefillParams(ctypes.Structure):
+    _fields_ = [
+        ("q", c_vp), ("k", c_vp), ("v", c_vp),
+        ("q_stride_b", c_i64), ("q_stride_h", c_i64), ("q_stride_s", c_i64),
+        ("k_stride_b", c_i64), ("k_stride_h", c_i64), ("k_stride_s", c_i64),
+        ("v_stride_b", c_i64), ("v_stride_h", c_i64), ("v_stride_s", c_i64),
+        ("out", c_vp), ("o_stride_b", c_i64), ("o_stride_h", c_i64), ("o_stride_s", c_i64),
+        ("q_lens", c_vp), ("kv_lens", c_vp), ("inv_tau", c_vp),
+        ("workspace", c_vp), ("workspace_bytes", c_i64),
+        ("sm_scale", c_f32), ("batch", c_i32), ("q_heads", c_i32), ("kv_heads", c_i32), ("seq_q", c_i32),
+        ("seq_kv", c_i32), ("window", c_i32), ("sinks", c_i32), ("type", c_i32), ("reserved", c_i32),
+    ]
+
+
+class PagedEvictParams(ctypes.Structure):
+    _fields_ = [
+        ("cache", PagedCache),
+        ("context_lens", c_vp), ("weights", c_vp), ("w_stride_b", c_i64), ("w_stride_h", c_i64),
+        ("new_lens", c_vp), ("kept", c_vp), ("new_weights", c_vp),
+        ("w_tokens", c_i32), ("budget", c_i32), ("sinks", c_i32), ("recent", c_i32),
+    ]
+
+
+# include/kvq_paged.h
+PAGED_SYMBOLS = (
+    "kvq_paged_append",
+    "kvq_paged_decode",
+    "kvq_paged_decode_workspace_bytes",
+    "kvq_prefill_attn",
+    "kvq_prefill_workspace_bytes",
+    "kvq_paged_evict",
+)
+
 EXPORTED_SYMBOLS = (
     "kvq_decode_attn",
     "kvq_decode_attn_noalloc",
@@ -196,6 +270,15 @@ def lib() -> ctypes.CDLL:
         L.kvq_append_plan.restype = c_i32
         L.kvq_append_division.argtypes = [c_vp, c_vp, c_vp, c_vp, c_i64, c_vp]
         L.kvq_append_division.restype = c_i32
+        # the paged cache (include/kvq_paged.h)
+        for name, params in (("kvq_paged_append", PagedAppendParams), ("kvq_paged_decode", PagedDecodeParams),
+                             ("kvq_prefill_attn", PrefillParams), ("kvq_paged_evict", PagedEvictParams)):
+            getattr(L, name).argtypes = [ctypes.POINTER(params), c_vp]
+            getattr(L, name).restype = c_i32
+        for name, params in (("kvq_paged_decode_workspace_bytes", PagedDecodeParams),
+                             ("kvq_prefill_workspace_bytes", PrefillParams)):
+            getattr(L, name).argtypes = [ctypes.POINTER(params)]
+            getattr(L, name).restype = c_i64
         ver = L.kvq_abi_version()
         if ver != ABI_VERSION:
             raise ImportError(f"{LIB_PATH} has ABI {ver}, this package needs {ABI_VERSION}; rebuild it")

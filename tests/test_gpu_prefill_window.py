@@ -1,0 +1,210 @@
+"""prefill_attn_window against float64 attention over the visible keys.
+
+Tolerance as derived in test_gpu_paged.py; the probabilities enter the product with V in the inputs' type."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+D = 128
+SM = 1 / math.sqrt(D)
+U = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+F16, BF16 = torch.float16, torch.bfloat16
+
+
+def reference(q, k, v, qn, kn, window, sinks, tau=None, sm=SM):
+    """float64 (out, tolerance) [Hq, S, 128] of one sequence; q [Hq, S, 128], k, v [H, T, 128] on the GPU."""
+    hq, S, _ = q.shape
+    u = U[q.dtype]
+    out = torch.zeros(hq, S, D, dtype=torch.float64, device=q.device)
+    tol = torch.zeros_like(out)
+    if qn == 0 or kn == 0:
+        return out, tol
+    pos = torch.arange(kn - qn, kn, device=q.device)[:, None]
+    key = torch.arange(kn, device=q.device)[None]
+    vis = key <= pos
+    if window:
+        vis &= (key > pos - window) | (key < sinks)
+    any_ = vis.any(1)
+    for h in range(hq):
+        f = sm * (1.0 if tau is None else float(tau[h]))
+        kk, vv, qq = k[h * k.shape[0] // hq, :kn].double(), v[h * k.shape[0] // hq, :kn].double(), q[h, :qn].double()
+        kk, vv = torch.nan_to_num(kk), torch.where(torch.isfinite(vv), vv, 0.0)
+        s = (qq @ kk.t().contiguous() * f).masked_fill(~vis, -math.inf)
+        top = s.amax(1, keepdim=True)
+        e = torch.exp(s - torch.where(any_[:, None], top, 0.0)).masked_fill(~vis, 0.0)
+        L = e.sum(1, keepdim=True).clamp(min=1e-300)
+        p = e / L
+        o = p @ vv
+        d = 130 * 2.0 ** -23 * (qq.abs() @ kk.abs().t().contiguous() * abs(f)).masked_fill(~vis, 0.0).amax(1, keepdim=True)
+        A = p @ vv.abs()
+        out[h, :qn] = o
+        sub = 2.0 ** -25 * (vis.double() @ vv.abs()) / L if q.dtype == F16 else 0.0
+        tol[h, :qn] = u * o.abs() + (u + 2 * d + kn * 2.0 ** -23 + 2.0 ** -20) * A + sub + 1e-7
+    out[:, :qn][:, ~any_] = 0
+    tol[:, :qn][:, ~any_] = 0
+    return out, tol
+
+
+def make(B, hq, hkv, S, T, dtype, seed):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    q = torch.randn(B, hq, S, D, generator=g, device=DEV).to(dtype)
+    k = torch.randn(B, hkv, T, D, generator=g, device=DEV).to(dtype)
+    k[..., :4] *= 8
+    v = torch.randn(B, hkv, T, D, generator=g, device=DEV).to(dtype)
+    return q, k, v
+
+
+def run(B, hq, hkv, S, T, dtype, window=None, sinks=0, q_lens=None, kv_lens=None, seed=0, tau=False, edit=None, layout="bhsd"):
+    import llm_kvcache_quantization_amd as K
+
+    print(f"[prefill] B{B} {hq}/{hkv} S{S} T{T} {dtype} window {window} sinks {sinks} q_lens {q_lens} kv_lens {kv_lens}", flush=True)
+    q, k, v = make(B, hq, hkv, S, T, dtype, seed)
+    if kv_lens is not None:  # what lies behind a sequence may hold anything
+        for b, n in enumerate(kv_lens):
+            k[b, :, max(n, 0):] = math.nan
+            v[b, :, max(n, 0):] = math.nan
+    if edit is not None:
+        edit(q, k, v)
+    args = (q, k, v)
+    if layout == "bshd":
+        args = tuple(x.transpose(1, 2).contiguous().transpose(1, 2) for x in args)
+    elif layout == "odd":
+        args = tuple(torch.nn.functional.pad(x, (0, 4))[..., :D] for x in args)
+    t = torch.rand(hq, device=DEV) + 0.5 if tau else None
+    ten = lambda x: None if x is None else torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    out = K.prefill_attn_window(*args, SM, window=window, sinks=sinks, q_lens=ten(q_lens), kv_lens=ten(kv_lens), inv_tau=t)
+    torch.cuda.synchronize()
+    assert out.shape == q.shape and out.dtype == dtype
+    for b in range(B):
+        qn, kn = (q_lens or [S] * B)[b], (kv_lens or [T] * B)[b]
+        ref, tol = reference(q[b], k[b], v[b], min(max(qn, 0), S), min(max(kn, 0), T), window, sinks, t)
+        assert not torch.isnan(out[b]).any()
+        bad = (out[b].double() - ref).abs() - tol
+        assert bad.max() <= 0, (b, float(bad.max()), float((out[b].double() - ref).abs().max()))
+    return q, k, v, out
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("n", [1, 2, 31, 32, 33, 63, 64, 65, 127, 128, 129, 200, 513])
+def test_causal_prompts(dtype, n):
+    run(1, 6, 2, n, n, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 2), (5, 1), (64, 0), (64, 4), (100, 70), (130, 129), (128, 200), (1000, 4)])
+def test_windows(dtype, window, sinks):
+    run(1, 2, 1, 700, 700, dtype, window, sinks)
+    run(1, 2, 1, 40, 700, dtype, window, sinks)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("S,T", [(1, 1000), (1, 64), (5, 2049), (100, 101), (130, 4000), (64, 8192)])
+def test_chunks(dtype, S, T):
+    run(1, 4, 2, S, T, dtype)
+    run(1, 4, 2, S, T, dtype, 300, 4)
+
+
+@pytest.mark.parametrize("hq,hkv", [(1, 1), (12, 2), (28, 4), (40, 8), (32, 1)])
+def test_heads(hq, hkv):
+    run(2, hq, hkv, 150, 150, BF16, 90, 3)
+    run(2, hq, hkv, 20, 900, F16)
+
+
+def test_padded_batches():
+    run(4, 4, 2, 200, 200, F16, None, 0, [200, 0, 1, 130], [200, 0, 1, 130])
+    run(4, 4, 2, 200, 333, BF16, 50, 4, [200, 0, 1, 130], [333, 100, 65, 200])
+    run(3, 4, 2, 100, 4000, F16, None, 0, [100, 3, 64], [4000, 2500, 64])
+    run(2, 4, 2, 100, 50, F16)  # more queries than keys: the first see nothing
+    run(3, 2, 1, 70, 70, F16, None, 0, [70, -4, 999], [40, 70, -1])
+
+
+@pytest.mark.parametrize("layout", ["bshd", "odd"])
+def test_layouts(layout):
+    run(2, 6, 2, 140, 140, F16, 60, 4, layout=layout)
+    run(2, 6, 2, 40, 1400, BF16, layout=layout)
+
+
+def test_inv_tau_and_default_scale():
+    import llm_kvcache_quantization_amd as K
+
+    run(1, 6, 2, 140, 140, F16, 60, 4, tau=True)
+    q, k, v, out = run(1, 6, 2, 140, 140, F16)
+    assert torch.equal(K.prefill_attn_window(q, k, v), out)
+
+
+def test_empty():
+    import llm_kvcache_quantization_amd as K
+
+    for B, S, T in ((0, 5, 5), (2, 0, 5), (2, 5, 0)):
+        q, k, v = make(B, 4, 2, S, T, F16, 0)
+        out = K.prefill_attn_window(q, k, v)
+        assert out.shape == q.shape and not out.any()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("S", [300, 60, 20])
+def test_masked_rows_that_are_not_finite(dtype, S):
+    """NaN and Inf in K and V rows reach the queries that see them, and no others: V rows share a matrix
+    product with queries that do not."""
+    import llm_kvcache_quantization_amd as K
+
+    T, window, sinks = 1300, 70, 2
+    q, k, v = make(1, 2, 1, S, T, dtype, 3)
+    clean = K.prefill_attn_window(q, k, v, SM, window=window, sinks=sinks)
+    ref, tol = reference(q[0], k[0], v[0], S, T, window, sinks)
+    rows = {T - 1: math.nan, T - 9: math.inf, T - 80: -math.inf, 5: math.nan}
+    if S > 100:
+        rows[T - 200] = math.nan
+    v2, k2 = v.clone(), k.clone()
+    for t, x in rows.items():
+        v2[0, 0, t, 3] = x
+    k2[0, 0, 7] = math.nan  # seen by nobody: behind the sinks, before the window
+    k2[0, 0, T - 40] = math.nan  # seen by the queries from T - 40 to T - 40 + window - 1
+    out = K.prefill_attn_window(q, k2, v2, SM, window=window, sinks=sinks)
+    pos = torch.arange(T - S, T, device=DEV)
+    hit = torch.zeros(S, dtype=torch.bool, device=DEV)
+    for t in rows:
+        hit |= (pos >= t) & (pos < t + window)
+    lost = (pos >= T - 40) & (pos < T - 40 + window)
+    assert torch.isnan(out[0][:, lost]).all()
+    ok = ~lost
+    assert not torch.isfinite(out[0][:, ok & hit][..., 3]).any()
+    other = [c for c in range(D) if c != 3]
+    err = (out[0].double() - ref).abs() - tol
+    assert (err[:, ok][..., other] <= 0).all()
+    assert (err[:, ok & ~hit] <= 0).all()
+    assert torch.isfinite(clean).all()
+
+
+def test_scores_beyond_fp16():
+    def up(q, k, v):
+        k[:] = (torch.linspace(-60, 60, k.shape[2], device=DEV).view(1, 1, -1, 1) / 8).to(k.dtype)
+        q[:] = 1
+
+    def down(q, k, v):
+        up(q, k, v)
+        k.neg_()
+
+    for e in (up, down):
+        run(1, 2, 1, 400, 400, F16, edit=e)
+        run(1, 2, 1, 400, 400, BF16, 100, 4, edit=e)
+
+
+def test_all_scores_minus_infinity():
+    """A query whose visible keys all score -inf has no softmax: NaN, as torch has it."""
+    import llm_kvcache_quantization_amd as K
+
+    q, k, v = make(1, 2, 1, 10, 10, F16, 1)
+    q[:] = 1
+    k[:] = 0
+    k[:, :, :4, 0] = -math.inf
+    out = K.prefill_attn_window(q, k, v, SM)
+    assert torch.isnan(out[:, :, :4]).all() and torch.isfinite(out[:, :, 4:]).all()
+
+
+def test_long():
+    run(1, 2, 1, 4500, 4500, BF16, 1000, 4)
+    run(1, 2, 1, 2500, 9000, F16)
