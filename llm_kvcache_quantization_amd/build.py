@@ -40,9 +40,13 @@ def sources() -> list[Path]:
 # packed-fp32 VALU forms are disabled: the code never relies on them
 _FLAGS = ["-O3", "-std=c++17", "-fPIC", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
+# prefill_attn: its accumulators (64 registers, carried round the loop) stay whole vectors; broken into
+# scalars, as the compiler does by default, they are copied from register to register once a key tile
+_FILE_FLAGS = {"prefill_attn.hip": ["-mllvm", "-amdgpu-codegenprepare-break-large-phis=0"]}
+
 
 def compile_command(src: Path, obj: Path) -> list[str]:
-    return [hipcc(), f"--offload-arch={ARCH}", *_FLAGS, f"-I{INCLUDE}", f"-I{CSRC}", "-c",
+    return [hipcc(), f"--offload-arch={ARCH}", *_FLAGS, *_FILE_FLAGS.get(src.name, []), f"-I{INCLUDE}", f"-I{CSRC}", "-c",
             str(src), "-o", str(obj)]
 
 

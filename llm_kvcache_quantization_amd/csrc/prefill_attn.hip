@@ -11,15 +11,16 @@
 //
 // Lane (q, hh) = (lane % 32, lane / 32) of a 32 x 32 result holds rows 8 (i / 4) + 4 hh + i % 4 of column
 // q, i < 16.  The 8 reduction slots that P^T's operand takes from it are keys 16 mm + {4 hh + r, 8 + 4 hh +
-// r}, r < 4; V is staged transposed with those keys side by side, 16 bytes a (channel, 16 keys, half).
+// r}, r < 4; V^T's operand has the same keys from two transposing LDS reads of 4 keys each.
 //
-// K and V tiles go through registers into LDS, two buffers each, the next tile's loads under the present
-// one's products.  Rows of both are XOR-swizzled in 16-byte chunks so that the operands' reads and the
-// stores spread over all banks.
+// K and V tiles go straight from memory into LDS, two buffers each, the next tile's loads under the present
+// one's products.  Rows are XOR-swizzled in 16-byte chunks (by the lanes' choice of what they load), so that
+// the operands' reads spread over all banks.
 //
-// What is masked may hold anything.  Keys at or past kv_lens are staged as zeros.  An Inf or NaN in a V row
-// that some query of a tile sees and another does not would reach both (0 x NaN): where a work-group's result
-// is not finite it runs again with such rows taken out of the products and added query by query.
+// What is masked may hold anything.  In the place of keys at or past kv_lens the last key is loaded.  An Inf or
+// NaN in a V row that some query of a tile sees and another does not would reach both (0 x NaN): where a
+// work-group's result is not finite it runs again with such rows taken out of the products and added query by
+// query.
 //
 // What bounds it: the matrix units and the exponentials, about equally.
 #include "paged.h"
@@ -74,10 +75,13 @@ __device__ __forceinline__ Row unit_of(const PreArgs& a, int64_t unit) {
   Row r;
   r.split = (int)(unit % a.splits);
   unit /= a.splits;
-  r.block = a.blocks - 1 - (int)(unit % a.blocks);  // the later queries see more keys: first
+  // blocks from both ends in turn: any run of units has its share of the long ones (the later queries') and
+  // the short ones; rows of a batch in turn for the same reason
+  const int x = (int)(unit % a.blocks);
+  r.block = x & 1 ? x >> 1 : a.blocks - 1 - (x >> 1);
   unit /= a.blocks;
-  r.h = (int)(unit % a.q_heads);
-  r.b = (int)(unit / a.q_heads);
+  r.b = (int)(unit % a.batch);
+  r.h = (int)(unit / a.batch);
   r.q_len = a.q_lens ? min(max(a.q_lens[r.b], 0), a.S) : a.S;
   r.kv_len = a.kv_lens ? min(max(a.kv_lens[r.b], 0), a.T) : a.T;
   r.off = r.kv_len - r.q_len;
@@ -89,101 +93,194 @@ __device__ __forceinline__ bool sees(int p, int key, int window, int sinks) {
   return key <= p && (window <= 0 || key > p - window || key < sinks);
 }
 __device__ __forceinline__ float xor32(float x) { return __shfl_xor(x, 32, 64); }
-__device__ __forceinline__ uint32_t pk_max_u16(uint32_t a, uint32_t b) {
-  typedef uint16_t u16v2 __attribute__((ext_vector_type(2)));
-  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16v2, a), __builtin_bit_cast(u16v2, b)));
-}
+struct Lds {
+  u32x4 k[2][kBN * 16];  // [key][16 chunks of 8 channels], chunk ^ (key % 16)
+  u32x4 v[2][kBN * 16];  // [key][16 chunks of 8 channels], chunk ^ 4 (key % 4)
+  uint32_t bad[2];       // keys of the tile whose V row is not finite
+};
 
-template <class T>
-struct Prefill {
-  struct Lds {
-    u32x4 k[2][kBN * 16];   // [key][16 chunks of 8 channels], chunk ^ (key % 16)
-    u32x4 v[2][128 * 8];    // [channel][8 chunks of 8 keys], chunk ^ swizzle(channel)
-    uint32_t bad[2];        // keys of the tile whose V row is not finite
-  };
-  static __device__ __forceinline__ int vswz(int ch) { return ((ch >> 1) ^ (ch >> 4)) & 7; }
+typedef __attribute__((address_space(3))) uint8_t lds_u8;
+typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+typedef const __attribute__((address_space(1))) void* gptr;
+typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-  u32x4 rk[4];
-  u32x2 rv[8];
-
-  // this thread's part of the tile at key0: K rows t / 16 + 16 u, chunk t % 16; V: channels 4 (t % 32) .. of
-  // the 8 keys of chunk t / 32.  A tile's base is the same for all threads, offsets in it fit 32 bits.
-  __device__ __forceinline__ void load(const uint8_t* k, const uint8_t* v, const PreArgs& a, int key0, int kv_len) {
-    const int t = threadIdx.x, grp = t >> 5;
-    const int krow = t >> 4, vrow = 16 * (grp >> 1) + 4 * (grp & 1);
-    const uint32_t ko = (uint32_t)krow * (uint32_t)a.kss + (t & 15) * 16, vo = (uint32_t)vrow * (uint32_t)a.vss + (t & 31) * 8;
-    const uint8_t* kb = k + key0 * a.kss;
-    const uint8_t* vb = v + key0 * a.vss;
+// One side's tiles of rows key0 .. key0 + 63 into LDS.  A wave instruction loads four rows; a lane takes the
+// chunk that belongs at its place, 16 bytes from those of its neighbours.
+template <bool V>
+struct TileLoad {
+  const uint8_t* x;
+  int64_t stride;
+  uint32_t off;    // this lane's place in the tile's first 16 rows
+  int row, kv_len;
+  __device__ __forceinline__ TileLoad(const uint8_t* x_, int64_t stride_, int kv_len_) : x(x_), stride(stride_), kv_len(kv_len_) {
+    const int lane = threadIdx.x & 63;
+    row = 4 * (threadIdx.x >> 6) + (lane >> 4);
+    off = (uint32_t)row * (uint32_t)stride + ((lane & 15) ^ (V ? (row & 3) << 2 : row & 15)) * 16;
+  }
+  __device__ __forceinline__ void operator()(int key0, u32x4* to) const {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint8_t* base = x + key0 * stride;
     if (key0 + kBN <= kv_len) {
 #pragma unroll
-      for (int u = 0; u < 4; ++u) rk[u] = *(const u32x4*)(kb + 16 * u * a.kss + ko);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) rv[j] = *(const u32x2*)(vb + ((j & 3) + 8 * (j >> 2)) * a.vss + vo);
-    } else {
-      const int left = kv_len - key0;
-#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        __builtin_amdgcn_global_load_lds((gptr)(base + 16 * u * stride + off),
+                                         (__attribute__((address_space(3))) void*)(to + (16 * u + 4 * wave) * 16), 16, 0, 0);
+    } else {  // the last tile: its last key in the place of those behind
       for (int u = 0; u < 4; ++u) {
-        rk[u] = u32x4{0, 0, 0, 0};
-        if (krow + 16 * u < left) rk[u] = *(const u32x4*)(kb + 16 * u * a.kss + ko);
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        rv[j] = u32x2{0, 0};
-        if (vrow + (j & 3) + 8 * (j >> 2) < left) rv[j] = *(const u32x2*)(vb + ((j & 3) + 8 * (j >> 2)) * a.vss + vo);
+        const int over = max(key0 + 16 * u + row - (kv_len - 1), 0);
+        __builtin_amdgcn_global_load_lds((gptr)(base + 16 * u * stride + off - over * stride),
+                                         (__attribute__((address_space(3))) void*)(to + (16 * u + 4 * wave) * 16), 16, 0, 0);
       }
     }
   }
-  template <bool ROBUST>
-  __device__ __forceinline__ void store(Lds& s, int buf) {
+};
+
+template <class T>
+struct Prefill {
+  float16v acc[4];
+  float m, l;
+  bool seen;
+
+  // V of the second run: rows with an Inf or NaN as zeros, their keys marked
+  static __device__ __forceinline__ void load_v_finite(const uint8_t* x, int64_t stride, int key0, int kv_len, Lds& s) {
     const int t = threadIdx.x;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int row = (t >> 4) + 16 * u;
-      s.k[buf][row * 16 + ((t & 15) ^ (row & 15))] = rk[u];
-    }
-    const int grp = t >> 5, c4 = t & 31;
-    if constexpr (ROBUST) {
+      u32x4 w = *(const u32x4*)(x + min(key0 + row, kv_len - 1) * stride + (t & 15) * 16);
+      bool odd = false;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        bool odd = false;
-#pragma unroll
-        for (int d = 0; d < 2; ++d)
-          odd |= !(fabsf(T::to_f((uint16_t)rv[j][d])) < __builtin_inff()) ||
-                 !(fabsf(T::to_f((uint16_t)(rv[j][d] >> 16))) < __builtin_inff());
-        // a row's 32 lanes are one half of the wave
-        const uint64_t m = __ballot(odd);
-        if ((uint32_t)(threadIdx.x & 32 ? m >> 32 : m)) {
-          rv[j] = u32x2{0, 0};
-          const int key = 16 * (grp >> 1) + 4 * (grp & 1) + (j & 3) + 8 * (j >> 2);
-          if (c4 == 0) atomicOr(&s.bad[key >> 5], 1u << (key & 31));
-        }
+      for (int d = 0; d < 4; ++d)
+        odd |= !(fabsf(T::to_f((uint16_t)w[d])) < __builtin_inff()) || !(fabsf(T::to_f((uint16_t)(w[d] >> 16))) < __builtin_inff());
+      const uint64_t any = __ballot(odd);  // a row is 16 lanes
+      if ((any >> (t & 48)) & 0xFFFF) {
+        w = u32x4{0, 0, 0, 0};
+        if ((t & 15) == 0) atomicOr(&s.bad[row >> 5], 1u << (row & 31));
       }
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int ch = 4 * c4 + e;
-      const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
-      u32x4 w;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = perm_b32(rv[2 * j + 1][e >> 1], rv[2 * j][e >> 1], sel);
-      s.v[buf][ch * 8 + (grp ^ vswz(ch))] = w;
+      s.v[0][row * 16 + ((t & 15) ^ ((row & 3) << 2))] = w;
     }
   }
 
-  float16v acc[4];
-  float m, l;
-  bool seen;
+  // The products of this wave's 32 queries with 32 keys of a tile, those from 32 u on.
+  __device__ __forceinline__ void half_tile(const u32x4* ks, const u32x4* vs, const PreArgs& a, const u32x4 (&q)[8], float scale,
+                                            int key0, int u, int p, bool full) {
+    const int lane = threadIdx.x & 63, ql = lane & 31, hh = lane >> 5;
+    float16v sc;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) sc[j] = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < 8; ++kk) sc = T::mfma32(ks[(32 * u + ql) * 16 + ((2 * kk + hh) ^ (ql & 15))], q[kk], sc);
+    float mul = scale;
+    if (!full) {
+      mul = 1.f;
+      // key = first + c, c < 32 a constant: c against this lane's last key, first key and end of the sinks
+      const int first = key0 + 32 * u + 4 * hh;
+      const int last = p - first, from = a.window > 0 ? p - a.window - first : -1, sink = a.sinks - first;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const int c = 8 * (j >> 2) + (j & 3);
+        const bool vis = (c <= last) & ((c > from) | (c < sink));
+        seen |= vis;
+        sc[j] = vis ? sc[j] * scale : kNegInf;
+      }
+    }
+    u32x4 pb[2];
+    auto exps = [&]() {
+      const float mm = -(m == kNegInf ? 0.f : m);
+      float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+      for (int j = 0; j < 16; j += 2) {
+        const float e0 = fast_exp2(fmaf(sc[j], mul, mm)), e1 = fast_exp2(fmaf(sc[j + 1], mul, mm));
+        s0 += e0;
+        s1 += e1;
+        pb[j >> 3][(j >> 1) & 3] = T::pack(e0, e1);
+      }
+      return s0 + s1;
+    };
+    // while a lane's sum stays below 64 so does each of its P: the maximum follows only where it does not
+    float sum = exps();
+    if (__any(!(sum <= 64.f) || m == kNegInf)) {
+      float mx = kNegInf;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) mx = fmaxf(mx, sc[j] * mul);
+      mx = fmaxf(fmaxf(mx, xor32(mx)), m);
+      const float f = fast_exp2(m - (mx == kNegInf ? 0.f : mx));
+      l *= f;
+#pragma unroll
+      for (int ct = 0; ct < 4; ++ct) acc[ct] *= f;
+      m = mx;
+      sum = exps();
+    }
+    l += sum;
+    // 16 lanes of a transposing read take 4 keys of 16 channels: lane i brings 4 channels of key i / 4
+    const lds_u8* const vt = (const lds_u8*)vs;
+    const int i = lane & 15, vrow = 32 * u + 4 * hh + (i >> 2);
+    const int vcol = 32 * ((lane >> 4) & 1) + 8 * (i & 3);  // bytes from the 32 channels' first
+#pragma unroll
+    for (int mm = 0; mm < 2; ++mm)
+#pragma unroll
+      for (int ct = 0; ct < 4; ++ct) {
+        u32x4 va;
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          const int row = 16 * mm + 8 * w + vrow;  // row % 4 = i / 4
+          const int at = row * 256 + ((64 * ct + vcol) ^ ((i >> 2) << 6));
+          const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(vt + at)));
+          va[2 * w] = x[0];
+          va[2 * w + 1] = x[1];
+        }
+        acc[ct] = T::mfma32(va, pb[mm], acc[ct]);
+      }
+  }
+
+  // The V rows taken out of the products: every lane scores its own query against the key again, and adds the
+  // row if it sees it.
+  __device__ __forceinline__ void add_bad(const Lds& s, const PreArgs& a, const uint8_t* k, const uint8_t* v, const u32x4 (&q)[8],
+                                          float scale, int key0, int p, int kv_len) {
+    const int hh = (threadIdx.x & 63) >> 5;
+    for (int w = 0; w < 2; ++w)
+      for (uint32_t left = s.bad[w]; left; left &= left - 1) {
+        const int key = key0 + 32 * w + __builtin_ctz(left);
+        if (key >= kv_len) break;
+        const uint8_t* kr = k + key * a.kss;
+        float d = 0.f;
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) {
+          const u32x4 x = *(const u32x4*)(kr + (16 * kk + 8 * hh) * 2);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            d = fmaf(T::to_f((uint16_t)q[kk][e]), T::to_f((uint16_t)x[e]), d);
+            d = fmaf(T::to_f((uint16_t)(q[kk][e] >> 16)), T::to_f((uint16_t)(x[e] >> 16)), d);
+          }
+        }
+        d += xor32(d);
+        if (sees(p, key, a.window, a.sinks)) {
+          const float e = fast_exp2(fmaf(d, scale, -(m == kNegInf ? 0.f : m)));
+#pragma unroll
+          for (int ct = 0; ct < 4; ++ct)
+#pragma unroll
+            for (int j = 0; j < 16; j += 4) {
+              const u32x2 x = *(const u32x2*)(v + key * a.vss + (32 * ct + 2 * j + 4 * hh) * 2);
+              acc[ct][j] += e * T::to_f((uint16_t)x[0]);
+              acc[ct][j + 1] += e * T::to_f((uint16_t)(x[0] >> 16));
+              acc[ct][j + 2] += e * T::to_f((uint16_t)x[1]);
+              acc[ct][j + 3] += e * T::to_f((uint16_t)(x[1] >> 16));
+            }
+        }
+      }
+  }
 
   template <bool ROBUST>
   __device__ __forceinline__ void attend(Lds& s, const PreArgs& a, const Row& r, const u32x4 (&q)[8], float scale,
                                          const KeyTiles& kt, int t0, int t1) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int ql = lane & 31, hh = lane >> 5;
     const uint8_t* k = a.k + r.b * a.ksb + (r.h / a.rep) * a.ksh;
     const uint8_t* v = a.v + r.b * a.vsb + (r.h / a.rep) * a.vsh;
-    const int i = r.i0 + 32 * wave + ql;
+    const TileLoad<false> load_k(k, a.kss, r.kv_len);
+    const TileLoad<true> load_v(v, a.vss, r.kv_len);
+    const int i0 = r.i0 + 32 * wave, i = i0 + (lane & 31);
     const int p = i < r.q_len ? r.off + i : -1;  // this lane's position; -1 sees nothing
-    const int pw0 = r.off + r.i0 + 32 * wave, pw1 = r.off + min(r.i0 + 32 * wave + 31, r.q_len - 1);
+    const int pw0 = r.off + i0, pw1 = r.off + min(i0 + 31, r.q_len - 1);
 #pragma unroll
     for (int ct = 0; ct < 4; ++ct)
 #pragma unroll
@@ -192,143 +289,45 @@ struct Prefill {
     l = 0.f;
     seen = false;
     if (t0 >= t1) return;
-    if (ROBUST) {
-      __syncthreads();
-      if (threadIdx.x < 2) s.bad[threadIdx.x] = 0;
-      __syncthreads();
+    __syncthreads();  // a first run's reads
+    if constexpr (!ROBUST) {
+      load_k(kt.key(t0), s.k[0]);
+      load_v(kt.key(t0), s.v[0]);
     }
-    load(k, v, a, kt.key(t0), r.kv_len);
-    store<ROBUST>(s, 0);
-    __syncthreads();
     for (int t = t0; t < t1; ++t) {
       const int buf = ROBUST ? 0 : (t - t0) & 1, key0 = kt.key(t);
-      const bool more = t + 1 < t1;
-      if (more) load(k, v, a, kt.key(t + 1), r.kv_len);
-      // what this wave's queries see of the tile: all, some, or nothing
-      const bool none = pw1 < key0 || pw1 < pw0 ||
-                        (a.window > 0 && key0 + kBN - 1 <= pw0 - a.window && key0 >= a.sinks);
-      const bool full = key0 + kBN - 1 <= pw0 && r.i0 + 32 * wave + 31 < r.q_len &&
-                        (a.window <= 0 || key0 > pw1 - a.window || key0 + kBN <= a.sinks);
-      if (!none) {
-        float16v sc[2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-#pragma unroll
-          for (int j = 0; j < 16; ++j) sc[u][j] = 0.f;
-          const int row = 32 * u + ql;
-#pragma unroll
-          for (int kk = 0; kk < 8; ++kk)
-            sc[u] = T::mfma32(s.k[buf][row * 16 + ((2 * kk + hh) ^ (row & 15))], q[kk], sc[u]);
-        }
-        float mul = scale;
-        if (!full) {
-          mul = 1.f;
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              const int key = key0 + 32 * u + 8 * (j >> 2) + 4 * hh + (j & 3);
-              const bool vis = sees(p, key, a.window, a.sinks);
-              seen |= vis;
-              sc[u][j] = vis ? sc[u][j] * scale : kNegInf;
-            }
-        } else {
-          seen = true;
-        }
-        u32x4 pb[2][2];
-        auto exps = [&]() {
-          const float mm = -(m == kNegInf ? 0.f : m);
-          uint32_t top = 0;
-          float sum = 0.f;
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int j = 0; j < 16; j += 2) {
-              const float e0 = fast_exp2(fmaf(sc[u][j], mul, mm)), e1 = fast_exp2(fmaf(sc[u][j + 1], mul, mm));
-              sum += e0 + e1;
-              const uint32_t w = T::pack(e0, e1);
-              pb[u][j >> 3][(j >> 1) & 3] = w;
-              top = pk_max_u16(top, w);
-            }
-          l += sum;
-          return max(top & 0xFFFFu, top >> 16);
-        };
-        // 64 as a 16-bit value: P's bits order as its values, which are not negative
-        const uint32_t limit = T::pack(64.f, 0.f);
-        const float l0 = l;
-        const uint32_t top = exps();
-        if (__any(top > limit || m == kNegInf)) {
-          // the maximum moves: rescale, and take the exponentials again
-          l = l0;
-          float mx = kNegInf;
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int j = 0; j < 16; ++j) mx = fmaxf(mx, sc[u][j] * mul);
-          mx = fmaxf(fmaxf(mx, xor32(mx)), m);
-          const float f = fast_exp2(m - (mx == kNegInf ? 0.f : mx));
-          l *= f;
-#pragma unroll
-          for (int ct = 0; ct < 4; ++ct) acc[ct] *= f;
-          m = mx;
-          exps();
-        }
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int mm = 0; mm < 2; ++mm)
-#pragma unroll
-            for (int ct = 0; ct < 4; ++ct) {
-              const int ch = 32 * ct + ql;
-              acc[ct] = T::mfma32(s.v[buf][ch * 8 + ((4 * u + 2 * mm + hh) ^ vswz(ch))], pb[u][mm], acc[ct]);
-            }
-        if constexpr (ROBUST) {
-          for (int w = 0; w < 2; ++w)
-            for (uint32_t left = s.bad[w]; left; left &= left - 1) {
-              const int kl = 32 * w + __builtin_ctz(left), key = key0 + kl;
-              // every lane makes the products of its own query's scores again, for this key
-              const uint8_t* kr = k + key * a.kss;
-              float d = 0.f;
-              for (int kk = 0; kk < 8; ++kk)
-                for (int e = 0; e < 8; ++e) {
-                  const uint16_t kb = *(const uint16_t*)(kr + (16 * kk + 8 * hh + e) * 2);
-                  uint32_t qb = 0;
-#pragma unroll
-                  for (int z = 0; z < 8; ++z)
-                    if (z == kk) qb = e & 1 ? q[z][e >> 1] >> 16 : q[z][e >> 1] & 0xFFFFu;
-                  d = fmaf(T::to_f((uint16_t)qb), T::to_f(kb), d);
-                }
-              d += xor32(d);
-              if (sees(p, key, a.window, a.sinks)) {
-                const float e = fast_exp2(fmaf(d, scale, -(m == kNegInf ? 0.f : m)));
-                for (int ct = 0; ct < 4; ++ct)
-#pragma unroll
-                  for (int j = 0; j < 16; ++j) {
-                    const int ch = 32 * ct + 8 * (j >> 2) + 4 * hh + (j & 3);
-                    const float x = e * T::to_f(*(const uint16_t*)(v + key * a.vss + ch * 2));
-#pragma unroll
-                    for (int z = 0; z < 4; ++z)
-                      if (z == ct) acc[z][j] += x;
-                  }
-              }
-            }
-        }
-      }
       if constexpr (ROBUST) {
-        __syncthreads();
         if (threadIdx.x < 2) s.bad[threadIdx.x] = 0;
         __syncthreads();
+        load_k(key0, s.k[0]);
+        load_v_finite(v, a.vss, key0, r.kv_len, s);
       }
-      if (more) store<ROBUST>(s, ROBUST ? 0 : buf ^ 1);
-      __syncthreads();
+      __syncthreads();  // waits for the tile's loads
+      if (!ROBUST && t + 1 < t1) {
+        load_k(kt.key(t + 1), s.k[buf ^ 1]);
+        load_v(kt.key(t + 1), s.v[buf ^ 1]);
+      }
+      // what this wave's queries see of the tile: nothing, all, or some
+      const bool none = pw1 < key0 || pw1 < pw0 ||
+                        (a.window > 0 && key0 + kBN - 1 <= pw0 - a.window && key0 >= a.sinks);
+      const bool full = key0 + kBN - 1 <= pw0 && i0 + 31 < r.q_len &&
+                        (a.window <= 0 || key0 > pw1 - a.window || key0 + kBN <= a.sinks);
+      if (!none) {
+        seen |= full;
+#pragma unroll 2
+        for (int u = 0; u < 2; ++u) half_tile(s.k[buf], s.v[buf], a, q, scale, key0, u, p, full);
+        if constexpr (ROBUST) add_bad(s, a, k, v, q, scale, key0, p, r.kv_len);
+      }
+      if constexpr (ROBUST) __syncthreads();
     }
+    __syncthreads();  // the buffers are free
   }
 };
 
 // One unit: its queries over its keys, and the output or the split's part.  Returns whether the result is
 // not finite (and then has written nothing), or false.
 template <class T, bool ROBUST>
-__device__ __forceinline__ bool attend_unit(typename Prefill<T>::Lds& s, const PreArgs& a, int64_t unit) {
+__device__ __forceinline__ bool attend_unit(Lds& s, const PreArgs& a, int64_t unit) {
   const Row r = unit_of(a, unit);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ql = lane & 31, hh = lane >> 5;
@@ -397,13 +396,13 @@ __device__ __forceinline__ bool attend_unit(typename Prefill<T>::Lds& s, const P
 
 // the rare second run, kept out of the kernel's own register allocation
 template <class T>
-__device__ __attribute__((noinline)) void attend_again(typename Prefill<T>::Lds* s, const PreArgs* a, int64_t unit) {
+__device__ __attribute__((noinline)) void attend_again(Lds* s, const PreArgs* a, int64_t unit) {
   attend_unit<T, true>(*s, *a, unit);
 }
 
 template <class T>
 __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(PreArgs a) {
-  __shared__ typename Prefill<T>::Lds s;
+  __shared__ Lds s;
   // work-groups go round the 8 XCDs: each XCD gets a run of units, whose heads share K and V in its L2
   const int64_t per = (a.units + 7) / 8;
   const int64_t unit = (int64_t)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
