@@ -14,14 +14,16 @@ int fail(int code, const std::string& msg);
 
 typedef __bf16 bf16_t;
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float float2v __attribute__((ext_vector_type(2)));
 typedef float float16v __attribute__((ext_vector_type(16)));
 
-// 16-bit element types: conversions round to nearest even
+// 16-bit element types: conversions round to nearest even (two values a v_cvt_pk)
 struct TF16 {
   using elem = half_t;
   __device__ __forceinline__ static float to_f(uint16_t b) { return (float)__builtin_bit_cast(half_t, b); }
   __device__ __forceinline__ static uint32_t pack(float a, float b) {
-    return (uint32_t)__builtin_bit_cast(uint16_t, (half_t)a) | ((uint32_t)__builtin_bit_cast(uint16_t, (half_t)b) << 16);
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((float2v{a, b}), half2v));
   }
   __device__ __forceinline__ static float4v mfma16(u32x4 a, u32x4 b, float4v c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8v, a), __builtin_bit_cast(half8v, b), c, 0, 0, 0);
@@ -34,7 +36,7 @@ struct TB16 {
   using elem = bf16_t;
   __device__ __forceinline__ static float to_f(uint16_t b) { return __builtin_bit_cast(float, (uint32_t)b << 16); }
   __device__ __forceinline__ static uint32_t pack(float a, float b) {
-    return (uint32_t)__builtin_bit_cast(uint16_t, (bf16_t)a) | ((uint32_t)__builtin_bit_cast(uint16_t, (bf16_t)b) << 16);
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((float2v{a, b}), bf16x2));
   }
   __device__ __forceinline__ static float4v mfma16(u32x4 a, u32x4 b, float4v c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);

@@ -71,17 +71,18 @@ struct Row {
   int b, h, block, split, q_len, kv_len, off, i0;
 };
 
-__device__ __forceinline__ Row unit_of(const PreArgs& a, int64_t unit) {
+__device__ __forceinline__ Row unit_of(const PreArgs& a, int64_t unit64) {
   Row r;
-  r.split = (int)(unit % a.splits);
-  unit /= a.splits;
+  uint32_t unit = (uint32_t)unit64;  // fewer than 2^31 of them
+  r.split = (int)(unit % (uint32_t)a.splits);
+  unit /= (uint32_t)a.splits;
   // blocks from both ends in turn: any run of units has its share of the long ones (the later queries') and
   // the short ones; rows of a batch in turn for the same reason
-  const int x = (int)(unit % a.blocks);
+  const int x = (int)(unit % (uint32_t)a.blocks);
   r.block = x & 1 ? x >> 1 : a.blocks - 1 - (x >> 1);
-  unit /= a.blocks;
-  r.b = (int)(unit % a.batch);
-  r.h = (int)(unit / a.batch);
+  unit /= (uint32_t)a.blocks;
+  r.b = (int)(unit % (uint32_t)a.batch);
+  r.h = (int)(unit / (uint32_t)a.batch);
   r.q_len = a.q_lens ? min(max(a.q_lens[r.b], 0), a.S) : a.S;
   r.kv_len = a.kv_lens ? min(max(a.kv_lens[r.b], 0), a.T) : a.T;
   r.off = r.kv_len - r.q_len;
@@ -93,10 +94,13 @@ __device__ __forceinline__ bool sees(int p, int key, int window, int sinks) {
   return key <= p && (window <= 0 || key > p - window || key < sinks);
 }
 __device__ __forceinline__ float xor32(float x) { return __shfl_xor(x, 32, 64); }
+// A tile in LDS.  K: [key][16 chunks of 8 channels], chunk ^ (key % 16); V: the same, chunk ^ 4 (key % 4).
+typedef u32x4 LdsTile[kBN * 16];
+// The buffers are variables of their own, and the loop is written out for both: only so does the compiler know
+// that the operands' reads of one need not wait for the loads into the other.
 struct Lds {
-  u32x4 k[2][kBN * 16];  // [key][16 chunks of 8 channels], chunk ^ (key % 16)
-  u32x4 v[2][kBN * 16];  // [key][16 chunks of 8 channels], chunk ^ 4 (key % 4)
-  uint32_t bad[2];       // keys of the tile whose V row is not finite
+  LdsTile &k0, &v0, &k1, &v1;
+  uint32_t (&bad)[2];  // keys of the tile whose V row is not finite
 };
 
 typedef __attribute__((address_space(3))) uint8_t lds_u8;
@@ -142,7 +146,7 @@ struct Prefill {
   bool seen;
 
   // V of the second run: rows with an Inf or NaN as zeros, their keys marked
-  static __device__ __forceinline__ void load_v_finite(const uint8_t* x, int64_t stride, int key0, int kv_len, Lds& s) {
+  static __device__ __forceinline__ void load_v_finite(const uint8_t* x, int64_t stride, int key0, int kv_len, const Lds& s) {
     const int t = threadIdx.x;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
@@ -157,48 +161,77 @@ struct Prefill {
         w = u32x4{0, 0, 0, 0};
         if ((t & 15) == 0) atomicOr(&s.bad[row >> 5], 1u << (row & 31));
       }
-      s.v[0][row * 16 + ((t & 15) ^ ((row & 3) << 2))] = w;
+      s.v0[row * 16 + ((t & 15) ^ ((row & 3) << 2))] = w;
     }
   }
 
-  // The products of this wave's 32 queries with 32 keys of a tile, those from 32 u on.
-  __device__ __forceinline__ void half_tile(const u32x4* ks, const u32x4* vs, const PreArgs& a, const u32x4 (&q)[8], float scale,
-                                            int key0, int u, int p, bool full) {
+  // K's operands of keys 32 u .. of the tile.
+  static __device__ __forceinline__ void read_k(const LdsTile& ks, int u, u32x4 (&kf)[8]) {
     const int lane = threadIdx.x & 63, ql = lane & 31, hh = lane >> 5;
+#pragma unroll
+    for (int kk = 0; kk < 8; ++kk) kf[kk] = ks[(32 * u + ql) * 16 + ((2 * kk + hh) ^ (ql & 15))];
+  }
+
+  // V^T's operands of keys 32 u + 16 mm .., channels 32 ct .., in vf[4 mm + ct].  16 lanes of a transposing read
+  // take 4 keys of 16 channels: lane i brings 4 channels of key i / 4.
+  static __device__ __forceinline__ void read_v(const LdsTile& vs, int u, u32x4 (&vf)[8]) {
+    const int lane = threadIdx.x & 63, hh = lane >> 5, i = lane & 15;
+    const lds_u8* const vt = (const lds_u8*)&vs[0];
+    const int vrow = 32 * u + 4 * hh + (i >> 2);
+    const int vcol = 32 * ((lane >> 4) & 1) + 8 * (i & 3);  // bytes from the 32 channels' first
+#pragma unroll
+    for (int mm = 0; mm < 2; ++mm)
+#pragma unroll
+      for (int ct = 0; ct < 4; ++ct)
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          const int row = 16 * mm + 8 * w + vrow;  // row % 4 = i / 4
+          const int at = row * 256 + ((64 * ct + vcol) ^ ((i >> 2) << 6));
+          const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(vt + at)));
+          vf[4 * mm + ct][2 * w] = x[0];
+          vf[4 * mm + ct][2 * w + 1] = x[1];
+        }
+  }
+
+  static __device__ __forceinline__ float16v scores(const u32x4 (&kf)[8], const u32x4 (&q)[8]) {
     float16v sc;
 #pragma unroll
     for (int j = 0; j < 16; ++j) sc[j] = 0.f;
 #pragma unroll
-    for (int kk = 0; kk < 8; ++kk) sc = T::mfma32(ks[(32 * u + ql) * 16 + ((2 * kk + hh) ^ (ql & 15))], q[kk], sc);
-    float mul = scale;
-    if (!full) {
-      mul = 1.f;
-      // key = first + c, c < 32 a constant: c against this lane's last key, first key and end of the sinks
-      const int first = key0 + 32 * u + 4 * hh;
-      const int last = p - first, from = a.window > 0 ? p - a.window - first : -1, sink = a.sinks - first;
+    for (int kk = 0; kk < 8; ++kk) sc = T::mfma32(kf[kk], q[kk], sc);
+    return sc;
+  }
+
+  // Scaled scores with -inf where this lane's query does not see the key.
+  __device__ __forceinline__ void mask(float16v& sc, const PreArgs& a, float scale, int key0, int u, int p) {
+    // key = first + c, c < 32 a constant: c against this lane's last key, first key and end of the sinks
+    const int first = key0 + 32 * u + 4 * ((threadIdx.x & 63) >> 5);
+    const int last = p - first, from = a.window > 0 ? p - a.window - first : -1, sink = a.sinks - first;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const int c = 8 * (j >> 2) + (j & 3);
-        const bool vis = (c <= last) & ((c > from) | (c < sink));
-        seen |= vis;
-        sc[j] = vis ? sc[j] * scale : kNegInf;
-      }
+    for (int j = 0; j < 16; ++j) {
+      const int c = 8 * (j >> 2) + (j & 3);
+      const bool vis = (c <= last) & ((c > from) | (c < sink));
+      seen |= vis;
+      sc[j] = vis ? sc[j] * scale : kNegInf;
     }
-    u32x4 pb[2];
-    auto exps = [&]() {
-      const float mm = -(m == kNegInf ? 0.f : m);
-      float s0 = 0.f, s1 = 0.f;
+  }
+
+  // P of 32 keys, in 16 bits, from the scores times mul; returns this lane's sum of it.
+  __device__ __forceinline__ float exps(const float16v& sc, float mul, u32x4 (&pb)[2]) const {
+    const float mm = -(m == kNegInf ? 0.f : m);
+    float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-      for (int j = 0; j < 16; j += 2) {
-        const float e0 = fast_exp2(fmaf(sc[j], mul, mm)), e1 = fast_exp2(fmaf(sc[j + 1], mul, mm));
-        s0 += e0;
-        s1 += e1;
-        pb[j >> 3][(j >> 1) & 3] = T::pack(e0, e1);
-      }
-      return s0 + s1;
-    };
-    // while a lane's sum stays below 64 so does each of its P: the maximum follows only where it does not
-    float sum = exps();
+    for (int j = 0; j < 16; j += 2) {
+      const float e0 = fast_exp2(fmaf(sc[j], mul, mm)), e1 = fast_exp2(fmaf(sc[j + 1], mul, mm));
+      s0 += e0;
+      s1 += e1;
+      pb[j >> 3][(j >> 1) & 3] = T::pack(e0, e1);
+    }
+    return s0 + s1;
+  }
+
+  // While a lane's sum stays below 64 so does each of its P: the maximum follows only where it does not.
+  __device__ __forceinline__ void add_sum(float sum, const float16v& sc, float mul, u32x4 (&pb)[2]) {
     if (__any(!(sum <= 64.f) || m == kNegInf)) {
       float mx = kNegInf;
 #pragma unroll
@@ -209,28 +242,39 @@ struct Prefill {
 #pragma unroll
       for (int ct = 0; ct < 4; ++ct) acc[ct] *= f;
       m = mx;
-      sum = exps();
+      sum = exps(sc, mul, pb);
     }
     l += sum;
-    // 16 lanes of a transposing read take 4 keys of 16 channels: lane i brings 4 channels of key i / 4
-    const lds_u8* const vt = (const lds_u8*)vs;
-    const int i = lane & 15, vrow = 32 * u + 4 * hh + (i >> 2);
-    const int vcol = 32 * ((lane >> 4) & 1) + 8 * (i & 3);  // bytes from the 32 channels' first
+  }
+
+  __device__ __forceinline__ void add_values(const u32x4 (&vf)[8], const u32x4 (&pb)[2]) {
 #pragma unroll
     for (int mm = 0; mm < 2; ++mm)
 #pragma unroll
-      for (int ct = 0; ct < 4; ++ct) {
-        u32x4 va;
+      for (int ct = 0; ct < 4; ++ct) acc[ct] = T::mfma32(vf[4 * mm + ct], pb[mm], acc[ct]);
+  }
+
+  // A tile's products, 32 keys at a time.  Operands are read from LDS a step before they are used: V's under
+  // the exponentials, the second half's K under the first half's product with V (the scheduling barriers keep
+  // the compiler from moving the reads to their uses).
+  __device__ __forceinline__ void tile(const LdsTile& ks, const LdsTile& vs, const PreArgs& a, const u32x4 (&q)[8], float scale,
+                                       int key0, int p, bool full) {
+    const float mul = full ? scale : 1.f;
+    u32x4 kf[8], vf[8], pb[2];
+    read_k(ks, 0, kf);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          const int row = 16 * mm + 8 * w + vrow;  // row % 4 = i / 4
-          const int at = row * 256 + ((64 * ct + vcol) ^ ((i >> 2) << 6));
-          const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(vt + at)));
-          va[2 * w] = x[0];
-          va[2 * w + 1] = x[1];
-        }
-        acc[ct] = T::mfma32(va, pb[mm], acc[ct]);
-      }
+    for (int u = 0; u < 2; ++u) {
+      float16v sc = scores(kf, q);
+      read_v(vs, u, vf);
+      __builtin_amdgcn_sched_barrier(0);
+      if (!full) mask(sc, a, scale, key0, u, p);
+      add_sum(exps(sc, mul, pb), sc, mul, pb);
+      if (u == 0) read_k(ks, 1, kf);
+      __builtin_amdgcn_sched_barrier(0);
+      add_values(vf, pb);
+    }
+    seen |= full;
   }
 
   // The V rows taken out of the products: every lane scores its own query against the key again, and adds the
@@ -271,7 +315,7 @@ struct Prefill {
   }
 
   template <bool ROBUST>
-  __device__ __forceinline__ void attend(Lds& s, const PreArgs& a, const Row& r, const u32x4 (&q)[8], float scale,
+  __device__ __forceinline__ void attend(const Lds& s, const PreArgs& a, const Row& r, const u32x4 (&q)[8], float scale,
                                          const KeyTiles& kt, int t0, int t1) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint8_t* k = a.k + r.b * a.ksb + (r.h / a.rep) * a.ksh;
@@ -289,36 +333,51 @@ struct Prefill {
     l = 0.f;
     seen = false;
     if (t0 >= t1) return;
-    __syncthreads();  // a first run's reads
-    if constexpr (!ROBUST) {
-      load_k(kt.key(t0), s.k[0]);
-      load_v(kt.key(t0), s.v[0]);
-    }
-    for (int t = t0; t < t1; ++t) {
-      const int buf = ROBUST ? 0 : (t - t0) & 1, key0 = kt.key(t);
-      if constexpr (ROBUST) {
-        if (threadIdx.x < 2) s.bad[threadIdx.x] = 0;
-        __syncthreads();
-        load_k(key0, s.k[0]);
-        load_v_finite(v, a.vss, key0, r.kv_len, s);
-      }
-      __syncthreads();  // waits for the tile's loads
-      if (!ROBUST && t + 1 < t1) {
-        load_k(kt.key(t + 1), s.k[buf ^ 1]);
-        load_v(kt.key(t + 1), s.v[buf ^ 1]);
-      }
-      // what this wave's queries see of the tile: nothing, all, or some
+    // what this wave's queries see of a tile: nothing, all, or some
+    auto products = [&](const LdsTile& kc, const LdsTile& vc, int key0) {
       const bool none = pw1 < key0 || pw1 < pw0 ||
                         (a.window > 0 && key0 + kBN - 1 <= pw0 - a.window && key0 >= a.sinks);
       const bool full = key0 + kBN - 1 <= pw0 && i0 + 31 < r.q_len &&
                         (a.window <= 0 || key0 > pw1 - a.window || key0 + kBN <= a.sinks);
-      if (!none) {
-        seen |= full;
-#pragma unroll 2
-        for (int u = 0; u < 2; ++u) half_tile(s.k[buf], s.v[buf], a, q, scale, key0, u, p, full);
-        if constexpr (ROBUST) add_bad(s, a, k, v, q, scale, key0, p, r.kv_len);
+      if (none) return;
+      tile(kc, vc, a, q, scale, key0, p, full);
+      if constexpr (ROBUST) add_bad(s, a, k, v, q, scale, key0, p, r.kv_len);
+    };
+    // this wave's loads have arrived, and then every wave's; the other buffer is free
+    auto arrived = [&]() {
+      __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+      __syncthreads();
+    };
+    __syncthreads();  // a first run's reads
+    if constexpr (ROBUST) {
+      for (int t = t0; t < t1; ++t) {
+        const int key0 = kt.key(t);
+        if (threadIdx.x < 2) s.bad[threadIdx.x] = 0;
+        __syncthreads();
+        load_k(key0, s.k0);
+        load_v_finite(v, a.vss, key0, r.kv_len, s);
+        arrived();
+        products(s.k0, s.v0, key0);
+        __syncthreads();
       }
-      if constexpr (ROBUST) __syncthreads();
+    } else {
+      load_k(kt.key(t0), s.k0);
+      load_v(kt.key(t0), s.v0);
+      for (int t = t0; t < t1; t += 2) {
+        arrived();
+        if (t + 1 < t1) {
+          load_k(kt.key(t + 1), s.k1);
+          load_v(kt.key(t + 1), s.v1);
+        }
+        products(s.k0, s.v0, kt.key(t));
+        if (t + 1 == t1) break;
+        arrived();
+        if (t + 2 < t1) {
+          load_k(kt.key(t + 2), s.k0);
+          load_v(kt.key(t + 2), s.v0);
+        }
+        products(s.k1, s.v1, kt.key(t + 1));
+      }
     }
     __syncthreads();  // the buffers are free
   }
@@ -327,13 +386,13 @@ struct Prefill {
 // One unit: its queries over its keys, and the output or the split's part.  Returns whether the result is
 // not finite (and then has written nothing), or false.
 template <class T, bool ROBUST>
-__device__ __forceinline__ bool attend_unit(Lds& s, const PreArgs& a, int64_t unit) {
+__device__ __forceinline__ bool attend_unit(const Lds& s, const PreArgs& a, int64_t unit) {
   const Row r = unit_of(a, unit);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ql = lane & 31, hh = lane >> 5;
   const int last = min(r.i0 + kBM, r.q_len) - 1;
   const KeyTiles kt(r.off + r.i0, last < r.i0 ? -1 : r.off + last, a.window, a.sinks);
-  const int t0 = (int)((int64_t)kt.count * r.split / a.splits), t1 = (int)((int64_t)kt.count * (r.split + 1) / a.splits);
+  const int t0 = kt.count * r.split / a.splits, t1 = kt.count * (r.split + 1) / a.splits;  // at most 2^24 tiles, 32 splits
 
   u32x4 q[8];
   {
@@ -373,14 +432,14 @@ __device__ __forceinline__ bool attend_unit(Lds& s, const PreArgs& a, int64_t un
   }
   // the maximum is -inf where nothing was seen (0), or where all that was seen scored -inf (NaN)
   const float inv = f.m == kNegInf && l == l ? (seen ? __builtin_nanf("") : 0.f) : 1.0f / l;
-  // through LDS for whole rows: [query][16 chunks], chunk ^ (query % 16); K's buffers are free
-  u32x2* const o = (u32x2*)&s.k[0][0];
+  // through LDS for whole rows: [query][16 chunks], chunk ^ (query % 16)
+  u32x2* const o = (u32x2*)(wave < 2 ? s.k0 : s.k1);
 #pragma unroll
   for (int ct = 0; ct < 4; ++ct)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int chunk = 4 * ct + e;  // 8 channels, this lane's half of them
-      o[(row * 16 + (chunk ^ (row & 15))) * 2 + hh] =
+      o[((row & 63) * 16 + (chunk ^ (row & 15))) * 2 + hh] =
           u32x2{T::pack(f.acc[ct][4 * e] * inv, f.acc[ct][4 * e + 1] * inv), T::pack(f.acc[ct][4 * e + 2] * inv, f.acc[ct][4 * e + 3] * inv)};
     }
   __syncthreads();
@@ -389,20 +448,22 @@ __device__ __forceinline__ bool attend_unit(Lds& s, const PreArgs& a, int64_t un
   for (int u = 0; u < 8; ++u) {
     const int x = (t >> 4) + 16 * u, i = r.i0 + x;
     if (i < a.S)
-      *(u32x4*)(a.out + r.b * a.osb + r.h * a.osh + i * a.oss + (t & 15) * 16) = ((const u32x4*)o)[x * 16 + ((t & 15) ^ (x & 15))];
+      *(u32x4*)(a.out + r.b * a.osb + r.h * a.osh + i * a.oss + (t & 15) * 16) = (u < 4 ? s.k0 : s.k1)[(x & 63) * 16 + ((t & 15) ^ (x & 15))];
   }
   return false;
 }
 
 // the rare second run, kept out of the kernel's own register allocation
 template <class T>
-__device__ __attribute__((noinline)) void attend_again(Lds* s, const PreArgs* a, int64_t unit) {
+__device__ __attribute__((noinline)) void attend_again(const Lds* s, const PreArgs* a, int64_t unit) {
   attend_unit<T, true>(*s, *a, unit);
 }
 
 template <class T>
 __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(PreArgs a) {
-  __shared__ Lds s;
+  __shared__ LdsTile k0, v0, k1, v1;
+  __shared__ uint32_t bad[2];
+  const Lds s{k0, v0, k1, v1, bad};
   // work-groups go round the 8 XCDs: each XCD gets a run of units, whose heads share K and V in its L2
   const int64_t per = (a.units + 7) / 8;
   const int64_t unit = (int64_t)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
