@@ -524,6 +524,8 @@ def test_evict_protected(budget, sinks, recent):
 def test_evict_long_rows():
     run_evict([5000, 700, 3001], 2, 16, F16, 0, 2100, 4, 100)
     run_evict([9000], 1, 64, BF16, 32, 4000, 0, 0)
+    run_evict([32768, 20000], 1, 256, BF16, 128, 3000, 4, 100)
+    run_evict([40000, 3001], 1, 256, F16, 128, 5000, 4, 100)  # more weights than a work-group's registers hold
 
 
 def test_evict_ties_and_special_weights():
