@@ -72,14 +72,16 @@ __device__ __forceinline__ int row_len(const DecArgs& a, int b) {
   return (int)min((int64_t)max(a.lens[b], 0), cap);
 }
 
-// pre[0..B] = tiles before each row; every thread of the work-group calls it
+// pre[0..B] = tiles before each row, len[0..B-1] their tokens; every thread of the work-group calls it
 template <int THREADS>
-__device__ void scan_rows(const DecArgs& a, int* pre, int* wsum) {
+__device__ void scan_rows(const DecArgs& a, int* pre, int* len, int* wsum) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int base = 0;
   for (int b0 = 0; b0 < a.c.batch; b0 += THREADS) {
     const int b = b0 + tid;
-    int x = b < a.c.batch ? RowTiles(row_len(a, b), a.window, a.sinks).count : 0;
+    const int n = b < a.c.batch ? row_len(a, b) : 0;
+    if (b < a.c.batch) len[b] = n;
+    int x = RowTiles(n, a.window, a.sinks).count;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
       const int y = __shfl_up(x, o, 64);
@@ -148,7 +150,7 @@ struct Tile<true> {
 };
 
 template <class T, bool I8, int GS, bool WT, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) void paged_decode_kernel(DecArgs a) {
+__global__ __launch_bounds__(WAVES * 64, 2) void paged_decode_kernel(DecArgs a) {
   using M = typename std::conditional<I8, TF16, T>::type;  // the matrix instructions' type
   constexpr int G = I8 ? 128 / GS : 1;
   extern __shared__ char lds[];
@@ -156,12 +158,13 @@ __global__ __launch_bounds__(WAVES * 64) void paged_decode_kernel(DecArgs a) {
   __shared__ float2 wml[WAVES][kHeads];
   float* const wacc = (float*)lds;                     // [4][32][64]
   int* const pre = (int*)(lds + 4 * 32 * 64 * 4);      // [batch + 1]
+  int* const len = pre + a.c.batch + 1;                // [batch]
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 15, g = lane >> 4;
   const int h = blockIdx.y, rep = a.rep;
   const PagedCache& pc = a.c;
 
-  scan_rows<WAVES * 64>(a, pre, wsum);
+  scan_rows<WAVES * 64>(a, pre, len, wsum);
   const int total = pre[pc.batch], per = tiles_each(a, total);
   if ((WT || !a.solo) && blockIdx.x == 0 && h == 0) {
     for (int b = tid; b <= pc.batch; b += WAVES * 64) a.pre[b] = pre[b];
@@ -196,7 +199,7 @@ __global__ __launch_bounds__(WAVES * 64) void paged_decode_kernel(DecArgs a) {
     const int rs = __builtin_amdgcn_readfirstlane(pre[row]), re = __builtin_amdgcn_readfirstlane(pre[row + 1]);
     if (re == rs) continue;
     const int end = min(t1, re);
-    const int n = __builtin_amdgcn_readfirstlane(row_len(a, row));
+    const int n = __builtin_amdgcn_readfirstlane(len[row]);
     const RowTiles rt(n, a.window, a.sinks);
     const const_i32 tab = (const_i32)(pc.table + row * pc.table_stride);
 
@@ -210,29 +213,6 @@ __global__ __launch_bounds__(WAVES * 64) void paged_decode_kernel(DecArgs a) {
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk)
         q[kk] = *(const u32x4*)(qp + (I8 && GS >= 64 ? 64 * (kk >> 1) + 16 * g + 8 * (kk & 1) : 32 * kk + 8 * g));
-      if constexpr (I8 && std::is_same<T, TB16>::value) {
-        // bf16 values in fp16: exact once the head's largest is scaled to [1, 2) by a power of two (what
-        // lies 2^24 and more below it loses bits that are below the sum's)
-        float top = 0.f;
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            top = fmaxf(top, fmaxf(fabsf(TB16::to_f((uint16_t)q[kk][j])), fabsf(TB16::to_f((uint16_t)(q[kk][j] >> 16)))));
-        top = wave_max_xor_groups(top);
-        int ex = (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127;
-        if (ex == 128 || ex == -127) ex = 0;  // Inf or NaN stays what it is; zero or a subnormal is 0
-        const float f = ldexpf(1.f, -ex);
-        scale = ldexpf(scale, ex);
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            q[kk][j] = TF16::pack(TB16::to_f((uint16_t)q[kk][j]) * f, TB16::to_f((uint16_t)(q[kk][j] >> 16)) * f);
-      }
-      if (c >= rep)
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk) q[kk] = u32x4{0, 0, 0, 0};
     }
     float m = kNegInf, l = 0.f;
     float4v acc[8];
@@ -240,56 +220,117 @@ __global__ __launch_bounds__(WAVES * 64) void paged_decode_kernel(DecArgs a) {
     for (int e = 0; e < 8; ++e) acc[e] = float4v{0, 0, 0, 0};
     bool any = false;
 
+    // A tile's place: its first token, its pages, this lane's rows and scales in them.  The page numbers are
+    // fetched a tile ahead of that, and K and V of a tile while the tile before it is worked on: each operand's
+    // registers are loaded again as soon as its products are done.
+    struct Place {
+      int tok;
+      bool full, bad;  // every token of the tile is seen; the page of this lane's V block is not there
+      const uint8_t *k, *v, *ks, *vs;
+    };
     const int i_end = end - rs;
-    for (int i = t - rs + wave; i < i_end; i += WAVES) {
-      const int tok = __builtin_amdgcn_readfirstlane(rt.token(i));
-      const int idx = tok >> pc.lg;
-      // a tile of 32 slots lies in one page, or in two of 16
-      int p0 = tab[idx], p1 = p0;
-      if (pc.lg == 4) p1 = idx + 1 < pc.max_pages ? tab[idx + 1] : -1;
+    auto page_at = [&](int i, int which) {  // of a tile of 32 slots: in one page, or in two of 16
+      const int idx = (rt.token(min(i, i_end - 1)) >> pc.lg) + which;
+      return idx < pc.max_pages ? tab[idx] : -1;
+    };
+    auto place = [&](int i, int p0, int p1, bool there) {
+      Place w;
+      w.tok = __builtin_amdgcn_readfirstlane(rt.token(i));
+      if (pc.lg != 4) p1 = p0;
       const bool bad0 = (uint32_t)p0 >= (uint32_t)pc.num_pages, bad1 = (uint32_t)p1 >= (uint32_t)pc.num_pages;
-      const bool full = !bad0 && !bad1 && tok + kTile <= n && (tok >= rt.lo || tok + kTile <= rt.sink_end);
+      w.full = !bad0 && !bad1 && w.tok + kTile <= n && (w.tok >= rt.lo || w.tok + kTile <= rt.sink_end);
       if (bad0) p0 = 0;  // read, and masked: page 0 is there
       if (bad1) p1 = 0;
       const int bk = c >> 2;  // this lane's K block of 8 tokens; its V block is g
-      const bool k1 = pc.lg == 4 && bk >= 2, v1 = pc.lg == 4 && g >= 2;
-      const int ko = (tok + 8 * bk + (c & 3)) & pc.page_mask, vo = (tok + 8 * g) & pc.page_mask;
-      const uint8_t* const kp = kh + (k1 ? p1 : p0) * pc.ksp + (uint32_t)ko * (uint32_t)pc.kst;
-      const uint8_t* const vp = vh + (v1 ? p1 : p0) * pc.vsp + (uint32_t)vo * (uint32_t)pc.vst;
-      Tile<I8> x;
-      if constexpr (!I8) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk) x.k[u][kk] = ld_stream<u32x4>(kp + u * 4 * pc.kst + 64 * kk + 16 * g);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x.v[j] = ld_stream<u32x4>(vp + j * pc.vst + 16 * c);
-      } else {
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const uint8_t* kr = kp + u * 4 * pc.kst;
-          if constexpr (GS >= 64) {
-#pragma unroll
-            for (int kk = 0; kk < 4; kk += 2) {
-              const u32x4 w = ld_stream<u32x4>(kr + 32 * kk + 16 * g);
-              x.k[u][kk] = u32x2{w[0], w[1]};
-              x.k[u][kk + 1] = u32x2{w[2], w[3]};
-            }
-          } else {
-#pragma unroll
-            for (int kk = 0; kk < 4; ++kk) x.k[u][kk] = ld_stream<u32x2>(kr + 32 * kk + 8 * g);
-          }
-        }
-        // scales of tokens 8 g .. 8 g + 7: [8][G] fp16, dense
-        const uint8_t* const sk = pc.ks + h * pc.kssh + (v1 ? p1 : p0) * pc.kssp + vo * (2 * G);
-        const uint8_t* const sv = pc.vs + h * pc.vssh + (v1 ? p1 : p0) * pc.vssp + vo * (2 * G);
-#pragma unroll
-        for (int j = 0; j < G; ++j) x.ks[j] = *(const u32x4*)(sk + 16 * j);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x.v[j] = ld_stream<u32x2>(vp + j * pc.vst + 8 * c);
-#pragma unroll
-        for (int j = 0; j < G; ++j) x.vs[j] = *(const u32x4*)(sv + 16 * j);
+      int pk = bk >= 2 ? p1 : p0, pv = g >= 2 ? p1 : p0;
+      int ko = (w.tok + 8 * bk + (c & 3)) & pc.page_mask, vo = (w.tok + 8 * g) & pc.page_mask;
+      if (!there) pk = pv = ko = vo = 0;  // the same few lines for all lanes
+      w.bad = g >= 2 ? bad1 : bad0;
+      w.k = kh + pk * pc.ksp + (uint32_t)ko * (uint32_t)pc.kst;
+      w.v = vh + pv * pc.vsp + (uint32_t)vo * (uint32_t)pc.vst;
+      if constexpr (I8) {  // scales of tokens 8 g .. 8 g + 7: [8][G] fp16, dense
+        w.ks = pc.ks + h * pc.kssh + pv * pc.kssp + vo * (2 * G);
+        w.vs = pc.vs + h * pc.vssh + pv * pc.vssp + vo * (2 * G);
       }
+      return w;
+    };
+    Tile<I8> x;
+    auto load_k = [&](const Place& w) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const uint8_t* kr = w.k + u * 4 * pc.kst;
+        if constexpr (!I8) {
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) x.k[u][kk] = ld_stream<u32x4>(kr + 64 * kk + 16 * g);
+        } else if constexpr (GS >= 64) {
+#pragma unroll
+          for (int kk = 0; kk < 4; kk += 2) {
+            const u32x4 y = ld_stream<u32x4>(kr + 32 * kk + 16 * g);
+            x.k[u][kk] = u32x2{y[0], y[1]};
+            x.k[u][kk + 1] = u32x2{y[2], y[3]};
+          }
+        } else {
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) x.k[u][kk] = ld_stream<u32x2>(kr + 32 * kk + 8 * g);
+        }
+      }
+      if constexpr (I8)
+#pragma unroll
+        for (int j = 0; j < G; ++j) x.ks[j] = *(const u32x4*)(w.ks + 16 * j);
+    };
+    auto load_v = [&](const Place& w) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if constexpr (!I8) x.v[j] = ld_stream<u32x4>(w.v + j * pc.vst + 16 * c);
+        else x.v[j] = ld_stream<u32x2>(w.v + j * pc.vst + 8 * c);
+      }
+      if constexpr (I8)
+#pragma unroll
+        for (int j = 0; j < G; ++j) x.vs[j] = *(const u32x4*)(w.vs + 16 * j);
+    };
+    int i = t - rs + wave;
+    Place w{};
+    int n0 = -1, n1 = -1;  // pages of the tile after this
+    if (i < i_end) {
+      w = place(i, page_at(i, 0), page_at(i, 1), true);
+      load_k(w);
+      __builtin_amdgcn_sched_barrier(0);  // in the loop's order: what waits for K must not wait for V
+      load_v(w);
+      n0 = page_at(i + WAVES, 0);
+      n1 = page_at(i + WAVES, 1);
+    }
+    // Q is waited for here, behind the first tile's loads
+    if constexpr (I8 && std::is_same<T, TB16>::value) {
+      // bf16 values in fp16: exact once the head's largest is scaled to [1, 2) by a power of two (what lies 2^24
+      // and more below it loses bits that are below the sum's)
+      float top = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          top = fmaxf(top, fmaxf(fabsf(TB16::to_f((uint16_t)q[kk][j])), fabsf(TB16::to_f((uint16_t)(q[kk][j] >> 16)))));
+      top = wave_max_xor_groups(top);
+      int ex = (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127;
+      if (ex == 128 || ex == -127) ex = 0;  // Inf or NaN stays what it is; zero or a subnormal is 0
+      const float f = ldexpf(1.f, -ex);
+      scale = ldexpf(scale, ex);
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          q[kk][j] = TF16::pack(TB16::to_f((uint16_t)q[kk][j]) * f, TB16::to_f((uint16_t)(q[kk][j] >> 16)) * f);
+    }
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) q[kk][j] = c < rep ? q[kk][j] : 0u;
+    for (; i < i_end; i += WAVES) {
+      // Past the end: page 0's first rows, which nothing uses.  A condition on the loads would have the loop wait for
+      // all of them to merge their two values.
+      const Place next = place(min(i + WAVES, i_end - 1), n0, n1, i + WAVES < i_end);
+      n0 = page_at(i + 2 * WAVES, 0);
+      n1 = page_at(i + 2 * WAVES, 1);
+      const int tok = w.tok;
 
       // scores of head c at tokens tok + 8 g + j
       float s[8];
@@ -325,40 +366,18 @@ __global__ __launch_bounds__(WAVES * 64) void paged_decode_kernel(DecArgs a) {
           }
         }
       }
-      // V's scale of this lane's channel group, tokens in pairs
-      uint32_t vsc[4];
-      if constexpr (I8) {
-        const uint32_t sel = ((8 * c / GS) & 1) ? 0x07060302u : 0x05040100u;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if constexpr (G == 1) {
-            vsc[j] = x.vs[0][j];
-          } else if constexpr (G == 2) {
-            vsc[j] = perm_b32(x.vs[(2 * j + 1) / 4][(2 * j + 1) % 4], x.vs[2 * j / 4][2 * j % 4], sel);
-          } else {
-            const bool up = c >= 8;
-            const uint32_t w0 = up ? x.vs[j][1] : x.vs[j][0], w1 = up ? x.vs[j][3] : x.vs[j][2];
-            vsc[j] = perm_b32(w1, w0, sel);
-          }
-        }
-      }
-      if (full) {
+      load_k(next);
+      uint32_t seen = 0xFF;  // bit j: token tok + 8 g + j
+      if (w.full) {
         any = true;
       } else {
-        const bool there = !(v1 ? bad1 : bad0);
-        uint32_t seen = 0;
+        seen = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const int tj = tok + 8 * g + j;
-          const bool vis = there && tj < n && (tj >= rt.lo || tj < rt.sink_end);
+          const bool vis = !w.bad && tj < n && (tj >= rt.lo || tj < rt.sink_end);
           seen |= (uint32_t)vis << j;
           if (!vis) s[j] = kNegInf;
-          // what is masked may hold anything: 0 x NaN is no 0
-          if constexpr (I8) {
-            if (!vis) vsc[j / 2] &= j & 1 ? 0x0000FFFFu : 0xFFFF0000u;
-          } else {
-            if (!vis) x.v[j] = u32x4{0, 0, 0, 0};
-          }
         }
         any |= __any(seen != 0);
       }
@@ -389,7 +408,12 @@ __global__ __launch_bounds__(WAVES * 64) void paged_decode_kernel(DecArgs a) {
       }
       // P in 16 bits: the products' rounding averages out over the tokens; the sum takes the unrounded
       const u32x4 pb = {M::pack(p[0], p[1]), M::pack(p[2], p[3]), M::pack(p[4], p[5]), M::pack(p[6], p[7])};
+      __builtin_amdgcn_sched_barrier(0);  // nothing that waits for V above
       if constexpr (!I8) {
+        if (!w.full)  // what is masked may hold anything: 0 x NaN is no 0
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (!(seen >> j & 1)) x.v[j] = u32x4{0, 0, 0, 0};
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           u32x4 va;
@@ -399,6 +423,24 @@ __global__ __launch_bounds__(WAVES * 64) void paged_decode_kernel(DecArgs a) {
           acc[e] = M::mfma16(va, pb, acc[e]);
         }
       } else {
+        // V's scale of this lane's channel group, tokens in pairs
+        uint32_t vsc[4];
+        const uint32_t sel = ((8 * c / GS) & 1) ? 0x07060302u : 0x05040100u;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if constexpr (G == 1) {
+            vsc[j] = x.vs[0][j];
+          } else if constexpr (G == 2) {
+            vsc[j] = perm_b32(x.vs[(2 * j + 1) / 4][(2 * j + 1) % 4], x.vs[2 * j / 4][2 * j % 4], sel);
+          } else {
+            const bool up = c >= 8;
+            vsc[j] = perm_b32(up ? x.vs[j][3] : x.vs[j][2], up ? x.vs[j][1] : x.vs[j][0], sel);
+          }
+        }
+        if (!w.full)  // a masked code is finite, its scale may not be
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            vsc[j] &= (seen >> 2 * j & 1 ? 0xFFFFu : 0u) | (seen >> (2 * j + 1) & 1 ? 0xFFFF0000u : 0u);
 #pragma unroll
         for (int e4 = 0; e4 < 2; ++e4) {
           u32x4 va[4];
@@ -416,6 +458,8 @@ __global__ __launch_bounds__(WAVES * 64) void paged_decode_kernel(DecArgs a) {
           for (int e = 0; e < 4; ++e) acc[4 * e4 + e] = M::mfma16(va[e], pb, acc[4 * e4 + e]);
         }
       }
+      load_v(next);
+      w = next;
     }
 
     // join the waves: acc[e][r] is channel 32 g + 8 r + e of head c
@@ -557,7 +601,7 @@ __global__ __launch_bounds__(256) void paged_weights_kernel(DecArgs a) {
 
 // ---------------------------------------------------------------- host
 
-constexpr int kTargetGroups = 1024;  // work-groups of a launch: four of 4 waves a CU
+constexpr int kTargetGroups = 512;  // work-groups of a launch: two of 4 waves a CU
 constexpr int kMinTiles = 8;
 constexpr int kSoloTiles = 32;
 
@@ -620,7 +664,7 @@ int check(const kvq_paged_decode_params* p, PagedCache& c) {
 template <class T, bool I8, int GS, bool WT>
 int launch(const DecArgs& a, const Plan& w, hipStream_t st) {
   const int H = a.c.kv_heads, B = a.c.batch;
-  const size_t lds = 4 * 32 * 64 * 4 + (size_t)(B + 1) * 4;
+  const size_t lds = 4 * 32 * 64 * 4 + (size_t)(2 * B + 1) * 4;
   const dim3 grid((unsigned)w.groups, (unsigned)H);
   if (w.solo) hipLaunchKernelGGL((paged_decode_kernel<T, I8, GS, WT, 8>), grid, dim3(512), lds, st, a);
   else hipLaunchKernelGGL((paged_decode_kernel<T, I8, GS, WT, 4>), grid, dim3(256), lds, st, a);
