@@ -135,8 +135,9 @@ __device__ __forceinline__ float half_of(uint32_t w, int up) {
 typedef const __attribute__((address_space(4))) int32_t* const_i32;
 
 // K rows of a tile: token of matrix row i of half t: 8 (i / 4) + 4 t + i % 4.  V: tokens 8 g .. 8 g + 7,
-// channels 8 c .. 8 c + 7.  INT8 K: matrix step kk holds channels 32 kk + 8 g .. (groups of 32), or 64
-// (kk / 2) + 16 g + 8 (kk % 2) .. (wider groups, 16-byte loads): a step's channels lie in one group.
+// channels 8 c .. 8 c + 7.  INT8 K comes by 16 channels a lane: matrix step kk holds channels 64 (kk / 2) + 16 g +
+// 8 (kk % 2) ..; groups of 32 then lie in half of the lane groups, and each step is made twice, with Q zero in
+// the other half (8 bytes a lane would put a step into one group, but read at 4.0 TB/s where 16 reach 5.7).
 template <bool I8>
 struct Tile;
 template <>
@@ -212,7 +213,7 @@ __global__ __launch_bounds__(WAVES * 64, 2) void paged_decode_kernel(DecArgs a) 
       if (a.inv_tau) scale *= a.inv_tau[head];
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk)
-        q[kk] = *(const u32x4*)(qp + (I8 && GS >= 64 ? 64 * (kk >> 1) + 16 * g + 8 * (kk & 1) : 32 * kk + 8 * g));
+        q[kk] = *(const u32x4*)(qp + (I8 ? 64 * (kk >> 1) + 16 * g + 8 * (kk & 1) : 32 * kk + 8 * g));
     }
     float m = kNegInf, l = 0.f;
     float4v acc[8];
@@ -262,16 +263,13 @@ __global__ __launch_bounds__(WAVES * 64, 2) void paged_decode_kernel(DecArgs a) 
         if constexpr (!I8) {
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk) x.k[u][kk] = ld_stream<u32x4>(kr + 64 * kk + 16 * g);
-        } else if constexpr (GS >= 64) {
+        } else {
 #pragma unroll
           for (int kk = 0; kk < 4; kk += 2) {
             const u32x4 y = ld_stream<u32x4>(kr + 32 * kk + 16 * g);
             x.k[u][kk] = u32x2{y[0], y[1]};
             x.k[u][kk + 1] = u32x2{y[2], y[3]};
           }
-        } else {
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk) x.k[u][kk] = ld_stream<u32x2>(kr + 32 * kk + 8 * g);
         }
       }
       if constexpr (I8)
@@ -324,6 +322,16 @@ __global__ __launch_bounds__(WAVES * 64, 2) void paged_decode_kernel(DecArgs a) 
     for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
       for (int j = 0; j < 4; ++j) q[kk][j] = c < rep ? q[kk][j] : 0u;
+    u32x4 qu[4];  // groups of 32: q for the upper lane groups, q for the lower
+    if constexpr (I8 && GS == 32) {
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          qu[kk][j] = g >= 2 ? q[kk][j] : 0u;
+          q[kk][j] = g < 2 ? q[kk][j] : 0u;
+        }
+    }
     for (; i < i_end; i += WAVES) {
       // Past the end: page 0's first rows, which nothing uses.  A condition on the loads would have the loop wait for
       // all of them to merge their two values.
@@ -351,7 +359,12 @@ __global__ __launch_bounds__(WAVES * 64, 2) void paged_decode_kernel(DecArgs a) 
             const uint32_t lo = x.k[u][kk][0] ^ 0x80808080u, hi = x.k[u][kk][1] ^ 0x80808080u;
             const u32x4 ka = {code_pair(lo, 0x04010400u), code_pair(lo, 0x04030402u), code_pair(hi, 0x04010400u),
                               code_pair(hi, 0x04030402u)};
-            d[kk * G / 4] = M::mfma16(ka, q[kk], d[kk * G / 4]);
+            if constexpr (GS == 32) {
+              d[kk & 2] = M::mfma16(ka, q[kk], d[kk & 2]);
+              d[(kk & 2) + 1] = M::mfma16(ka, qu[kk], d[(kk & 2) + 1]);
+            } else {
+              d[kk * G / 4] = M::mfma16(ka, q[kk], d[kk * G / 4]);
+            }
           }
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
