@@ -33,6 +33,7 @@ from .cache import (  # noqa: F401
     load_per_layer_bits_from_policy,
 )
 from .paged import append_paged, decode_attn_paged, evict_paged, prefill_attn_window  # noqa: F401
+from .paged_cache import PagedKVCache  # noqa: F401
 from .patch import (  # noqa: F401
     INT8CacheWrapper,
     INT8CacheWrapperContainer,
@@ -62,6 +63,7 @@ __all__ = [
     "decode_attn_int4_kivi",
     "decode_attn_int4_asym_v2",
     "decode_attn_int4_asym_gqa",
+    "PagedKVCache",
     "append_paged",
     "decode_attn_paged",
     "prefill_attn_window",

@@ -12,7 +12,8 @@ proxy runs :func:`_fused_forward_impl`:
    formats, append then attention otherwise);
 4. ``o_proj``.
 
-Every other call (prefill, no quantized cache) goes to the original forward.  The decode
+A prompt over an engine that attends prompts itself (:class:`PagedKVCache`) goes through its ``prefill_attn``
+(:func:`_prefill_forward_impl`).  Every other call (prefill, no quantized cache) goes to the original forward.  The decode
 implementation is the engine's ``decode_attn_impl``: ``"hip_fused"`` and the reference's
 ``"triton_fused"`` run the HIP kernels; ``"torch_ref"`` is the reference's own torch
 decode path (:func:`_decode_attn_int8_torch_ref`), a mode the caller selects explicitly for
@@ -82,7 +83,7 @@ class INT8CacheWrapper:
 def _is_quantized_engine(engine) -> bool:
     return any(hasattr(engine, n) for n in (
         "get_int8_tensors", "get_int4_tensors", "get_int4_asym_tensors", "get_int4_g32_tensors",
-        "get_k8v4_tensors", "get_kivi_tensors", "get_mixed_tensors"))
+        "get_k8v4_tensors", "get_kivi_tensors", "get_mixed_tensors", "get_paged_tensors"))
 
 
 class INT8CacheWrapperContainer:
@@ -447,6 +448,44 @@ def _fused_forward_impl(self, hidden_states, cache_wrapper, attention_mask=None,
     return attn_output, None
 
 
+def _attends_prompts(engine) -> bool:
+    """Whether the engine attends prompts itself (PagedKVCache), through its own window or budget."""
+    return callable(getattr(type(engine), "prefill_attn", None))
+
+
+def _prefill_forward_impl(self, hidden_states, cache_wrapper, attention_mask=None, position_ids=None,
+                          position_embeddings=None, return_cache=False):
+    """A prompt, or a chunk of one, over an engine that attends prompts itself: projections, RoPE, the engine's
+    ``prefill_attn``, output projection.  No counterpart in the reference, whose prompts run the model's own
+    attention."""
+    if attention_mask is not None:
+        # a causal mask says nothing new, and its last row is open; padding is not in the engine's terms
+        seen = attention_mask if attention_mask.ndim == 2 else attention_mask[..., -1, :]
+        if not bool(torch.all(seen if seen.dtype == torch.bool else seen == (1 if attention_mask.ndim == 2 else 0))):
+            raise ValueError("an engine that attends prompts itself takes no padding or window mask: give its prefill_attn "
+                             "the lengths")
+    layer_idx = getattr(cache_wrapper, "layer_idx", getattr(self, "layer_idx", 0))
+    bsz, q_len, _ = hidden_states.shape
+    q_heads, kv_heads, head_dim = _resolve_attn_shape_meta(self)
+    engine = cache_wrapper.engine
+    q = self.q_proj(hidden_states).view(bsz, q_len, q_heads, head_dim).transpose(1, 2)
+    k = self.k_proj(hidden_states).view(bsz, q_len, kv_heads, head_dim).transpose(1, 2)
+    v = self.v_proj(hidden_states).view(bsz, q_len, kv_heads, head_dim).transpose(1, 2)
+    if getattr(self, "q_norm", None) is not None:
+        q = self.q_norm(q)
+    if getattr(self, "k_norm", None) is not None:
+        k = self.k_norm(k)
+    cos, sin = _get_rope_cos_sin(self, v, position_ids, position_embeddings)
+    if cos is None or sin is None:
+        raise RuntimeError("Failed to obtain RoPE cos/sin for the prompt. "
+                           "Check transformers version/model API (position_ids/position_embeddings).")
+    q, k = _apply_rope(q, k, cos, sin)
+    out = engine.prefill_attn(layer_idx, q, k, v, sm_scale=float(getattr(self, "scaling", 1.0 / math.sqrt(head_dim))),
+                              inv_tau=_layer_inv_tau(engine, layer_idx, q_heads, q.device, q.dtype))
+    attn_output = self.o_proj(out.transpose(1, 2).reshape(bsz, q_len, q_heads * head_dim).to(hidden_states.dtype))
+    return (attn_output, None, cache_wrapper) if return_cache else (attn_output, None)
+
+
 def apply_int8_fused_patch(model) -> None:
     """Patch the model's attention class for fused quantized decode
     (src/engine/patch_model.py:1011-1226)."""
@@ -527,6 +566,11 @@ def apply_int8_fused_patch(model) -> None:
                                        position_ids=position_ids, position_embeddings=pos_emb,
                                        cache_position=cache_pos,
                                        return_cache=use_cache if has_use_cache else False)
+        if hidden_states is not None and cache_wrapper is not None and _attends_prompts(cache_wrapper.engine):
+            return _prefill_forward_impl(self, hidden_states, cache_wrapper, attention_mask=attention_mask,
+                                         position_ids=position_ids,
+                                         position_embeddings=kwargs.pop("position_embeddings", None),
+                                         return_cache=use_cache if has_use_cache else False)
         kw = dict(attention_mask=attention_mask, position_ids=position_ids,
                   output_attentions=output_attentions, use_cache=use_cache, **kwargs)
         kw = _filter_kwargs(kw)
