@@ -270,10 +270,9 @@ def lib() -> ctypes.CDLL:
         L.kvq_append_plan.restype = c_i32
         L.kvq_append_division.argtypes = [c_vp, c_vp, c_vp, c_vp, c_i64, c_vp]
         L.kvq_append_division.restype = c_i32
-        # the paged cache (include/kvq_paged.h)
-        for name, params in (("kvq_paged_append", PagedAppendParams), ("kvq_paged_decode", PagedDecodeParams),
-                             ("kvq_prefill_attn", PrefillParams), ("kvq_paged_evict", PagedEvictParams)):
-            getattr(L, name).argtypes = [ctypes.POINTER(params), c_vp]
+        # the paged cache (include/kvq_paged.h); a parameter block may be given as packed bytes
+        for name in ("kvq_paged_append", "kvq_paged_decode", "kvq_prefill_attn", "kvq_paged_evict"):
+            getattr(L, name).argtypes = [c_vp, c_vp]
             getattr(L, name).restype = c_i32
         for name, params in (("kvq_paged_decode_workspace_bytes", PagedDecodeParams),
                              ("kvq_prefill_workspace_bytes", PrefillParams)):

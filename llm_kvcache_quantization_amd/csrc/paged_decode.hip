@@ -646,7 +646,7 @@ Plan plan_of(const kvq_paged_decode_params& p, bool weights) {
     w.bytes += (bytes + 63) / 64 * 64;
     return at;
   };
-  w.pre = take(4 * (B + 2));
+  if (!w.solo || weights) w.pre = take(4 * (B + 2));
   if (!w.solo) {
     w.ml = take(8 * H * w.groups * 2 * rep);
     w.acc = take(512 * H * w.groups * 2 * rep);
@@ -704,7 +704,7 @@ int decode(const kvq_paged_decode_params* p, hipStream_t st) {
   if (((uintptr_t)p->q | (uintptr_t)p->out) % 16 || (p->q_stride_b | p->q_stride_h) % 8)
     return fail(KVQ_ERR_INVALID, "paged decode: q rows must be 16-byte aligned");
   const Plan w = plan_of(*p, p->weights != nullptr);
-  if (!p->workspace || p->workspace_bytes < w.bytes || (uintptr_t)p->workspace % 16)
+  if (w.bytes && (!p->workspace || p->workspace_bytes < w.bytes || (uintptr_t)p->workspace % 16))
     return fail(KVQ_ERR_INVALID, "paged decode: workspace too small or not 16-byte aligned");
   // without pages every row sees nothing: no column of the table is read
   if (a.c.num_pages == 0) a.c.max_pages = 0;

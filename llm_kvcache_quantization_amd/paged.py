@@ -32,6 +32,7 @@ src/cache/fp16_cache.py).
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 import struct
 from typing import Optional, Tuple
@@ -59,29 +60,30 @@ def _packer(cls) -> struct.Struct:
     return struct.Struct("@" + "".join(_leaves(cls)))
 
 
+_SM = 1.0 / math.sqrt(HEAD_DIM)
 _APPEND, _DECODE, _PREFILL, _EVICT = (_packer(c) for c in (
     C.PagedAppendParams, C.PagedDecodeParams, C.PrefillParams, C.PagedEvictParams))
 
 
 
 
-def _no_grad(*tensors: Tensor) -> None:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise NotImplementedError("the paged operators have no backward pass: call them under torch.no_grad()")
+def _no_grad() -> None:
+    raise NotImplementedError("the paged operators have no backward pass: call them under torch.no_grad()")
 
 
-def _call(fn, block, device: torch.device) -> None:
-    if device.index != torch.cuda.current_device():
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _call(fn, block: bytes, device: torch.device) -> None:
+    if device.index != _current_device():
         with torch.cuda.device(device):
             C.check(fn(block, C.stream_handle(device)))
     else:
         C.check(fn(block, C.stream_handle(device)))
 
 
-def _i32(t: Optional[Tensor], name: str, batch: int, device: torch.device) -> Optional[Tensor]:
+def _i32(t: Tensor, name: str, batch: int, device: torch.device) -> Tensor:
     """A [B] tensor of lengths or positions as contiguous int32 on the device."""
-    if t is None:
-        return None
     if t.ndim != 1 or t.shape[0] != batch:
         raise ValueError(f"{name} must be [B] = [{batch}], got {tuple(t.shape)}")
     if t.dtype != torch.int32 or t.device != device:
@@ -89,10 +91,6 @@ def _i32(t: Optional[Tensor], name: str, batch: int, device: torch.device) -> Op
             raise ValueError(f"{name} must be integers, got {t.dtype}")
         t = t.to(device=device, dtype=torch.int32)
     return t.contiguous()
-
-
-def _ptr(t: Optional[Tensor]) -> int:
-    return 0 if t is None else t.data_ptr()
 
 
 def _cache_fields(k_pages: Tensor, v_pages: Tensor, k_scale: Optional[Tensor], v_scale: Optional[Tensor],
@@ -104,11 +102,11 @@ def _cache_fields(k_pages: Tensor, v_pages: Tensor, k_scale: Optional[Tensor], v
     if v_pages.shape != shape:
         raise ValueError(f"k/v pages differ in shape: {tuple(shape)} vs {tuple(v_pages.shape)}")
     pages, heads, size, _ = shape
-    dtype, device = k_pages.dtype, k_pages.device
+    dtype, index = k_pages.dtype, k_pages.get_device()
     if not k_pages.is_cuda:
         raise ValueError("the paged operators need GPU (ROCm) tensors")
-    if v_pages.dtype != dtype or v_pages.device != device:
-        raise ValueError(f"k/v pages differ: {dtype} on {device} vs {v_pages.dtype} on {v_pages.device}")
+    if v_pages.dtype != dtype or v_pages.get_device() != index:
+        raise ValueError(f"k/v pages differ: {dtype} on {k_pages.device} vs {v_pages.dtype} on {v_pages.device}")
     if size not in PAGE_SIZES:
         raise ValueError(f"page_size must be one of {PAGE_SIZES}, got {size}")
     if heads == 0:
@@ -119,14 +117,14 @@ def _cache_fields(k_pages: Tensor, v_pages: Tensor, k_scale: Optional[Tensor], v
             raise ValueError("INT8 pages need k_scale and v_scale")
         groups = k_scale.shape[-1]
         for name, s in (("k_scale", k_scale), ("v_scale", v_scale)):
-            if s.dtype != torch.float16 or s.device != device or s.shape != (pages, heads, size, groups) or \
+            if s.dtype != torch.float16 or s.get_device() != index or s.shape != (pages, heads, size, groups) or \
                     groups not in (1, 2, 4):
-                raise ValueError(f"{name} must be fp16 [{pages}, {heads}, {size}, G] with G 1, 2 or 4 on {device}, got "
+                raise ValueError(f"{name} must be fp16 [{pages}, {heads}, {size}, G] with G 1, 2 or 4 on {k_pages.device}, got "
                                  f"{s.dtype} {tuple(s.shape)} on {s.device}")
-            if s.numel() and (s.stride(3) != 1 and groups > 1 or s.stride(2) != groups):
-                raise ValueError(f"{name}: a page's scales must be dense, got strides {s.stride()}")
-        group = HEAD_DIM // groups
         ks, vs = k_scale.stride(), v_scale.stride()
+        if pages and (ks[2] != groups or vs[2] != groups or groups > 1 and (ks[3] != 1 or vs[3] != 1)):
+            raise ValueError(f"a page's scales must be dense, got strides {ks} and {vs}")
+        group = HEAD_DIM // groups
         scales = (k_scale.data_ptr(), v_scale.data_ptr(), 2 * ks[0], 2 * ks[1], 2 * vs[0], 2 * vs[1])
     else:
         fmt, item, group = _TYPES.get(dtype), 2, 0
@@ -138,29 +136,28 @@ def _cache_fields(k_pages: Tensor, v_pages: Tensor, k_scale: Optional[Tensor], v
     k, v = k_pages.stride(), v_pages.stride()
     if k[3] != 1 or v[3] != 1:
         raise ValueError("page rows must be contiguous")
-    if table.ndim != 2 or table.dtype != torch.int32 or table.device != device:
-        raise ValueError(f"block_table must be int32 [B, max_pages] on {device}, got {table.dtype} {tuple(table.shape)} "
-                         f"on {table.device}")
+    if table.ndim != 2 or table.dtype != torch.int32 or table.get_device() != index:
+        raise ValueError(f"block_table must be int32 [B, max_pages] on {k_pages.device}, got {table.dtype} "
+                         f"{tuple(table.shape)} on {table.device}")
     rows, cols = table.shape
-    if cols > 1 and table.stride(1) != 1:
+    step, inner = table.stride()
+    if cols > 1 and inner != 1:
         raise ValueError("block_table rows must be contiguous")
     if batch is not None and rows != batch:
         raise ValueError(f"block_table has {rows} rows for a batch of {batch}")
     return (k_pages.data_ptr(), v_pages.data_ptr(), item * k[0], item * k[1], item * k[2], item * v[0], item * v[1],
-            item * v[2], *scales, table.data_ptr(), table.stride(0), pages, cols, size, fmt, group, rows, heads, 0)
+            item * v[2], *scales, table.data_ptr(), step, pages, cols, size, fmt, group, rows, heads, 0)
 
 
 def _rows16(x: Tensor) -> Tensor:
     """x itself if its rows of 128 are contiguous and 16-byte aligned, else a copy."""
-    s = x.stride()
-    if s[-1] != 1 or any(v % 8 for v in s[:-1]) or x.data_ptr() % 16:
+    *outer, inner = x.stride()
+    if inner != 1 or x.data_ptr() & 15 or any([v & 7 for v in outer]):
         return x.clone(memory_format=torch.contiguous_format)
     return x
 
 
-def _tau(inv_tau: Optional[Tensor], heads: int, device: torch.device) -> Optional[Tensor]:
-    if inv_tau is None:
-        return None
+def _tau(inv_tau: Tensor, heads: int, device: torch.device) -> Tensor:
     if inv_tau.shape != (heads,):
         raise ValueError(f"inv_tau must be [{heads}] (one per query head), got {tuple(inv_tau.shape)}")
     return inv_tau.to(device=device, dtype=torch.float32).contiguous()
@@ -174,6 +171,28 @@ def _window(window: Optional[int], sinks: int) -> Tuple[int, int]:
     if sinks < 0:
         raise ValueError(f"sinks must be >= 0, got {sinks}")
     return min(int(window), 1 << 30), min(int(sinks), 1 << 30)
+
+
+@functools.lru_cache(maxsize=256)
+def _decode_scratch(pages: int, cols: int, size: int, rows: int, heads: int, q_heads: int, window: int, sinks: int,
+                    weights: bool) -> int:
+    """Bytes of scratch of a decode call: a matter of its sizes alone."""
+    p = C.PagedDecodeParams()
+    c = p.cache
+    c.k_stride_t = c.v_stride_t = 2 * HEAD_DIM
+    c.num_pages, c.max_pages, c.page_size, c.batch, c.kv_heads = pages, cols, size, rows, heads
+    c.k = c.v = c.table = p.weights = 16  # not read
+    if not weights:
+        p.weights = None
+    p.window, p.sinks, p.q_heads = window, sinks, q_heads
+    return C.lib().kvq_paged_decode_workspace_bytes(ctypes.byref(p))
+
+
+@functools.lru_cache(maxsize=256)
+def _prefill_scratch(batch: int, q_heads: int, heads: int, seq: int, total: int, window: int, sinks: int) -> int:
+    p = C.PrefillParams()
+    p.batch, p.q_heads, p.kv_heads, p.seq_q, p.seq_kv, p.window, p.sinks = batch, q_heads, heads, seq, total, window, sinks
+    return C.lib().kvq_prefill_workspace_bytes(ctypes.byref(p))
 
 
 def append_paged(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, block_table: Tensor, write_pos: Tensor,
@@ -202,14 +221,14 @@ def append_paged(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, block_t
         raise ValueError(f"k/v must lie on {device}, got {k.device} / {v.device}")
     if heads != k_pages.shape[1]:
         raise ValueError(f"k/v have {heads} heads, the pages {k_pages.shape[1]}")
-    _no_grad(k, v)
+    if (k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
+        _no_grad()
     pos = _i32(write_pos, "write_pos", batch, device)
-    lens = _i32(new_lens, "new_lens", batch, device)
+    lens = None if new_lens is None else _i32(new_lens, "new_lens", batch, device)
     k, v = _rows16(k), _rows16(v)
-    block = C.PagedAppendParams.from_buffer_copy(_APPEND.pack(
-        *cache, k.data_ptr(), v.data_ptr(), *k.stride()[:3], *v.stride()[:3], pos.data_ptr(), _ptr(lens), seq,
-        _TYPES[k.dtype]))
-    _call(C.lib().kvq_paged_append, block, device)
+    _call(C.lib().kvq_paged_append, _APPEND.pack(
+        *cache, k.data_ptr(), v.data_ptr(), *k.stride()[:3], *v.stride()[:3], pos.data_ptr(),
+        0 if lens is None else lens.data_ptr(), seq, _TYPES[k.dtype]), device)
 
 
 def decode_attn_paged(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_table: Tensor, context_lens: Tensor,
@@ -238,7 +257,8 @@ def decode_attn_paged(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_table: 
         raise ValueError(f"q must lie on {device}, got {q.device}")
     if q_heads == 0 or q_heads % heads:
         raise ValueError(f"q_heads={q_heads} must be a multiple of kv_heads={heads}")
-    _no_grad(q)
+    if q.requires_grad and torch.is_grad_enabled():
+        _no_grad()
     lens = _i32(context_lens, "context_lens", batch, device)
     window, sinks = _window(window, sinks)
     w = (0, 0, 0)
@@ -253,19 +273,18 @@ def decode_attn_paged(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_table: 
         if batch > 1 and ws[0] == 0 or heads > 1 and ws[1] == 0:
             raise ValueError("weights must have memory of their own for every sequence and head")
         w = (weights.data_ptr(), ws[0], ws[1])
-    tau = _tau(inv_tau, q_heads, device)
+    tau = None if inv_tau is None else _tau(inv_tau, q_heads, device)
     q = _rows16(q)
-    out = torch.empty(q.shape, dtype=q.dtype, device=device)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if batch == 0:
         return out
-    lib = C.lib()
-    block = C.PagedDecodeParams.from_buffer_copy(_DECODE.pack(
-        *cache, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), lens.data_ptr(), _ptr(tau), *w, 0, 0,
-        1.0 / math.sqrt(HEAD_DIM) if sm_scale is None else sm_scale, window, sinks, q_heads, _TYPES[q.dtype], 0))
-    nbytes = lib.kvq_paged_decode_workspace_bytes(block)
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    block.workspace, block.workspace_bytes = scratch.data_ptr(), nbytes
-    _call(lib.kvq_paged_decode, block, device)
+    # (the sizes' limits are checked in the library, by both calls)
+    nbytes = _decode_scratch(k_pages.shape[0], block_table.shape[1], k_pages.shape[2], batch, heads, q_heads, window, sinks, weights is not None)
+    scratch = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    _call(C.lib().kvq_paged_decode, _DECODE.pack(
+        *cache, q.data_ptr(), *q.stride()[:2], out.data_ptr(), lens.data_ptr(), 0 if tau is None else tau.data_ptr(), *w,
+        0 if scratch is None else scratch.data_ptr(), nbytes, _SM if sm_scale is None else sm_scale, window, sinks, q_heads,
+        _TYPES[q.dtype], 0), device)
     return out
 
 
@@ -293,26 +312,23 @@ def prefill_attn_window(q: Tensor, k: Tensor, v: Tensor, sm_scale: Optional[floa
         raise ValueError(f"q, k and v must be all fp16 or all bf16, got {q.dtype} / {k.dtype} / {v.dtype}")
     if q_heads == 0 or heads == 0 or q_heads % heads:
         raise ValueError(f"q_heads={q_heads} must be a multiple of kv_heads={heads}")
-    _no_grad(q, k, v)
-    ql = _i32(q_lens, "q_lens", batch, device)
-    kl = _i32(kv_lens, "kv_lens", batch, device)
+    if (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
+        _no_grad()
+    ql = None if q_lens is None else _i32(q_lens, "q_lens", batch, device)
+    kl = None if kv_lens is None else _i32(kv_lens, "kv_lens", batch, device)
     window, sinks = _window(window, sinks)
-    tau = _tau(inv_tau, q_heads, device)
+    tau = None if inv_tau is None else _tau(inv_tau, q_heads, device)
     q, k, v = _rows16(q), _rows16(k), _rows16(v)
-    out = torch.empty((batch, q_heads, seq, HEAD_DIM), dtype=q.dtype, device=device)
-    if out.numel() == 0:
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    if batch == 0 or seq == 0:
         return out
-    lib = C.lib()
-    block = C.PrefillParams.from_buffer_copy(_PREFILL.pack(
+    nbytes = _prefill_scratch(batch, q_heads, heads, seq, total, window, sinks)
+    scratch = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    _call(C.lib().kvq_prefill_attn, _PREFILL.pack(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], out.data_ptr(),
-        *out.stride()[:3], _ptr(ql), _ptr(kl), _ptr(tau), 0, 0,
-        1.0 / math.sqrt(HEAD_DIM) if sm_scale is None else sm_scale, batch, q_heads, heads, seq, total, window, sinks,
-        _TYPES[q.dtype], 0))
-    nbytes = lib.kvq_prefill_workspace_bytes(block)
-    if nbytes:
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        block.workspace, block.workspace_bytes = scratch.data_ptr(), nbytes
-    _call(lib.kvq_prefill_attn, block, device)
+        *out.stride()[:3], 0 if ql is None else ql.data_ptr(), 0 if kl is None else kl.data_ptr(),
+        0 if tau is None else tau.data_ptr(), 0 if scratch is None else scratch.data_ptr(), nbytes,
+        _SM if sm_scale is None else sm_scale, batch, q_heads, heads, seq, total, window, sinks, _TYPES[q.dtype], 0), device)
     return out
 
 
@@ -344,13 +360,11 @@ def evict_paged(k_pages: Tensor, v_pages: Tensor, block_table: Tensor, context_l
         raise ValueError(f"budget must be positive and hold sinks + recent, got {budget}, {sinks} + {recent}")
     if budget >= 1 << 31:
         raise ValueError(f"budget too large: {budget}")
-    tokens = weights.shape[2]
-    new_lens = torch.empty(batch, dtype=torch.int32, device=device)
-    kept = torch.empty((batch, heads, budget), dtype=torch.int32, device=device)
-    new_weights = torch.empty((batch, heads, tokens), dtype=torch.float32, device=device)
+    new_lens = torch.empty_like(lens)
+    kept = lens.new_empty((batch, heads, budget))
+    new_weights = torch.empty_like(weights, memory_format=torch.contiguous_format)
     if batch:
-        block = C.PagedEvictParams.from_buffer_copy(_EVICT.pack(
-            *cache, lens.data_ptr(), weights.data_ptr(), weights.stride(0), weights.stride(1), new_lens.data_ptr(),
-            kept.data_ptr(), new_weights.data_ptr(), tokens, budget, sinks, recent))
-        _call(C.lib().kvq_paged_evict, block, device)
+        _call(C.lib().kvq_paged_evict, _EVICT.pack(
+            *cache, lens.data_ptr(), weights.data_ptr(), *weights.stride()[:2], new_lens.data_ptr(), kept.data_ptr(),
+            new_weights.data_ptr(), weights.shape[2], budget, sinks, recent), device)
     return new_lens, kept, new_weights

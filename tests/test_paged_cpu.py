@@ -182,9 +182,10 @@ def test_bad_calls_are_refused():
                  dict(v=AT + 2), dict(k_stride_s=130), dict(v_stride_h=4)):
         _refused(L, "kvq_paged_append", _append(C, c, **over))
     for over in (dict(q_type=7), dict(q_type=C.KVQ_PAGED_BF16), dict(q_heads=6), dict(q_heads=0), dict(q_heads=68),
-                 dict(q=None), dict(out=None), dict(context_lens=None), dict(q=AT + 8), dict(q_stride_h=132),
-                 dict(workspace=None), dict(workspace_bytes=8), dict(workspace=AT + 4)):
+                 dict(q=None), dict(out=None), dict(context_lens=None), dict(q=AT + 8), dict(q_stride_h=132)):
         _refused(L, "kvq_paged_decode", _decode(C, c, **over))
+    for over in (dict(workspace=None), dict(workspace_bytes=8), dict(workspace=AT + 4)):  # rows that are shared out
+        _refused(L, "kvq_paged_decode", _decode(C, _cache(C, max_pages=1000), **over))
     _refused(L, "kvq_paged_decode", _decode(C, _cache(C, batch=4097)))
     for over in (dict(budget=0), dict(sinks=-1), dict(recent=-1), dict(recent=47), dict(w_tokens=127), dict(weights=None),
                  dict(kept=None), dict(new_lens=None), dict(sinks=2 ** 31 - 1, recent=2 ** 31 - 1)):
@@ -218,7 +219,7 @@ def test_workspace_covers_what_a_call_writes():
             p = _decode(C, _cache(C, batch=batch, kv_heads=heads, max_pages=pages, page_size=size), q_heads=heads * rep, weights=weights)
             n = L.kvq_paged_decode_workspace_bytes(ctypes.byref(p))
             tiles = -(-pages * size // 32)
-            assert n >= 4 * (batch + 2)
+            assert n >= 4 * (batch + 2) or (n == 0 and tiles <= 32 and not weights)
             if weights:
                 assert n >= 4 * heads * batch * tiles * rep * 32 + 4 * batch * heads * rep
             assert n <= (4 << 20) + 2 * 1088 * 16 * 520 + (0 if not weights else 5 * heads * batch * (tiles + 1) * rep * 32)
