@@ -23,7 +23,7 @@ namespace kvq {
 namespace {
 
 constexpr int kTile = 32;        // token slots a tile
-constexpr int kMaxRows = 4096;   // rows of a call (their tile counts are scanned in LDS)
+constexpr int kMaxRows = 4096;   // rows of a call (the tiles before each lie in LDS)
 constexpr int kHeads = 16;       // query heads of a KV head, padded
 
 struct DecArgs {
@@ -72,21 +72,59 @@ __device__ __forceinline__ int row_len(const DecArgs& a, int b) {
   return (int)min((int64_t)max(a.lens[b], 0), cap);
 }
 
-// pre[0..B] = tiles before each row, len[0..B-1] their tokens; every thread of the work-group calls it
-template <int THREADS>
-__device__ void scan_rows(const DecArgs& a, int* pre, int* len, int* wsum) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  int base = 0;
-  for (int b0 = 0; b0 < a.c.batch; b0 += THREADS) {
-    const int b = b0 + tid;
-    const int n = b < a.c.batch ? row_len(a, b) : 0;
-    if (b < a.c.batch) len[b] = n;
-    int x = RowTiles(n, a.window, a.sinks).count;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int y = __shfl_up(x, o, 64);
-      if (lane >= o) x += y;
+// The tiles before each row.  Up to 64 rows every wave has them in its lanes, with the rows' token counts, by a
+// scan of its own; more are scanned by the work-group into LDS.
+struct Rows {
+  int* pre;  // [batch + 1]
+  int before, tokens, total;  // lane b: row b's
+  bool small;
+  __device__ __forceinline__ int start(int b) const { return small ? __builtin_amdgcn_readlane(before, b) : pre[b]; }
+  __device__ __forceinline__ int end(int b, int batch) const { return b + 1 < batch ? start(b + 1) : total; }
+  __device__ __forceinline__ int length(const DecArgs& a, int b) const {
+    return small ? __builtin_amdgcn_readlane(tokens, b) : row_len(a, b);
+  }
+  // the last row that begins at or before tile t < total: it is not empty
+  __device__ __forceinline__ int of(int t, int batch) const {
+    if (small) return 63 - __builtin_clzll(__ballot((int)(threadIdx.x & 63) < batch && before <= t));
+    int row = 0;
+    for (int hi = batch; hi - row > 1;) {
+      const int mid = (row + hi) >> 1;
+      if (pre[mid] <= t) row = mid; else hi = mid;
     }
+    return row;
+  }
+};
+
+__device__ __forceinline__ int scan64(int x) {  // inclusive, over the lanes
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(x, o, 64);
+    if (lane >= o) x += y;
+  }
+  return x;
+}
+
+// every thread of the work-group calls it
+template <int THREADS>
+__device__ __forceinline__ Rows scan_rows(const DecArgs& a, int* lds, int* wsum) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, batch = a.c.batch;
+  Rows r;
+  r.pre = lds;
+  r.small = batch <= 64;
+  if (r.small) {
+    r.tokens = lane < batch ? row_len(a, lane) : 0;
+    const int x = RowTiles(r.tokens, a.window, a.sinks).count;
+    const int y = scan64(x);
+    r.before = y - x;
+    r.total = __builtin_amdgcn_readlane(y, 63);
+    return r;
+  }
+  r.before = r.tokens = 0;
+  int base = 0;
+  for (int b0 = 0; b0 < batch; b0 += THREADS) {
+    const int b = b0 + tid;
+    const int x = scan64(RowTiles(b < batch ? row_len(a, b) : 0, a.window, a.sinks).count);
     if (lane == 63) wsum[wave] = x;
     __syncthreads();
     int before = base, all = base;
@@ -94,12 +132,14 @@ __device__ void scan_rows(const DecArgs& a, int* pre, int* len, int* wsum) {
       if (w < wave) before += wsum[w];
       all += wsum[w];
     }
-    if (b < a.c.batch) pre[b + 1] = before + x;
+    if (b < batch) r.pre[b + 1] = before + x;
     base = all;
     __syncthreads();
   }
-  if (tid == 0) pre[0] = 0;
+  if (tid == 0) r.pre[0] = 0;
   __syncthreads();
+  r.total = base;
+  return r;
 }
 
 __device__ __forceinline__ int tiles_each(const DecArgs& a, int total) {
@@ -158,49 +198,50 @@ __global__ __launch_bounds__(WAVES * 64, 2) void paged_decode_kernel(DecArgs a) 
   __shared__ int wsum[WAVES];
   __shared__ float2 wml[WAVES][kHeads];
   float* const wacc = (float*)lds;                     // [4][32][64]
-  int* const pre = (int*)(lds + 4 * 32 * 64 * 4);      // [batch + 1]
-  int* const len = pre + a.c.batch + 1;                // [batch]
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 15, g = lane >> 4;
   const int h = blockIdx.y, rep = a.rep;
   const PagedCache& pc = a.c;
 
-  scan_rows<WAVES * 64>(a, pre, len, wsum);
-  const int total = pre[pc.batch], per = tiles_each(a, total);
+  const Rows rows = scan_rows<WAVES * 64>(a, (int*)(lds + 4 * 32 * 64 * 4), wsum);
+  const int total = rows.total, per = tiles_each(a, total);
   if ((WT || !a.solo) && blockIdx.x == 0 && h == 0) {
-    for (int b = tid; b <= pc.batch; b += WAVES * 64) a.pre[b] = pre[b];
-    if (tid == 0) a.pre[pc.batch + 1] = per;
+    if (rows.small) {
+      if (tid < pc.batch) a.pre[tid] = rows.before;
+    } else {
+      for (int b = tid; b < pc.batch; b += WAVES * 64) a.pre[b] = rows.pre[b];
+    }
+    if (tid == 0) {
+      a.pre[pc.batch] = total;
+      a.pre[pc.batch + 1] = per;
+    }
   }
   // rows that see nothing
   for (int b = blockIdx.x; b < pc.batch; b += gridDim.x)
-    if (pre[b + 1] == pre[b])
+    if (rows.end(b, pc.batch) == rows.start(b))
       for (int i = tid; i < rep * 64; i += WAVES * 64)
         ((uint32_t*)a.out)[((int64_t)b * a.q_heads + h * rep) * 64 + i] = 0;
 
   int t, t1;
   if (a.solo) {
-    t = pre[blockIdx.x];
-    t1 = pre[blockIdx.x + 1];
+    t = rows.start(blockIdx.x);
+    t1 = rows.end(blockIdx.x, pc.batch);
   } else {
     t = (int)min((int64_t)blockIdx.x * per, (int64_t)total);
     t1 = (int)min((int64_t)t + per, (int64_t)total);
   }
   if (t >= t1) return;
-  int row = 0;
-  for (int hi = pc.batch; hi - row > 1;) {  // the last row with pre[row] <= t: it is not empty
-    const int mid = (row + hi) >> 1;
-    if (pre[mid] <= t) row = mid; else hi = mid;
-  }
+  int row = a.solo ? (int)blockIdx.x : rows.of(t, pc.batch);
 
   const uint8_t* const kh = pc.k + h * pc.ksh;
   const uint8_t* const vh = pc.v + h * pc.vsh;
   const int t0 = t;
   for (; t < t1; ++row) {
     row = __builtin_amdgcn_readfirstlane(row);
-    const int rs = __builtin_amdgcn_readfirstlane(pre[row]), re = __builtin_amdgcn_readfirstlane(pre[row + 1]);
+    const int rs = __builtin_amdgcn_readfirstlane(rows.start(row)), re = __builtin_amdgcn_readfirstlane(rows.end(row, pc.batch));
     if (re == rs) continue;
     const int end = min(t1, re);
-    const int n = __builtin_amdgcn_readfirstlane(len[row]);
+    const int n = __builtin_amdgcn_readfirstlane(rows.length(a, row));
     const RowTiles rt(n, a.window, a.sinks);
     const const_i32 tab = (const_i32)(pc.table + row * pc.table_stride);
 
@@ -550,21 +591,35 @@ __global__ __launch_bounds__(WAVES * 64, 2) void paged_decode_kernel(DecArgs a) 
   }
 }
 
-// Joins a row that several work-groups share: one work-group a (row, query head), 16 parts at a time, 8
+// A row's part of the shared rows' parts: work-groups first .. last, the slot of each.
+struct Parts {
+  int first, last, start, per;
+  int64_t base;
+  __device__ __forceinline__ Parts(const DecArgs& a, int h, int b) {
+    start = a.pre[b];
+    const int end = a.pre[b + 1];
+    per = a.pre[a.c.batch + 1];
+    first = start / per;
+    last = end > start ? (end - 1) / per : first;
+    base = (int64_t)h * a.groups * 2;
+  }
+  __device__ __forceinline__ bool whole() const { return first == last; }  // written by its work-group
+  __device__ __forceinline__ int64_t slot(int w) const { return base + 2 * w + ((int64_t)w * per >= start ? 0 : 1); }
+};
+
+// Joins a row that several work-groups share: a work-group a (row, query head), 16 parts at a time, 8
 // channels a thread.
-template <class T, bool WT>
-__global__ __launch_bounds__(256) void paged_join_kernel(DecArgs a) {
+template <class T>
+__device__ __forceinline__ void join_row(const DecArgs& a, int r, int h, int b) {
   __shared__ float part[16][16][10];  // 8 values, maximum, sum
-  const int r = blockIdx.x, h = blockIdx.y, b = blockIdx.z, rep = a.rep;
-  const int cc = threadIdx.x & 15, sl = threadIdx.x >> 4;
-  const int rs = a.pre[b], re = a.pre[b + 1], per = a.pre[a.c.batch + 1];
-  const int w0 = rs / per, w1 = re > rs ? (re - 1) / per : w0;
-  if (w0 == w1) return;  // written whole
+  const int rep = a.rep, cc = threadIdx.x & 15, sl = threadIdx.x >> 4;
+  const Parts parts(a, h, b);
+  if (parts.whole()) return;
   float m = kNegInf, l = 0.f, o[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) o[k] = 0.f;
-  for (int w = w0 + sl; w <= w1; w += 16) {
-    const int64_t slot = (((int64_t)h * a.groups + w) * 2 + ((int64_t)w * per >= rs ? 0 : 1)) * rep + r;
+  for (int w = parts.first + sl; w <= parts.last; w += 16) {
+    const int64_t slot = parts.slot(w) * rep + r;
     const float2 p = a.ml[slot];
     const float4v x = *(const float4v*)(a.acc + slot * 128 + cc * 8), y = *(const float4v*)(a.acc + slot * 128 + cc * 8 + 4);
     const float M = fmaxf(m, p.x), f0 = part_of(m, M), f1 = part_of(p.x, M);
@@ -591,25 +646,57 @@ __global__ __launch_bounds__(256) void paged_join_kernel(DecArgs a) {
     L += sum_in(part[w][pc][8], part[w][pc][9], M);
     v = fmaf(part_of(part[w][pc][8], M), part[w][pc][pk], v);
   }
-  const int64_t oh = (int64_t)b * a.q_heads + h * rep + r;
-  a.out[oh * 128 + ch] = (uint16_t)T::pack(v * inverse_of(M, L), 0.f);
-  if (WT && ch == 0) a.lse[oh] = log_of(M, L);
+  a.out[((int64_t)b * a.q_heads + h * rep + r) * 128 + ch] = (uint16_t)T::pack(v * inverse_of(M, L), 0.f);
 }
 
-// weights[b,g,t] += sum_h p_h(t) from the stored scores and the rows' denominators; half a wave a tile
-__global__ __launch_bounds__(256) void paged_weights_kernel(DecArgs a) {
-  const int h = blockIdx.y, b = blockIdx.z, rep = a.rep;
-  const int n = row_len(a, b);
+// weights[b,g,t] += sum_h p_h(t) from the stored scores and the rows' denominators: eight tiles a work-group, half
+// a wave each
+__device__ __forceinline__ void add_weights(const DecArgs& a, int chunk, int h, int b) {
+  __shared__ float lse[kHeads];
+  const int rep = a.rep, n = row_len(a, b);
   const RowTiles rt(n, a.window, a.sinks);
-  const int i = blockIdx.x * 8 + (threadIdx.x >> 5), u = threadIdx.x & 31;
+  if (chunk * 8 >= rt.count) return;
+  const int r = threadIdx.x >> 4, sl = threadIdx.x & 15;
+  bool whole = a.solo;
+  if (!whole) {
+    const Parts parts(a, h, b);
+    whole = parts.whole();
+    if (!whole && r < rep) {
+      float m = kNegInf, l = 0.f;
+      for (int w = parts.first + sl; w <= parts.last; w += 16) {
+        const float2 p = a.ml[parts.slot(w) * rep + r];
+        const float M = fmaxf(m, p.x);
+        l = sum_in(m, l, M) + sum_in(p.x, p.y, M);
+        m = M;
+      }
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) {
+        const float m2 = __shfl_xor(m, o, 16), l2 = __shfl_xor(l, o, 16), M = fmaxf(m, m2);
+        l = sum_in(m, l, M) + sum_in(m2, l2, M);
+        m = M;
+      }
+      if (sl == 0) lse[r] = log_of(m, l);
+    }
+  }
+  if (whole && sl == 0 && r < rep) lse[r] = a.lse[(int64_t)b * a.q_heads + h * rep + r];
+  __syncthreads();
+  const int i = chunk * 8 + (threadIdx.x >> 5), u = threadIdx.x & 31;
   if (i >= rt.count) return;
   const int tok = rt.token(i) + u;
   if (tok >= n) return;
   const float* s = a.scores + (h * a.tiles_cap + a.pre[b] + i) * (int64_t)rep * kTile + u;
   float* w = a.weights + b * a.wsb + h * a.wsh + tok;
   float p = 0.f;
-  for (int r = 0; r < rep; ++r) p += fast_exp2(s[r * kTile] - a.lse[(int64_t)b * a.q_heads + h * rep + r]);
+  for (int k = 0; k < rep; ++k) p += fast_exp2(s[k * kTile] - lse[k]);
   *w += p;
+}
+
+// What is left when every part is there, in one launch: the first `joins` work-groups of a (KV head, row) join its
+// query heads, the others add the weights.
+template <class T, bool WT>
+__global__ __launch_bounds__(256) void paged_finish_kernel(DecArgs a, int joins) {
+  if ((int)blockIdx.x < joins) join_row<T>(a, blockIdx.x, blockIdx.y, blockIdx.z);
+  else if constexpr (WT) add_weights(a, (int)blockIdx.x - joins, blockIdx.y, blockIdx.z);
 }
 
 // ---------------------------------------------------------------- host
@@ -677,18 +764,16 @@ int check(const kvq_paged_decode_params* p, PagedCache& c) {
 template <class T, bool I8, int GS, bool WT>
 int launch(const DecArgs& a, const Plan& w, hipStream_t st) {
   const int H = a.c.kv_heads, B = a.c.batch;
-  const size_t lds = 4 * 32 * 64 * 4 + (size_t)(2 * B + 1) * 4;
+  const size_t lds = 4 * 32 * 64 * 4 + (B > 64 ? (size_t)(B + 1) * 4 : 0);  // at most 49 KB
   const dim3 grid((unsigned)w.groups, (unsigned)H);
   if (w.solo) hipLaunchKernelGGL((paged_decode_kernel<T, I8, GS, WT, 8>), grid, dim3(512), lds, st, a);
   else hipLaunchKernelGGL((paged_decode_kernel<T, I8, GS, WT, 4>), grid, dim3(256), lds, st, a);
   int rc = launched();
   if (rc) return rc;
-  if (!w.solo) {
-    hipLaunchKernelGGL((paged_join_kernel<T, WT>), dim3((unsigned)a.rep, (unsigned)H, (unsigned)B), dim3(256), 0, st, a);
-    if ((rc = launched())) return rc;
-  }
-  if (WT) {
-    hipLaunchKernelGGL(paged_weights_kernel, dim3((unsigned)((w.max_tiles + 7) / 8), (unsigned)H, (unsigned)B), dim3(256), 0, st, a);
+  const int joins = w.solo ? 0 : a.rep;
+  const int64_t chunks = WT ? (w.max_tiles + 7) / 8 : 0;
+  if (joins + chunks > 0) {
+    hipLaunchKernelGGL((paged_finish_kernel<T, WT>), dim3((unsigned)(joins + chunks), (unsigned)H, (unsigned)B), dim3(256), 0, st, a, joins);
     rc = launched();
   }
   return rc;

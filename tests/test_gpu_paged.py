@@ -227,6 +227,38 @@ def test_decode_one_long_row_and_many_rows():
     run_decode([(i * 7919) % 1500 for i in range(90)], 2, 1, 16, BF16)
 
 
+@pytest.mark.parametrize("rows", [63, 64, 65, 127, 4096])
+@pytest.mark.parametrize("split", [False, True])
+@pytest.mark.parametrize("weights", [False, True])
+def test_decode_many_rows(rows, split, weights):
+    """Rows at and past a wave's lanes, up to the most of a call; a table of many columns has the rows' tiles shared
+    out over work-groups that know nothing of rows."""
+    K = _k()
+    print(f"[decode] rows {rows} split {split} weights {weights}", flush=True)
+    g = torch.Generator().manual_seed(rows)
+    lens = torch.randint(0, 49, (rows,), generator=g)
+    lens[torch.rand(rows, generator=g) < 0.3] = 0
+    lens[0], lens[-1] = 0, 48
+    lens = lens.tolist()
+    pool = Pool(lens, 1, 16, F16)
+    T = pool.cols * 16
+    vis = [visible(n, T, None, 0) for n in lens]
+    pool.fill(lambda b: vis[b]).cuda()
+    q = torch.randn(rows, 2, D, generator=g).to(F16)
+    table = torch.cat([pool.table, torch.full((rows, 70), -1, dtype=torch.int32, device=DEV)], 1) if split else pool.table
+    w = torch.zeros(rows, 1, table.shape[1] * 16, device=DEV) if weights else None
+    out = K.decode_attn_paged(q.to(DEV), pool.k, pool.v, table, torch.tensor(lens, dtype=torch.int32, device=DEV), SM, weights=w)
+    torch.cuda.synchronize()
+    kd, vd = pool.values()
+    for b in range(rows):
+        ref, tol, p, ptol = reference(q[b], kd[b], vd[b], vis[b], SM, F16, F16, 0)
+        check(out[b], ref, tol, ("row", b))
+        if weights:
+            got = w[b].double().cpu()
+            assert ((got[:, :T] - p).abs() - ptol - 2.0 ** -23 * p).max() <= 0, ("weights", b)
+            assert not got[:, T:].any()
+
+
 def test_decode_default_scale_and_long_lens():
     """No sm_scale means 1/sqrt(128); int64 lengths are taken; lengths past the table are clamped to it."""
     K = _k()
