@@ -39,7 +39,8 @@ struct DecArgs {
   int32_t min_tiles;   // least tiles of a work-group
   int32_t solo;        // a work-group takes one whole row: nothing to join
   // workspace
-  int32_t* pre;        // [batch + 1] tiles before each row, then the tiles of a work-group
+  int32_t* pre;        // [batch + 1] tiles before each row, the tiles of a work-group (negative: work-groups of one
+                       // row), [batch] the work-groups before each row
   float2* ml;          // [kv_heads][groups][2][rep] maximum (log2 units) and sum of a shared row's part:
                        // the first slot the part its tiles begin with, the second the part they end with
   float* acc;          // [kv_heads][groups][2][rep][128]
@@ -96,12 +97,12 @@ struct Rows {
 };
 
 __device__ __forceinline__ int scan64(int x) {  // inclusive, over the lanes
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(x, o, 64);
-    if (lane >= o) x += y;
-  }
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // 1, 2, 4, 8 lanes up in rows of 16
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // lane 15 to the row above, lane 31 to the half above
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
   return x;
 }
 
@@ -142,9 +143,31 @@ __device__ __forceinline__ Rows scan_rows(const DecArgs& a, int* lds, int* wsum)
   return r;
 }
 
-__device__ __forceinline__ int tiles_each(const DecArgs& a, int total) {
-  return max((total + a.groups - 1) / a.groups, a.min_tiles);
-}
+// How the rows' tiles are shared out.  `per` tiles a work-group over all rows laid end to end is even, but a
+// work-group that ends a row and begins another pays for two prologues and joins (3 to 5 us).  So work-groups of
+// one row each, its last one shorter, are taken where they fit with up to 3 more tiles (of 0.65 us) a work-group: 16
+// rows x 4 heads of 1500 tokens 16.1 us, end to end 18.4; of 5000 tokens 34.6 and 36.4; but 24 rows of 1500 tokens,
+// with 6 more tiles, 23.7 and 22.4.
+struct Share {
+  int per, parts;  // parts, lane b: those of the rows before row b
+  bool by_row;
+  __device__ __forceinline__ Share(const DecArgs& a, const Rows& rows) {
+    per = max((rows.total + a.groups - 1) / a.groups, a.min_tiles);
+    parts = 0;
+    by_row = false;
+    if (!rows.small || a.solo) return;
+    const int lane = threadIdx.x & 63, count = lane < a.c.batch ? RowTiles(rows.tokens, a.window, a.sinks).count : 0;
+#pragma unroll 1
+    for (int k = 0; k < 4; ++k) {
+      const int some = per + k, x = (count + some - 1) / some, y = scan64(x);
+      if (__builtin_amdgcn_readlane(y, 63) > a.groups) continue;
+      per = some;
+      parts = y - x;
+      by_row = true;
+      return;
+    }
+  }
+};
 
 // A running softmax: maximum (log2 units; -inf before the first finite score), sum.  While the maximum is
 // -inf the sum is not a sum: 1 if a token was seen (all its scores were -inf, the result is NaN), else 0.
@@ -204,16 +227,20 @@ __global__ __launch_bounds__(WAVES * 64, 2) void paged_decode_kernel(DecArgs a) 
   const PagedCache& pc = a.c;
 
   const Rows rows = scan_rows<WAVES * 64>(a, (int*)(lds + 4 * 32 * 64 * 4), wsum);
-  const int total = rows.total, per = tiles_each(a, total);
+  const int total = rows.total;
+  const Share share(a, rows);
   if ((WT || !a.solo) && blockIdx.x == 0 && h == 0) {
     if (rows.small) {
-      if (tid < pc.batch) a.pre[tid] = rows.before;
+      if (tid < pc.batch) {
+        a.pre[tid] = rows.before;
+        a.pre[pc.batch + 2 + tid] = share.parts;
+      }
     } else {
       for (int b = tid; b < pc.batch; b += WAVES * 64) a.pre[b] = rows.pre[b];
     }
     if (tid == 0) {
       a.pre[pc.batch] = total;
-      a.pre[pc.batch + 1] = per;
+      a.pre[pc.batch + 1] = share.by_row ? -share.per : share.per;
     }
   }
   // rows that see nothing
@@ -222,16 +249,20 @@ __global__ __launch_bounds__(WAVES * 64, 2) void paged_decode_kernel(DecArgs a) 
       for (int i = tid; i < rep * 64; i += WAVES * 64)
         ((uint32_t*)a.out)[((int64_t)b * a.q_heads + h * rep) * 64 + i] = 0;
 
-  int t, t1;
+  int t, t1, row = blockIdx.x;
   if (a.solo) {
-    t = rows.start(blockIdx.x);
-    t1 = rows.end(blockIdx.x, pc.batch);
+    t = rows.start(row);
+    t1 = rows.end(row, pc.batch);
+  } else if (share.by_row) {  // the last row whose parts begin here or before; those before the first row with any are 0
+    row = 63 - __builtin_clzll(__ballot(lane < pc.batch && share.parts <= (int)blockIdx.x));
+    t = rows.start(row) + ((int)blockIdx.x - __builtin_amdgcn_readlane(share.parts, row)) * share.per;
+    t1 = min(t + share.per, rows.end(row, pc.batch));
   } else {
-    t = (int)min((int64_t)blockIdx.x * per, (int64_t)total);
-    t1 = (int)min((int64_t)t + per, (int64_t)total);
+    t = (int)min((int64_t)blockIdx.x * share.per, (int64_t)total);
+    t1 = (int)min((int64_t)t + share.per, (int64_t)total);
+    if (t < t1) row = rows.of(t, pc.batch);
   }
   if (t >= t1) return;
-  int row = a.solo ? (int)blockIdx.x : rows.of(t, pc.batch);
 
   const uint8_t* const kh = pc.k + h * pc.ksh;
   const uint8_t* const vh = pc.v + h * pc.vsh;
@@ -599,9 +630,15 @@ struct Parts {
     start = a.pre[b];
     const int end = a.pre[b + 1];
     per = a.pre[a.c.batch + 1];
-    first = start / per;
-    last = end > start ? (end - 1) / per : first;
     base = (int64_t)h * a.groups * 2;
+    if (per < 0) {  // work-groups of one row: always their first part
+      first = a.pre[a.c.batch + 2 + b];
+      last = end > start ? first + (end - 1 - start) / -per : first;
+      start = per = 0;
+    } else {
+      first = start / per;
+      last = end > start ? (end - 1) / per : first;
+    }
   }
   __device__ __forceinline__ bool whole() const { return first == last; }  // written by its work-group
   __device__ __forceinline__ int64_t slot(int w) const { return base + 2 * w + ((int64_t)w * per >= start ? 0 : 1); }
@@ -701,9 +738,16 @@ __global__ __launch_bounds__(256) void paged_finish_kernel(DecArgs a, int joins)
 
 // ---------------------------------------------------------------- host
 
-constexpr int kTargetGroups = 512;  // work-groups of a launch: two of 4 waves a CU
-constexpr int kMinTiles = 8;
-constexpr int kSoloTiles = 32;
+// Measured on fp16 pages of 16 tokens, 7 query heads a KV head, 4 KV heads, us a call in a graph:
+// Work-groups of a launch, one of 4 waves a CU: 64 rows of 2048 tokens 49.3 (512: 52.2, 768: 57.2, 192: 63), 16 of
+// 8192 50.4 (51.2, 55.2, 59.4), 1 of 32768 19.8 (22.1, 22.2, 21.2).  8 waves in each: 50.2, 51.2, 20.5.
+constexpr int kTargetGroups = 256;
+// Least tiles of a work-group.  1 row of 1000 tokens 9.0 (4: 9.6, 8: 10.3, 16: 13), 4 of 700 9.7 (4: 12.6).
+constexpr int kMinTiles = 2;
+// Rows of at most these tiles are not split: one launch and no workspace.  At 512 tokens 1 row takes 10.0 us and 4
+// rows 12.5, split 9.1 and 9.8; but called one by one, where launches count, 10.0 and 13.6.  At 1000 tokens split
+// rows win both ways: 9.0 and 9.9 for 17.5 and 19.7.
+constexpr int kSoloTiles = 20;
 
 struct Plan {
   int64_t max_tiles;  // of a row
@@ -733,7 +777,7 @@ Plan plan_of(const kvq_paged_decode_params& p, bool weights) {
     w.bytes += (bytes + 63) / 64 * 64;
     return at;
   };
-  if (!w.solo || weights) w.pre = take(4 * (B + 2));
+  if (!w.solo || weights) w.pre = take(4 * (2 * B + 2));
   if (!w.solo) {
     w.ml = take(8 * H * w.groups * 2 * rep);
     w.acc = take(512 * H * w.groups * 2 * rep);
@@ -756,7 +800,7 @@ int check(const kvq_paged_decode_params* p, PagedCache& c) {
   if (p->q_heads / p->cache.kv_heads > kHeads) return fail(KVQ_ERR_UNSUPPORTED, "paged decode: more than 16 query heads a KV head");
   if (p->cache.batch > kMaxRows) return fail(KVQ_ERR_UNSUPPORTED, "paged decode: more than 4096 rows");
   if (p->cache.kv_heads > 65535) return fail(KVQ_ERR_UNSUPPORTED, "paged decode: too many heads");
-  if (((int64_t)p->cache.max_pages * p->cache.page_size / kTile + 1) * p->cache.batch > (1 << 30))
+  if (((int64_t)p->cache.max_pages * p->cache.page_size / kTile + 1) * p->cache.batch > (1 << 28))
     return fail(KVQ_ERR_UNSUPPORTED, "paged decode: too many token slots in a batch");
   return KVQ_OK;
 }

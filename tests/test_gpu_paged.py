@@ -259,6 +259,15 @@ def test_decode_many_rows(rows, split, weights):
             assert not got[:, T:].any()
 
 
+@pytest.mark.parametrize("dtype,int8", [(F16, 0), (BF16, 64)])
+@pytest.mark.parametrize("lens", [[600] * 13, [530, 0, 0, 1100, 40, 0, 640, 3, 1025, 0], [577] * 40, [0] * 20 + [900, 0, 1] * 12])
+def test_decode_shares_of_rows(dtype, int8, lens):
+    """Even and uneven rows, fewer and more of them than work-groups a KV head: work-groups of one row, and those
+    that end a row and begin another."""
+    for hq, hkv in ((5, 5), (16, 16)):
+        run_decode(lens, hq, hkv, 32, dtype, int8, weights=int8 == 0)
+
+
 def test_decode_default_scale_and_long_lens():
     """No sm_scale means 1/sqrt(128); int64 lengths are taken; lengths past the table are clamped to it."""
     K = _k()
