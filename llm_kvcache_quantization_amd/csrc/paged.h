@@ -21,6 +21,7 @@ typedef float float16v __attribute__((ext_vector_type(16)));
 // 16-bit element types: conversions round to nearest even (two values a v_cvt_pk)
 struct TF16 {
   using elem = half_t;
+  static constexpr uint32_t kInf = 0x7C00;
   __device__ __forceinline__ static float to_f(uint16_t b) { return (float)__builtin_bit_cast(half_t, b); }
   __device__ __forceinline__ static uint32_t pack(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((float2v{a, b}), half2v));
@@ -34,6 +35,7 @@ struct TF16 {
 };
 struct TB16 {
   using elem = bf16_t;
+  static constexpr uint32_t kInf = 0x7F80;
   __device__ __forceinline__ static float to_f(uint16_t b) { return __builtin_bit_cast(float, (uint32_t)b << 16); }
   __device__ __forceinline__ static uint32_t pack(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((float2v{a, b}), bf16x2));

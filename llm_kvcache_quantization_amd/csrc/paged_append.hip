@@ -28,8 +28,53 @@ struct AppArgs {
   int64_t rows;  // batch * heads * seq_new
 };
 
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h16x2 __attribute__((ext_vector_type(2)));
+
 template <int CTRL>
-__device__ __forceinline__ float dpp_max(float x) { return fmaxf(x, dppf<CTRL>(x)); }
+__device__ __forceinline__ uint32_t dpp_max(uint32_t x) {
+  return max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xf, 0xf, true));
+}
+
+// Codes of 8 values, and their group's scale: s = fp16(max(absmax, 1e-5) / 127), code = rint(fp16(x / s)) within
+// +-127; zeros and a NaN scale for a group that is not all finite.
+template <class T, int GS>
+__device__ __forceinline__ u32x2 encode(const u32x4& w, half_t& sc) {
+  // magnitudes order as their bits do, and those from Inf's on are not finite
+  u16x2 t = __builtin_bit_cast(u16x2, w[0] & 0x7FFF7FFFu);
+#pragma unroll
+  for (int j = 1; j < 4; ++j) t = __builtin_elementwise_max(t, __builtin_bit_cast(u16x2, w[j] & 0x7FFF7FFFu));
+  uint32_t top = max((uint32_t)t[0], (uint32_t)t[1]);
+  // over the group's lanes: quad_perm [1,0,3,2] and [2,3,0,1], then half-row and row mirrors
+  top = dpp_max<0xB1>(top);
+  top = dpp_max<0x4E>(top);
+  if (GS >= 64) top = dpp_max<0x141>(top);
+  if (GS >= 128) top = dpp_max<0x140>(top);
+  sc = (half_t)fminf(__fdiv_rn(fmaxf(T::to_f((uint16_t)top), 1e-5f), 127.0f), 65504.0f);
+  const float sf = (float)sc, inv = __fdiv_rn(1.f, sf);
+  uint32_t code[2] = {0, 0};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    h16x2 h;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      // x / s as the IEEE division has it, by one correction of x * (1 / s), which is within 2^-23: the remainder is
+      // exact, the corrected value within 2^-46 before its rounding, and a quotient of two 11-bit significands
+      // is no nearer than 2^-36 to a point between two floats.  (Where x is so small that the remainder underflows,
+      // or x / s so large that fp16 has no room for it, the code is 0 or 127 all the same.)
+      const float x = T::to_f((uint16_t)(w[j] >> 16 * k)), q = x * inv;
+      h[k] = (_Float16)__builtin_fmaf(__builtin_fmaf(-q, sf, x), inv, q);
+    }
+    h = __builtin_elementwise_min(__builtin_elementwise_max(h, (h16x2){-127, -127}), (h16x2){127, 127});
+#pragma unroll
+    for (int k = 0; k < 2; ++k) code[j >> 1] |= (uint32_t)(uint8_t)(int8_t)__builtin_rintf16(h[k]) << (16 * (j & 1) + 8 * k);
+  }
+  if (top >= T::kInf) {
+    code[0] = code[1] = 0;
+    sc = __builtin_bit_cast(half_t, (uint16_t)0x7E00);
+  }
+  return u32x2{code[0], code[1]};
+}
 
 template <class T, int GS>  // GS 0: rows as they are; else INT8 in groups of GS
 __global__ __launch_bounds__(kAppThreads) void paged_append_kernel(AppArgs a) {
@@ -43,47 +88,16 @@ __global__ __launch_bounds__(kAppThreads) void paged_append_kernel(AppArgs a) {
     const int64_t pos = (int64_t)a.write_pos[b] + i;
     if (a.new_lens && (int32_t)i >= a.new_lens[b]) continue;
     if (pos < 0 || pos >= ((int64_t)pc.max_pages << pc.lg)) continue;
+    const u32x4 w = *(const u32x4*)(s.x + b * s.sb + h * s.sh + i * s.ss + c * 16);
     const int32_t page = pc.table[b * pc.table_stride + (pos >> pc.lg)];
     if ((uint32_t)page >= (uint32_t)pc.num_pages) continue;
     const int32_t slot = (int32_t)pos & pc.page_mask;
-    const u32x4 w = *(const u32x4*)(s.x + b * s.sb + h * s.sh + i * s.ss + c * 16);
     uint8_t* dst = side ? pc.v + page * pc.vsp + h * pc.vsh + slot * pc.vst : pc.k + page * pc.ksp + h * pc.ksh + slot * pc.kst;
     if constexpr (GS == 0) {
       *(u32x4*)(dst + c * 16) = w;
     } else {
-      float x[8], top = 0.f;
-      bool odd = false;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        x[2 * j] = T::to_f((uint16_t)w[j]);
-        x[2 * j + 1] = T::to_f((uint16_t)(w[j] >> 16));
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float m = fabsf(x[j]);
-        odd |= !(m <= 3.4028234663852886e38f);
-        top = fmaxf(top, m);
-      }
-      // the groups of lanes: quad_perm [1,0,3,2] and [2,3,0,1], then half-row and row mirrors
-      float bad = odd ? 1.f : 0.f;
-      top = dpp_max<0xB1>(top); bad = dpp_max<0xB1>(bad);
-      top = dpp_max<0x4E>(top); bad = dpp_max<0x4E>(bad);
-      if (GS >= 64) { top = dpp_max<0x141>(top); bad = dpp_max<0x141>(bad); }
-      if (GS >= 128) { top = dpp_max<0x140>(top); bad = dpp_max<0x140>(bad); }
-      half_t sc = (half_t)fminf(__fdiv_rn(fmaxf(top, 1e-5f), 127.0f), 65504.0f);
-      const float sf = (float)sc;
-      uint32_t lo = 0, hi = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float q = rintf((float)(half_t)__fdiv_rn(x[j], sf));
-        const uint32_t code = (uint32_t)(uint8_t)(int8_t)(int)fminf(fmaxf(q, -127.f), 127.f);
-        if (j < 4) lo |= code << (8 * j); else hi |= code << (8 * (j - 4));
-      }
-      if (bad > 0.f) {
-        lo = hi = 0;
-        sc = __builtin_bit_cast(half_t, (uint16_t)0x7E00);
-      }
-      *(u32x2*)(dst + c * 8) = u32x2{lo, hi};
+      half_t sc;
+      *(u32x2*)(dst + c * 8) = encode<T, GS>(w, sc);
       constexpr int G = 128 / GS;
       if (c % (GS / 8) == 0) {
         uint8_t* so = side ? pc.vs + page * pc.vssp + h * pc.vssh : pc.ks + page * pc.kssp + h * pc.kssh;
