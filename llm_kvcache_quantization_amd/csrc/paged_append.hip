@@ -2,9 +2,11 @@
 //
 // 16 lanes take a token row of 128 values, 8 a lane: one 16-byte load, one store of 16 bytes (8 of
 // codes), so that a wave instruction moves four whole rows.  The group's absmax is DPP steps within the
-// 16 lanes.  The division is the IEEE one (the framework's codes rest on its rounding).
+// 16 lanes.
 //
-// What bounds it: a launch for a step's rows, HBM for prompts.
+// What bounds it: the launch for a step's rows (one token of 2 heads 2.3 us in the kernel); for prompts HBM and the
+// chain length, page, row (4 padded prompts of up to 4095 tokens, 8 heads, bf16 to INT8 of groups of 32: 19.6 us, where
+// a copy of their bytes takes 11.8).
 #include "paged.h"
 
 #pragma clang fp contract(off)
@@ -14,6 +16,7 @@ namespace {
 
 constexpr int kAppThreads = 256;
 constexpr int kAppRows = kAppThreads / 16;  // rows a work-group takes at a time
+constexpr int kAppTokens = 4 * kAppRows;    // tokens a work-group takes of a long prompt
 
 struct AppSide {
   const uint8_t* x;
@@ -76,7 +79,35 @@ __device__ __forceinline__ u32x2 encode(const u32x4& w, half_t& sc) {
   return u32x2{code[0], code[1]};
 }
 
+// The place of a row: its page (or none) and its slot.
+struct AppPlace {
+  int32_t page, slot;
+  __device__ __forceinline__ AppPlace(const PagedCache& pc, uint32_t b, int64_t pos, bool there) {
+    page = -1;
+    if (there && pos >= 0 && pos < ((int64_t)pc.max_pages << pc.lg)) page = pc.table[b * pc.table_stride + (pos >> pc.lg)];
+    slot = (int32_t)pos & pc.page_mask;
+  }
+};
+
 template <class T, int GS>  // GS 0: rows as they are; else INT8 in groups of GS
+__device__ __forceinline__ void put(const PagedCache& pc, int side, uint32_t h, const AppPlace& at, const u32x4& w, int c) {
+  if ((uint32_t)at.page >= (uint32_t)pc.num_pages) return;
+  uint8_t* dst = side ? pc.v + at.page * pc.vsp + h * pc.vsh + at.slot * pc.vst : pc.k + at.page * pc.ksp + h * pc.ksh + at.slot * pc.kst;
+  if constexpr (GS == 0) {
+    *(u32x4*)(dst + c * 16) = w;
+  } else {
+    half_t sc;
+    *(u32x2*)(dst + c * 8) = encode<T, GS>(w, sc);
+    constexpr int G = 128 / GS;
+    if (c % (GS / 8) == 0) {
+      uint8_t* so = side ? pc.vs + at.page * pc.vssp + h * pc.vssh : pc.ks + at.page * pc.kssp + h * pc.kssh;
+      ((half_t*)so)[at.slot * G + c / (GS / 8)] = sc;
+    }
+  }
+}
+
+// Few new tokens a sequence: the rows of all sequences and heads in one line, a row per 16 lanes.
+template <class T, int GS>
 __global__ __launch_bounds__(kAppThreads) void paged_append_kernel(AppArgs a) {
   const int side = blockIdx.y, c = threadIdx.x & 15;
   const AppSide s = a.side[side];
@@ -87,23 +118,36 @@ __global__ __launch_bounds__(kAppThreads) void paged_append_kernel(AppArgs a) {
     const uint32_t b = bh / (uint32_t)pc.kv_heads, h = bh % (uint32_t)pc.kv_heads;
     const int64_t pos = (int64_t)a.write_pos[b] + i;
     if (a.new_lens && (int32_t)i >= a.new_lens[b]) continue;
-    if (pos < 0 || pos >= ((int64_t)pc.max_pages << pc.lg)) continue;
     const u32x4 w = *(const u32x4*)(s.x + b * s.sb + h * s.sh + i * s.ss + c * 16);
-    const int32_t page = pc.table[b * pc.table_stride + (pos >> pc.lg)];
-    if ((uint32_t)page >= (uint32_t)pc.num_pages) continue;
-    const int32_t slot = (int32_t)pos & pc.page_mask;
-    uint8_t* dst = side ? pc.v + page * pc.vsp + h * pc.vsh + slot * pc.vst : pc.k + page * pc.ksp + h * pc.ksh + slot * pc.kst;
-    if constexpr (GS == 0) {
-      *(u32x4*)(dst + c * 16) = w;
-    } else {
-      half_t sc;
-      *(u32x2*)(dst + c * 8) = encode<T, GS>(w, sc);
-      constexpr int G = 128 / GS;
-      if (c % (GS / 8) == 0) {
-        uint8_t* so = side ? pc.vs + page * pc.vssp + h * pc.vssh : pc.ks + page * pc.kssp + h * pc.kssh;
-        ((half_t*)so)[slot * G + c / (GS / 8)] = sc;
-      }
+    put<T, GS>(pc, side, h, AppPlace(pc, b, pos, true), w, c);
+  }
+}
+
+// kAppTokens and more: a work-group takes as many consecutive tokens of a sequence and head, four rows a thread with
+// their loads side by side (the prompts above 19.6 us; in one line 21.4; two or eight rows a thread 19.7 and 23.8).
+template <class T, int GS>
+__global__ __launch_bounds__(kAppThreads) void paged_append_long_kernel(AppArgs a) {
+  constexpr int R = kAppTokens / kAppRows;
+  const int side = blockIdx.y, c = threadIdx.x & 15;
+  const AppSide s = a.side[side];
+  const PagedCache& pc = a.c;
+  const uint32_t chunks = (uint32_t)(a.seq_new + kAppTokens - 1) / kAppTokens, blocks = chunks * (uint32_t)(a.rows / a.seq_new);
+  for (uint32_t at = blockIdx.x; at < blocks; at += gridDim.x) {
+    const uint32_t i0 = at % chunks * kAppTokens, bh = at / chunks, b = bh / (uint32_t)pc.kv_heads, h = bh % (uint32_t)pc.kv_heads;
+    const int32_t n = a.new_lens ? min(a.new_lens[b], a.seq_new) : a.seq_new;
+    if ((int32_t)i0 >= n) continue;
+    const int64_t pos0 = a.write_pos[b];
+    const uint8_t* const x = s.x + b * s.sb + h * s.sh + c * 16;
+    u32x4 w[R];
+    int32_t i[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      i[r] = i0 + r * kAppRows + (threadIdx.x >> 4);
+      w[r] = *(const u32x4*)(x + min(i[r], n - 1) * s.ss);
     }
+    AppPlace place[R] = {{pc, b, pos0 + i[0], i[0] < n}, {pc, b, pos0 + i[1], i[1] < n}, {pc, b, pos0 + i[2], i[2] < n}, {pc, b, pos0 + i[3], i[3] < n}};
+#pragma unroll
+    for (int r = 0; r < R; ++r) put<T, GS>(pc, side, h, place[r], w[r], c);
   }
 }
 
@@ -128,16 +172,19 @@ int append(const kvq_paged_append_params* p, hipStream_t st) {
   a.write_pos = p->write_pos;
   a.new_lens = p->new_lens;
   a.seq_new = p->seq_new;
-  int64_t gx = (a.rows + kAppRows - 1) / kAppRows;
+  const bool lng = a.seq_new >= kAppTokens;
+  int64_t gx = lng ? a.rows / a.seq_new * ((a.seq_new + kAppTokens - 1) / kAppTokens) : (a.rows + kAppRows - 1) / kAppRows;
   if (gx > 65536) gx = 65536;
   const dim3 grid((unsigned)gx, 2), block(kAppThreads);
   const bool b16 = p->x_type == KVQ_PAGED_BF16;
   const int gs = fmt == KVQ_PAGED_INT8 ? p->cache.group_size : 0;
-#define KVQ_APP(T, G) hipLaunchKernelGGL((paged_append_kernel<T, G>), grid, block, 0, st, a)
-  if (gs == 0) KVQ_APP(TF16, 0);  // a copy of 16-bit values, whatever they are
-  else if (gs == 32) { if (b16) KVQ_APP(TB16, 32); else KVQ_APP(TF16, 32); }
-  else if (gs == 64) { if (b16) KVQ_APP(TB16, 64); else KVQ_APP(TF16, 64); }
-  else { if (b16) KVQ_APP(TB16, 128); else KVQ_APP(TF16, 128); }
+#define KVQ_APP(T, G)                                                            \
+  if (lng) hipLaunchKernelGGL((paged_append_long_kernel<T, G>), grid, block, 0, st, a); \
+  else hipLaunchKernelGGL((paged_append_kernel<T, G>), grid, block, 0, st, a)
+  if (gs == 0) { KVQ_APP(TF16, 0); }  // a copy of 16-bit values, whatever they are
+  else if (gs == 32) { if (b16) { KVQ_APP(TB16, 32); } else { KVQ_APP(TF16, 32); } }
+  else if (gs == 64) { if (b16) { KVQ_APP(TB16, 64); } else { KVQ_APP(TF16, 64); } }
+  else { if (b16) { KVQ_APP(TB16, 128); } else { KVQ_APP(TF16, 128); } }
 #undef KVQ_APP
   return launched();
 }

@@ -472,6 +472,40 @@ def test_append_values():
             run_append(1, 1, 6, 16, dtype, int8, [0], edit=edit)
 
 
+@pytest.mark.parametrize("dtype,int8", TYPES)
+def test_append_long(dtype, int8):
+    """Prompts of 64 and more new tokens: about the work-groups' share of them, padded, at the ends of the table."""
+    def table(t):
+        t[0, 2] = -1
+        t[1, 3] = 10 ** 6
+
+    for S in (63, 64, 65, 129):
+        run_append(2, 3, S, 16, dtype, int8, [0, 37])
+    run_append(4, 3, 150, 32, dtype, int8, [5, 0, 64, 31], lens=[150, 0, 65, 1], layout="bshd", pages="tokens")
+    run_append(2, 2, 100, 16, dtype, int8, [0, 3], slots=90, table=table, layout="odd")
+    run_append(3, 2, 70, 16, dtype, int8, [-3, -70, 2 ** 31 - 80], slots=80, lens=[70, -5, 1000])
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_append_every_value(dtype, group):
+    """Every 16-bit pattern beside a largest value of its group of each magnitude: the codes are those of the IEEE
+    quotient."""
+    bits = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(dtype)
+    g = torch.Generator().manual_seed(group)
+
+    def edit(k, v):
+        for x in (k, v):
+            rows = bits[torch.randperm(65536, generator=g)].view(4, 2, 64, D)
+            x.copy_(rows)
+            top = bits[torch.randint(0, 0x7800, (4, 2, 64, D // group), generator=g)]
+            keep = x.unflatten(-1, (-1, group)).abs() <= top.abs().unsqueeze(-1)
+            x.copy_(torch.where(keep, x.unflatten(-1, (-1, group)), top.unsqueeze(-1)).flatten(-2))
+
+    for seed in range(8):
+        run_append(4, 2, 64, 16, dtype, group, [0, 1, 2, 3], seed=seed, edit=edit)
+
+
 @pytest.mark.parametrize("group", [32, 64, 128])
 def test_append_codes_are_the_dense_engines(group):
     K = _k()
