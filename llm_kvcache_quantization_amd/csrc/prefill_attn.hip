@@ -76,8 +76,8 @@ __device__ __forceinline__ Row unit_of(const PreArgs& a, int64_t unit64) {
   uint32_t unit = (uint32_t)unit64;  // fewer than 2^31 of them
   r.split = (int)(unit % (uint32_t)a.splits);
   unit /= (uint32_t)a.splits;
-  // blocks from both ends in turn: any run of units has its share of the long ones (the later queries') and
-  // the short ones; rows of a batch in turn for the same reason
+  // blocks from both ends in turn: a part of them has its share of the long ones (the later queries') and the short
+  // ones; rows of a batch in turn for the same reason
   const int x = (int)(unit % (uint32_t)a.blocks);
   r.block = x & 1 ? x >> 1 : a.blocks - 1 - (x >> 1);
   unit /= (uint32_t)a.blocks;
@@ -88,6 +88,24 @@ __device__ __forceinline__ Row unit_of(const PreArgs& a, int64_t unit64) {
   r.off = r.kv_len - r.q_len;
   r.i0 = r.block * kBM;
   return r;
+}
+
+// The unit of a work-group, -1: none.  Work-groups go round the 8 XCDs; each XCD has a run of `per` units, whose heads
+// share K and V in its L2.  It takes them by the place of their queries, the last and longest first, so that short
+// ones are left for the end.  An XCD's work-groups go round its shader engines in turn, whatever those have left to
+// do: the (row, head)s shift by one from place to place, or long and short rows would each have engines of their own.
+// us, a (row, head) at a time / without the shift / so: 4 padded prompts of up to 2047 tokens, 40 heads, window 1024
+// 168 / 209 / 149; 8192 tokens, 28 heads, no window 717 / - / 516; 4 x 32 heads of 4096 tokens with K and V of their
+// own 780 / - / 680.
+__device__ __forceinline__ int64_t unit_at(const PreArgs& a, uint32_t at) {
+  const uint32_t xcd = at & 7, k = at >> 3, depth = (uint32_t)a.blocks * (uint32_t)a.splits;
+  const uint32_t per = (uint32_t)((a.units + 7) / 8), start = xcd * per, columns = (per + depth - 1) / depth;
+  const uint32_t d = k / columns, column = (k + d) % columns;
+  // the place of block (blocks - 1 - d / splits) in its (row, head), and that place's distance from the run's first
+  const uint32_t x = d / (uint32_t)a.splits, y = 2 * x < (uint32_t)a.blocks ? 2 * x : 2 * ((uint32_t)a.blocks - 1 - x) + 1;
+  const uint32_t z = y * (uint32_t)a.splits + d % (uint32_t)a.splits, z0 = start % depth;
+  const uint32_t u = column * depth + (z >= z0 ? z - z0 : z + depth - z0);
+  return u < per && start + u < (uint32_t)a.units ? (int64_t)(start + u) : -1;
 }
 
 __device__ __forceinline__ bool sees(int p, int key, int window, int sinks) {
@@ -464,10 +482,8 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(PreArgs a) {
   __shared__ LdsTile k0, v0, k1, v1;
   __shared__ uint32_t bad[2];
   const Lds s{k0, v0, k1, v1, bad};
-  // work-groups go round the 8 XCDs: each XCD gets a run of units, whose heads share K and V in its L2
-  const int64_t per = (a.units + 7) / 8;
-  const int64_t unit = (int64_t)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
-  if ((int64_t)(blockIdx.x >> 3) >= per || unit >= a.units) return;
+  const int64_t unit = unit_at(a, blockIdx.x);
+  if (unit < 0) return;
   if (attend_unit<T, false>(s, a, unit)) {
     const PreArgs again = a;
     attend_again<T>(&s, &again, unit);
@@ -503,7 +519,7 @@ constexpr int kMaxSplits = 32;
 
 struct Plan {
   int blocks, splits;
-  int64_t units, ml, bytes;
+  int64_t units, grid, ml, bytes;
 };
 
 Plan plan_of(const kvq_prefill_params& p) {
@@ -525,6 +541,8 @@ Plan plan_of(const kvq_prefill_params& p) {
   }
   w.splits = (int)s;
   w.units = whole * s;
+  const int64_t depth = w.blocks * s;
+  if (depth > 0) w.grid = 8 * (((w.units + 7) / 8 + depth - 1) / depth) * depth;  // whole (row, head)s an XCD
   if (s > 1) {
     w.ml = w.units * kBM * 128 * 4;
     w.bytes = w.ml + w.units * kBM * 8;
@@ -538,7 +556,8 @@ int check(const kvq_prefill_params* p) {
   if (p->q_heads % p->kv_heads) return fail(KVQ_ERR_INVALID, "prefill: q_heads must be a multiple of kv_heads");
   if (p->type != KVQ_PAGED_F16 && p->type != KVQ_PAGED_BF16) return fail(KVQ_ERR_INVALID, "prefill: unknown type");
   if (p->seq_q > (1 << 30) || p->seq_kv > (1 << 30)) return fail(KVQ_ERR_UNSUPPORTED, "prefill: more than 2^30 tokens");
-  if ((int64_t)p->batch * p->q_heads * ((p->seq_q + kBM - 1) / kBM) > (1 << 26)) return fail(KVQ_ERR_UNSUPPORTED, "prefill: too many queries");
+  if ((int64_t)p->batch * p->q_heads * ((p->seq_q + kBM - 1) / kBM) > (1 << 26) || plan_of(*p).grid >= (1 << 24))
+    return fail(KVQ_ERR_UNSUPPORTED, "prefill: too many queries");  // 2^32 threads are no launch
   return KVQ_OK;
 }
 
@@ -570,7 +589,7 @@ int prefill(const kvq_prefill_params* p, hipStream_t st) {
   a.part = (float*)p->workspace;
   a.ml = (float2*)((uint8_t*)p->workspace + w.ml);
   const bool b16 = p->type == KVQ_PAGED_BF16;
-  const dim3 grid((unsigned)((w.units + 7) / 8 * 8)), block(kThreads);
+  const dim3 grid((unsigned)w.grid), block(kThreads);
   if (b16) hipLaunchKernelGGL(prefill_kernel<TB16>, grid, block, 0, st, a);
   else hipLaunchKernelGGL(prefill_kernel<TF16>, grid, block, 0, st, a);
   if ((rc = launched())) return rc;
