@@ -22,7 +22,9 @@
 // work-group's result is not finite it runs again with such rows taken out of the products and added query by
 // query.
 //
-// What bounds it: the matrix units and the exponentials, about equally.
+// What bounds it: the matrix units (35% busy) and the vector units (45%, half of it exponentials), in turn in each
+// wave.  Measured: 16384 tokens through a window of 4096, 28 heads, bf16, 1000 us (842 TFLOP/s); 8192 tokens
+// without a window 516 us (930 TFLOP/s); a tile of 64 keys takes 2.5 us whether one or two work-groups share the CU.
 #include "paged.h"
 
 namespace kvq {
