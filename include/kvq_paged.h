@@ -29,7 +29,7 @@ extern "C" {
 #define KVQ_PAGED_INT8 2
 
 /* One layer's pages and the rows' page tables.  K and V rows are 128 values, contiguous; strides
- * are in bytes, multiples of 16 (8 for INT8 rows), as are the base addresses. */
+ * are in bytes, multiples of 16, as are the base addresses. */
 typedef struct kvq_paged_cache {
   void* k;
   void* v;

@@ -65,10 +65,11 @@ _APPEND, _DECODE, _PREFILL, _EVICT = (_packer(c) for c in (
     C.PagedAppendParams, C.PagedDecodeParams, C.PrefillParams, C.PagedEvictParams))
 
 
-
-
-def _no_grad() -> None:
-    raise NotImplementedError("the paged operators have no backward pass: call them under torch.no_grad()")
+def _no_grad(*tensors: Optional[Tensor]) -> None:
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise NotImplementedError("the paged operators have no backward pass: call them under torch.no_grad()")
 
 
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
@@ -221,8 +222,7 @@ def append_paged(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, block_t
         raise ValueError(f"k/v must lie on {device}, got {k.device} / {v.device}")
     if heads != k_pages.shape[1]:
         raise ValueError(f"k/v have {heads} heads, the pages {k_pages.shape[1]}")
-    if (k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
-        _no_grad()
+    _no_grad(k, v, k_pages, v_pages)
     pos = _i32(write_pos, "write_pos", batch, device)
     lens = None if new_lens is None else _i32(new_lens, "new_lens", batch, device)
     k, v = _rows16(k), _rows16(v)
@@ -257,8 +257,7 @@ def decode_attn_paged(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_table: 
         raise ValueError(f"q must lie on {device}, got {q.device}")
     if q_heads == 0 or q_heads % heads:
         raise ValueError(f"q_heads={q_heads} must be a multiple of kv_heads={heads}")
-    if q.requires_grad and torch.is_grad_enabled():
-        _no_grad()
+    _no_grad(q, k_pages, v_pages, inv_tau, weights)
     lens = _i32(context_lens, "context_lens", batch, device)
     window, sinks = _window(window, sinks)
     w = (0, 0, 0)
@@ -312,8 +311,7 @@ def prefill_attn_window(q: Tensor, k: Tensor, v: Tensor, sm_scale: Optional[floa
         raise ValueError(f"q, k and v must be all fp16 or all bf16, got {q.dtype} / {k.dtype} / {v.dtype}")
     if q_heads == 0 or heads == 0 or q_heads % heads:
         raise ValueError(f"q_heads={q_heads} must be a multiple of kv_heads={heads}")
-    if (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
-        _no_grad()
+    _no_grad(q, k, v, inv_tau)
     ql = None if q_lens is None else _i32(q_lens, "q_lens", batch, device)
     kl = None if kv_lens is None else _i32(kv_lens, "kv_lens", batch, device)
     window, sinks = _window(window, sinks)
@@ -356,6 +354,7 @@ def evict_paged(k_pages: Tensor, v_pages: Tensor, block_table: Tensor, context_l
                          f"got {weights.dtype} {tuple(weights.shape)} on {weights.device}")
     if weights.shape[2] > 1 and weights.stride(2) != 1:
         raise ValueError("weights must be contiguous over the tokens")
+    _no_grad(k_pages, v_pages, weights)
     if budget < 1 or sinks < 0 or recent < 0 or sinks + recent > budget:
         raise ValueError(f"budget must be positive and hold sinks + recent, got {budget}, {sinks} + {recent}")
     if budget >= 1 << 31:

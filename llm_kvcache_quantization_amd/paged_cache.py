@@ -31,7 +31,8 @@ class PagedKVCache(_EngineBase):
     ``num_pages`` fixes the pool (``RuntimeError`` when it is used up); without it the pool grows by doubling.
     ``max_seq_len`` bounds the tokens held of a sequence.  Layers share the block table: call them in the same
     order with the same token counts, as a model's forward does.  K and V are fp16 or bf16; float pages have their
-    type, INT8 pages take either.
+    type, INT8 pages take either.  What the engine keeps (pools, table, lengths) belongs to the stream it was made on:
+    use it on one stream, or make the other wait before and after.
     """
 
     def __init__(self, num_layers: int, device: str = "cuda", dtype: torch.dtype = torch.float16, page_size: int = 64,

@@ -274,6 +274,35 @@ def _step(pool, q, lens, w, new, budget=500):
     return (out, *K.evict_paged(*pool.args(), n, w, budget, sinks=4, recent=50))
 
 
+def test_no_gradients():
+    """Whatever would want a gradient is refused where autograd records, and taken as data where it does not."""
+    K = _k()
+    q = torch.randn(1, 2, 128, device=DEV, dtype=torch.float16)
+    pages = [torch.randn(3, 2, 16, 128, device=DEV, dtype=torch.float16) for _ in range(2)]
+    x = torch.randn(1, 2, 4, 128, device=DEV, dtype=torch.float16)
+    table, lens = torch.tensor([[2, 0]], dtype=torch.int32, device=DEV), torch.tensor([20], device=DEV)
+    w, tau = torch.zeros(1, 2, 32, device=DEV), torch.ones(2, device=DEV)
+
+    def calls(grad):
+        def g(name, t):
+            return t.clone().requires_grad_(name == grad)
+
+        k, v = g("k_pages", pages[0]), g("v_pages", pages[1])
+        return {"append": (lambda: K.append_paged(g("x", x), x, k, v, table, lens), ("x", "k_pages", "v_pages")),
+                "decode": (lambda: K.decode_attn_paged(g("q", q), k, v, table, lens, inv_tau=g("tau", tau), weights=g("w", w)),
+                           ("q", "k_pages", "v_pages", "tau", "w")),
+                "prefill": (lambda: K.prefill_attn_window(g("x", x), x, x, inv_tau=g("tau", tau)), ("x", "tau")),
+                "evict": (lambda: K.evict_paged(k, v, table, lens, g("w", w), 8), ("k_pages", "v_pages", "w"))}
+
+    for name in calls(""):
+        for grad in calls("")[name][1]:
+            with pytest.raises(NotImplementedError):
+                calls(grad)[name][0]()
+            with torch.no_grad():
+                calls(grad)[name][0]()
+    torch.cuda.synchronize()
+
+
 def test_other_streams_and_two_calls_at_once():
     print("[streams]", flush=True)
     want = []
