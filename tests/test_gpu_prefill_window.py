@@ -121,6 +121,31 @@ def test_padded_batches():
     run(3, 2, 1, 70, 70, F16, None, 0, [70, -4, 999], [40, 70, -1])
 
 
+@pytest.mark.parametrize("S,T", [(200, 200), (140, 3000)])  # one run over the keys, and split
+def test_padded_queries_are_zero_whatever_they_hold(S, T):
+    """Padding of NaN and Inf, behind sequences whose last query is finite, or sees a NaN itself."""
+    import llm_kvcache_quantization_amd as K
+
+    g = torch.Generator().manual_seed(S)
+    q, k, v = (torch.randn(3, n, t, 128, generator=g).to(F16).to(DEV) for n, t in ((4, S), (2, T), (2, T)))
+    ql, kl = [S - 5, 37, 131], [T, T - 7, T - 60]
+    kd, vd = k.clone(), v.clone()
+    for b, (m, n) in enumerate(zip(ql, kl)):
+        q[b, :, m:] = math.inf if b == 1 else math.nan
+        kd[b, :, n:] = math.nan
+        vd[b, :, n:] = math.nan
+    vd[2, :, kl[2] - 1] = math.nan  # the last query's own key
+    lens = [torch.tensor(x, device=DEV) for x in (ql, kl)]
+    out = K.prefill_attn_window(q, kd, vd, q_lens=lens[0], kv_lens=lens[1])
+    one = [K.prefill_attn_window(q[b : b + 1, :, :m], k[b : b + 1, :, :n], v[b : b + 1, :, :n]) for b, (m, n) in enumerate(zip(ql, kl))]
+    torch.cuda.synchronize()
+    for b, m in enumerate(ql):
+        assert not out[b, :, m:].any() and torch.isfinite(out[b, :, : m - 1]).all()
+        # the same products, perhaps split otherwise: P's rounding and the output's (2^-11 each, |v| < 5) on either side
+        assert (out[b, :, : m - 1].float() - one[b][0, :, : m - 1].float()).abs().max() <= 2 * 5 * 2.0 ** -10
+    assert torch.isfinite(out[:2]).all() and torch.isnan(out[2, :, ql[2] - 1]).all()
+
+
 @pytest.mark.parametrize("layout", ["bshd", "odd"])
 def test_layouts(layout):
     run(2, 6, 2, 140, 140, F16, 60, 4, layout=layout)
