@@ -278,13 +278,21 @@ struct Prefill {
   // the exponentials, the second half's K under the first half's product with V (the scheduling barriers keep
   // the compiler from moving the reads to their uses).
   __device__ __forceinline__ void tile(const LdsTile& ks, const LdsTile& vs, const PreArgs& a, const u32x4 (&q)[8], float scale,
-                                       int key0, int p, bool full) {
-    const float mul = full ? scale : 1.f;
+                                       int key0, int p, int pw0, int pw1) {
     u32x4 kf[8], vf[8], pb[2];
     read_k(ks, 0, kf);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
+      // the wave's queries see none of these 32 keys, or all of them, or some
+      const int kb = key0 + 32 * u;
+      if (pw1 < kb || (a.window > 0 && kb + 31 <= pw0 - a.window && kb >= a.sinks)) {
+        if (u == 0) read_k(ks, 1, kf);
+        continue;
+      }
+      const bool full = kb + 31 <= pw0 && (a.window <= 0 || kb > pw1 - a.window || kb + 32 <= a.sinks);
+      const float mul = full ? scale : 1.f;
+      seen |= full;
       float16v sc = scores(kf, q);
       read_v(vs, u, vf);
       __builtin_amdgcn_sched_barrier(0);
@@ -294,7 +302,6 @@ struct Prefill {
       __builtin_amdgcn_sched_barrier(0);
       add_values(vf, pb);
     }
-    seen |= full;
   }
 
   // The V rows taken out of the products: every lane scores its own query against the key again, and adds the
@@ -355,14 +362,11 @@ struct Prefill {
     l = 0.f;
     seen = false;
     if (t0 >= t1) return;
-    // what this wave's queries see of a tile: nothing, all, or some
     auto products = [&](const LdsTile& kc, const LdsTile& vc, int key0) {
       const bool none = pw1 < key0 || pw1 < pw0 ||
                         (a.window > 0 && key0 + kBN - 1 <= pw0 - a.window && key0 >= a.sinks);
-      const bool full = key0 + kBN - 1 <= pw0 &&
-                        (a.window <= 0 || key0 > pw1 - a.window || key0 + kBN <= a.sinks);
-      if (none) return;
-      tile(kc, vc, a, q, scale, key0, p, full);
+      if (none) return;  // this wave's queries see nothing of the tile
+      tile(kc, vc, a, q, scale, key0, p, pw0, pw1);
       if constexpr (ROBUST) add_bad(s, a, k, v, q, scale, key0, p, r.kv_len);
     };
     // this wave's loads have arrived, and then every wave's; the other buffer is free
