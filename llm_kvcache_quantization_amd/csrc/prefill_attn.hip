@@ -541,12 +541,21 @@ Plan plan_of(const kvq_prefill_params& p) {
     const int64_t some = ((int64_t)p.window + kBM + kBN - 1) / kBN + 1 + ((p.sinks > 0 ? p.sinks : 0) + kBN - 1) / kBN;
     if (some < tiles) tiles = some;
   }
+  // Fewer blocks than work-groups fit: the number of splits, of at least four tiles, that takes the least time by what
+  // was measured: a tile 2.3 us (1.75 where a work-group has its CU alone), a work-group's start 6, a join 3 and 0.016
+  // a part.  Against as many splits as fit at once, us: 1024 queries of 40 heads over 16384 keys 371 (476 in one), 4 x 300
+  // of 28 heads over 4096 118 (127), 1024 of 28 heads 29 (37); 512 of 28 heads over 4096 53 (in two rounds 67).
   int64_t s = 1;
   if (whole > 0 && whole < kTarget) {
-    s = kTarget / whole;
-    if (s > tiles / 4) s = tiles / 4;  // a split of fewer than four tiles costs more in the join than it gains
-    if (s > kMaxSplits) s = kMaxSplits;
-    if (s < 1) s = 1;
+    float least = 0;
+    for (int64_t n = 1; n == 1 || (n <= kMaxSplits && 4 * n <= tiles); ++n) {
+      const int64_t units = whole * n, rounds = (units + kTarget - 1) / kTarget;
+      const float us = rounds * ((tiles + n - 1) / n * (units <= kTarget / 2 ? 1.75f : 2.3f) + 6.f) + (n > 1 ? 3.f + 0.016f * units : 0.f);
+      if (n == 1 || us < least) {
+        least = us;
+        s = n;
+      }
+    }
   }
   w.splits = (int)s;
   w.units = whole * s;
