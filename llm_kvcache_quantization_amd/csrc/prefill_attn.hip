@@ -499,26 +499,48 @@ __global__ __launch_bounds__(kThreads, 2) void prefill_kernel(PreArgs a) {
   }
 }
 
-// Joins the splits of a block: a wave a query, two channels a lane.
+// Joins the splits of a block: a wave a query, two channels a lane.  A split's weight is worked out by the lane of its
+// number; their parts' loads are four side by side.
 template <class T>
 __global__ __launch_bounds__(256) void prefill_join_kernel(PreArgs a) {
   const int64_t unit = (int64_t)blockIdx.x * a.splits;
   const Row r = unit_of(a, unit);
   const int row = blockIdx.y * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63, i = r.i0 + row;
   if (i >= a.S) return;
-  float M = kNegInf, L = 0.f, x = 0.f, y = 0.f;
-  for (int s = 0; s < a.splits; ++s) M = fmaxf(M, a.ml[(unit + s) * kBM + row].x);
-  const float shift = M == kNegInf ? 0.f : M;
-  for (int s = 0; s < a.splits; ++s) {
-    const float2 p = a.ml[(unit + s) * kBM + row];
-    const float2 o = *(const float2*)(a.part + ((unit + s) * kBM + row) * 128 + 2 * lane);
-    const float f = fast_exp2(p.x - shift);
-    L += p.y * (M == kNegInf ? 1.f : f);
-    x = fmaf(o.x, f, x);
-    y = fmaf(o.y, f, y);
+  uint32_t result = 0;
+  if (i < r.q_len) {
+    const float2 ml = lane < a.splits ? a.ml[(unit + lane) * kBM + row] : float2{kNegInf, 0.f};
+    float M = ml.x, x = 0.f, y = 0.f;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+    const float f = fast_exp2(ml.x - (M == kNegInf ? 0.f : M));
+    float L = lane < a.splits ? ml.y * (M == kNegInf ? 1.f : f) : 0.f;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) L += __shfl_xor(L, o, 64);
+    const float* part = a.part + (unit * kBM + row) * 128 + 2 * lane;
+    int s = 0;
+    for (; s + 4 <= a.splits; s += 4) {
+      float2 o[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) o[u] = *(const float2*)(part + (int64_t)(s + u) * kBM * 128);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float fs = __shfl(f, s + u, 64);
+        x = fmaf(o[u].x, fs, x);
+        y = fmaf(o[u].y, fs, y);
+      }
+    }
+    for (; s < a.splits; ++s) {
+      const float2 o = *(const float2*)(part + (int64_t)s * kBM * 128);
+      const float fs = __shfl(f, s, 64);
+      x = fmaf(o.x, fs, x);
+      y = fmaf(o.y, fs, y);
+    }
+    // no maximum: nothing was seen (0), or all that was seen scored -inf (NaN)
+    const float inv = M == kNegInf && L == L ? (L > 0.f ? __builtin_nanf("") : 0.f) : 1.0f / L;
+    result = T::pack(x * inv, y * inv);
   }
-  const float inv = M == kNegInf && L == L ? (L > 0.f ? __builtin_nanf("") : 0.f) : 1.0f / L;
-  *(uint32_t*)(a.out + r.b * a.osb + r.h * a.osh + i * a.oss + 4 * lane) = i < r.q_len ? T::pack(x * inv, y * inv) : 0u;
+  *(uint32_t*)(a.out + r.b * a.osb + r.h * a.osh + i * a.oss + 4 * lane) = result;
 }
 
 // ---------------------------------------------------------------- host
