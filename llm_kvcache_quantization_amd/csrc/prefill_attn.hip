@@ -22,9 +22,9 @@
 // work-group's result is not finite it runs again with such rows taken out of the products and added query by
 // query.
 //
-// What bounds it: the matrix units (35% busy) and the vector units (45%, half of it exponentials), in turn in each
-// wave.  Measured: 16384 tokens through a window of 4096, 28 heads, bf16, 1000 us (842 TFLOP/s); 8192 tokens
-// without a window 516 us (930 TFLOP/s); a tile of 64 keys takes 2.5 us whether one or two work-groups share the CU.
+// What bounds it: the matrix units (42% busy) and the vector units (43%, half of it exponentials), in turn in each
+// wave.  Measured: 16384 tokens through a window of 4096, 28 heads, bf16, 938 us (898 TFLOP/s); 8192 tokens
+// without a window 506 us (950 TFLOP/s); a tile of 64 keys takes 1.75 us on a CU of its own, 2.3 where two share one.
 #include "paged.h"
 
 namespace kvq {
