@@ -287,6 +287,12 @@ class PagedKVCache(_EngineBase):
             raise ValueError(f"a decode step appends one token, got k {tuple(k.shape)}")
         if q.ndim != 3 or q.shape[0] != k.shape[0] or q.shape[1] % max(k.shape[1], 1):
             raise ValueError(f"q must be [B, Hq, {HEAD_DIM}] for k {tuple(k.shape)}, got {tuple(q.shape)}")
+        # refused before anything is appended
+        if q.shape[1] > 16 * k.shape[1]:
+            raise NotImplementedError(f"more than 16 query heads a KV head: {q.shape[1]} / {k.shape[1]}")
+        if q.shape[2] != HEAD_DIM or q.shape[1] == 0 or q.device != k.device or \
+                q.dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"q must be fp16 or bf16 [B, Hq, {HEAD_DIM}] on {k.device}, got {q.dtype} {tuple(q.shape)} on {q.device}")
         if self.dtype != torch.int8:  # the hook hands q over in fp16, K and V in the model's type
             q, k, v = q.to(self.dtype), k.to(self.dtype), v.to(self.dtype)
         self.append(layer_id, k, v)

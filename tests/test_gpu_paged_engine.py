@@ -202,6 +202,23 @@ def test_engine_refusals():
         c.prefill_attn(0, x[:, :, :3], x, x)
 
 
+def test_refused_step_appends_nothing():
+    K = _k()
+    eng = K.PagedKVCache(1, dtype=torch.int8)
+    k = torch.randn(2, 2, 5, 128, device=DEV, dtype=torch.float16)
+    eng.append(0, k, k)
+    one = k[:, :, :1]
+    for q, error in ((k.new_zeros(2, 34, 128), NotImplementedError), (k.new_zeros(2, 4, 64), ValueError),
+                     (k.new_zeros(2, 3, 128), ValueError), (torch.zeros(2, 4, 128), ValueError), (k.new_zeros(1, 4, 128), ValueError),
+                     (torch.zeros(2, 4, 128, device=DEV), ValueError)):
+        with pytest.raises(error):
+            eng.append_decode_attn(0, q, one, one)
+        assert eng.get_seq_lens(0) == [5, 5] and eng.get_seq_len() == 5
+    out = eng.append_decode_attn(0, k.new_zeros(2, 4, 128), one, one)
+    torch.cuda.synchronize()
+    assert eng.get_seq_lens(0) == [6, 6] and torch.isfinite(out).all()
+
+
 def test_operator_refusals():
     """What needs GPU tensors to be seen."""
     K = _k()
