@@ -453,21 +453,32 @@ def _attends_prompts(engine) -> bool:
     return callable(getattr(type(engine), "prefill_attn", None))
 
 
+def _says_causal(mask: torch.Tensor, q_len: int, past: int) -> bool:
+    """Whether a mask says what causal attention of q_len tokens after `past` others does anyway: [B, keys] all open, or
+    [..., q_len, past + q_len] open (True, or 0) for query i up to key past + i and closed behind it (False, or a bias of
+    -1e4 and less, whose weight e^-10000 is 0)."""
+    if mask.ndim == 2:
+        return bool(torch.all(mask == 1))
+    if mask.ndim < 2 or mask.shape[-2:] != (q_len, past + q_len):
+        return False
+    opened = torch.ones(q_len, past + q_len, dtype=torch.bool, device=mask.device).tril_(past)
+    if mask.dtype == torch.bool:
+        return bool(torch.all(mask == opened))
+    return mask.is_floating_point() and bool(torch.all(torch.where(opened, mask == 0, mask <= -1e4)))
+
+
 def _prefill_forward_impl(self, hidden_states, cache_wrapper, attention_mask=None, position_ids=None,
                           position_embeddings=None, return_cache=False):
     """A prompt, or a chunk of one, over an engine that attends prompts itself: projections, RoPE, the engine's
     ``prefill_attn``, output projection.  No counterpart in the reference, whose prompts run the model's own
     attention."""
-    if attention_mask is not None:
-        # a causal mask says nothing new, and its last row is open; padding is not in the engine's terms
-        seen = attention_mask if attention_mask.ndim == 2 else attention_mask[..., -1, :]
-        if not bool(torch.all(seen if seen.dtype == torch.bool else seen == (1 if attention_mask.ndim == 2 else 0))):
-            raise ValueError("an engine that attends prompts itself takes no padding or window mask: give its prefill_attn "
-                             "the lengths")
     layer_idx = getattr(cache_wrapper, "layer_idx", getattr(self, "layer_idx", 0))
     bsz, q_len, _ = hidden_states.shape
     q_heads, kv_heads, head_dim = _resolve_attn_shape_meta(self)
     engine = cache_wrapper.engine
+    if attention_mask is not None and not _says_causal(attention_mask, q_len, engine._layer_seq_lens[layer_idx]):
+        raise ValueError("an engine that attends prompts itself takes no padding or window mask, and no other that is not "
+                         "causal: give its prefill_attn the lengths")
     q = self.q_proj(hidden_states).view(bsz, q_len, q_heads, head_dim).transpose(1, 2)
     k = self.k_proj(hidden_states).view(bsz, q_len, kv_heads, head_dim).transpose(1, 2)
     v = self.v_proj(hidden_states).view(bsz, q_len, kv_heads, head_dim).transpose(1, 2)
