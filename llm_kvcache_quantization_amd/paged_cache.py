@@ -83,7 +83,7 @@ class PagedKVCache(_EngineBase):
     def _forget(self) -> None:
         n = self.num_layers
         self._held: List[List[int]] = [[] for _ in range(n)]   # tokens held of each sequence, per layer
-        self._seen: List[int] = [0] * n                        # tokens appended to the longest sequence
+        self._seen: List[List[int]] = [[] for _ in range(n)]   # tokens appended to each sequence, per layer
         self._rows: List[List[int]] = [[] for _ in range(self._batch)]  # pages of each sequence, -1: given back
         self._free: List[int] = list(range(self._total - 1, -1, -1))
         self._table: Optional[Tensor] = None
@@ -224,9 +224,9 @@ class PagedKVCache(_EngineBase):
         append_paged(k, v, kp, vp, table, self._device_ints(held, k.device),
                      None if lens is None else self._device_ints(counts, k.device), k_scale=ks, v_scale=vs)
         self._held[layer_id] = [h + c for h, c in zip(held, counts)]
-        self._seen[layer_id] += max(counts, default=0)
-        self._layer_seq_lens[layer_id] = self._seen[layer_id]
-        self._seq_len = max(self._seq_len, self._seen[layer_id])
+        self._seen[layer_id] = [s + c for s, c in zip(self._seen[layer_id] or [0] * batch, counts)]
+        self._layer_seq_lens[layer_id] = max(self._seen[layer_id], default=0)
+        self._seq_len = max(self._layer_seq_lens)
 
     def get_seq_lens(self, layer_id: int = 0) -> List[int]:
         """Tokens held of each sequence (``get_seq_len`` counts all that the longest was given, the position of
