@@ -202,19 +202,44 @@ class PagedKVCache(_EngineBase):
             w = self._weights[layer_id] = grown
         return w
 
+    # A call that is refused leaves the cache as it was: what an append changed is put back (slots behind the tokens
+    # held may hold anything, and a first call that did not come about fixes no batch).
+
+    def _state(self, layer_id: int) -> tuple:
+        return self._held[layer_id], self._seen[layer_id], self._batch
+
+    def _put_back(self, layer_id: int, state: tuple) -> None:
+        self._held[layer_id], self._seen[layer_id], batch = state
+        if not batch:
+            self._drop()
+            return
+        self._layer_seq_lens[layer_id] = max(self._seen[layer_id], default=0)
+        self._seq_len = max(self._layer_seq_lens)
+
     # ---------------------------------------------------------------- the cache
 
     def append(self, layer_id: int, k: Tensor, v: Tensor, lens: Optional[Sequence[int]] = None) -> None:
         """Appends k, v [B, Hkv, S, 128]; ``lens``: the real tokens of each sequence of a padded batch."""
         self._check(layer_id, k, v)
         batch, heads, seq, _ = k.shape
+        counts = self._counts(lens, batch, seq)
+        if not batch:
+            return
+        before = self._state(layer_id)
+        try:
+            self._append(layer_id, k, v, counts, lens is not None)
+        except BaseException:
+            self._put_back(layer_id, before)
+            raise
+
+    def _append(self, layer_id: int, k: Tensor, v: Tensor, counts: List[int], ragged: bool) -> None:
+        batch, heads = k.shape[:2]
         if not self._batch:
             self._batch, self._heads = batch, heads
             self._rows = [[] for _ in range(batch)]
             if self.num_pages is not None:
                 self._total = self.num_pages
                 self._free = list(range(self._total - 1, -1, -1))
-        counts = self._counts(lens, batch, seq)
         if layer_id == 0 and (self.window is not None or self.budget is not None):
             self._give_back()
         self._reserve(layer_id, counts, k.device)
@@ -222,7 +247,7 @@ class PagedKVCache(_EngineBase):
         kp, vp, ks, vs = self._pool(layer_id, k.device)
         table = self._block_table(k.device)
         append_paged(k, v, kp, vp, table, self._device_ints(held, k.device),
-                     None if lens is None else self._device_ints(counts, k.device), k_scale=ks, v_scale=vs)
+                     self._device_ints(counts, k.device) if ragged else None, k_scale=ks, v_scale=vs)
         self._held[layer_id] = [h + c for h, c in zip(held, counts)]
         self._seen[layer_id] = [s + c for s, c in zip(self._seen[layer_id] or [0] * batch, counts)]
         self._layer_seq_lens[layer_id] = max(self._seen[layer_id], default=0)
@@ -295,8 +320,13 @@ class PagedKVCache(_EngineBase):
             raise ValueError(f"q must be fp16 or bf16 [B, Hq, {HEAD_DIM}] on {k.device}, got {q.dtype} {tuple(q.shape)} on {q.device}")
         if self.dtype != torch.int8:  # the hook hands q over in fp16, K and V in the model's type
             q, k, v = q.to(self.dtype), k.to(self.dtype), v.to(self.dtype)
+        before = self._state(layer_id)
         self.append(layer_id, k, v)
-        out = self._attend_one(layer_id, q, sm_scale, inv_tau, self._layer_weights(layer_id, k.device))
+        try:
+            out = self._attend_one(layer_id, q, sm_scale, inv_tau, self._layer_weights(layer_id, k.device))
+        except BaseException:
+            self._put_back(layer_id, before)
+            raise
         self._evict(layer_id, self.slack)
         return out
 
@@ -315,17 +345,22 @@ class PagedKVCache(_EngineBase):
         kk, vv = k, v
         if any(held):
             kk, vv = self._with_past(layer_id, k, v, held, counts)
-        self.append(layer_id, k, v, lens)
         ragged = lens is not None or len(set(held)) > 1
         out = prefill_attn_window(
             q, kk, vv, sm_scale, window=self.window, sinks=self.sinks, inv_tau=inv_tau,
             q_lens=self._device_ints(counts, k.device) if ragged else None,
             kv_lens=self._device_ints([h + c for h, c in zip(held, counts)], k.device) if ragged else None)
+        before = self._state(layer_id)
+        self.append(layer_id, k, v, lens)
         if self.budget is not None and batch and seq:
-            last = self._device_ints([max(c - 1, 0) for c in counts], k.device).long()
-            ql = q.gather(2, last.view(-1, 1, 1, 1).expand(-1, q.shape[1], 1, HEAD_DIM)).squeeze(2)
-            self._attend_one(layer_id, ql, sm_scale, inv_tau, self._layer_weights(layer_id, k.device),
-                             [h if c else 0 for h, c in zip(self._held[layer_id], counts)])
+            try:
+                last = self._device_ints([max(c - 1, 0) for c in counts], k.device).long()
+                ql = q.gather(2, last.view(-1, 1, 1, 1).expand(-1, q.shape[1], 1, HEAD_DIM)).squeeze(2)
+                self._attend_one(layer_id, ql, sm_scale, inv_tau, self._layer_weights(layer_id, k.device),
+                                 [h if c else 0 for h, c in zip(self._held[layer_id], counts)])
+            except BaseException:
+                self._put_back(layer_id, before)
+                raise
             self._evict(layer_id, 0)
         return out
 

@@ -1,0 +1,65 @@
+"""PagedKVCache on the GPU: refused calls, layers in every order, bounds that bind in several layers, types.
+
+Attention is compared with float64 over what the cache should hold, with the tolerances derived in
+test_gpu_paged.py."""
+import math
+
+import pytest
+import torch
+
+from test_gpu_paged import BF16, F16, SM
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+D = 128
+
+
+def _k():
+    import llm_kvcache_quantization_amd as K
+
+    return K
+
+
+@pytest.mark.parametrize("budget", [None, 40])
+@pytest.mark.parametrize("dtype", [F16, torch.int8])
+def test_refused_prompts_and_steps_change_nothing(budget, dtype):
+    """A retry after a refusal gives what a cache that never saw the refused call gives, bit for bit."""
+    K = _k()
+    print(f"[refusals] {budget} {dtype}", flush=True)
+    g = torch.Generator(device=DEV).manual_seed(2)
+    c, clean = (K.PagedKVCache(1, device=DEV, dtype=dtype, page_size=16, budget=budget) for _ in range(2))
+    draw = lambda *s: torch.randn(*s, generator=g, device=DEV).half()  # noqa: E731
+    for S in (30, 25):
+        q, k, v = draw(2, 4, S, D), draw(2, 2, S, D), draw(2, 2, S, D)
+        bad = [dict(q=q.bfloat16()), dict(q=q.float()), dict(q=q.cpu()), dict(q=q[:, :3]), dict(q=q[..., :64]), dict(k=k[:, :1]),
+               dict(inv_tau=torch.ones(3, device=DEV)), dict(q=q.clone().requires_grad_()), dict(k=k.clone().requires_grad_()),
+               dict(lens=[S, S + 1]), dict(lens=[S]), dict(v=v.float()), dict(v=v[:, :, :-1])]
+        if budget:
+            bad.append(dict(q=torch.zeros(2, 34, S, D, device=DEV, dtype=F16)))
+        for kw in bad:
+            with pytest.raises((ValueError, NotImplementedError)):
+                c.prefill_attn(0, **dict(dict(q=q, k=k, v=v), **kw))
+            assert c.get_seq_lens() == clean.get_seq_lens() and c.get_seq_len() == clean.get_seq_len(), kw.keys()
+        assert torch.equal(c.prefill_attn(0, q, k, v, SM), clean.prefill_attn(0, q, k, v, SM))
+        for step in range(12):
+            q, k, v = draw(2, 4, D), draw(2, 2, 1, D), draw(2, 2, 1, D)
+            bad = [dict(q=q.float()), dict(q=q[:, :3]), dict(q=q.clone().requires_grad_()), dict(inv_tau=torch.ones(3, device=DEV)),
+                   dict(q=torch.zeros(2, 34, D, device=DEV, dtype=F16)), dict(inv_tau=torch.ones(4, device=DEV).requires_grad_()),
+                   dict(k=k.clone().requires_grad_()), dict(v=v[:, :1])]
+            with pytest.raises((ValueError, NotImplementedError)):
+                c.append_decode_attn(0, **dict(dict(q=q, k=k, v=v), **bad[step % len(bad)]))
+            assert c.get_seq_lens() == clean.get_seq_lens() and c.get_seq_len() == clean.get_seq_len(), step
+            assert torch.equal(c.append_decode_attn(0, q, k, v, SM), clean.append_decode_attn(0, q, k, v, SM)), step
+    for a, b in zip(c.get_kv(0), clean.get_kv(0)):
+        assert torch.equal(a, b)
+
+
+def test_refused_batch_of_too_many_rows():
+    K = _k()
+    c = K.PagedKVCache(1, device=DEV, page_size=16)
+    one = torch.zeros(4097, 1, 1, D, device=DEV, dtype=F16)
+    with pytest.raises(NotImplementedError, match="4096"):
+        c.append_decode_attn(0, one[:, :, 0], one, one)
+    assert c.get_seq_len() == 0
+    c.append(0, one[:2], one[:2])
+    assert c.get_seq_lens() == [1, 1]

@@ -75,3 +75,79 @@ def test_evicted_tokens_count_as_positions(calls):
     assert c.get_seq_lens() == [8, 3] and c.get_seq_len() == 20
     append(c, [1, 1])
     assert c.get_seq_len() == 21
+
+
+def snapshot(c):
+    return [list(h) for h in c._held], c.get_seq_len(), list(c._layer_seq_lens), c._batch
+
+
+def refuse(monkeypatch, name, after=0):
+    """From now on the operator refuses its calls, after so many that it takes."""
+    taken, left = getattr(M, name), [after]
+
+    def fn(*args, **kw):
+        if left[0] == 0:
+            raise ValueError("refused here")
+        left[0] -= 1
+        return taken(*args, **kw)
+
+    monkeypatch.setattr(M, name, fn)
+
+
+@pytest.mark.parametrize("budget", [None, 40])
+@pytest.mark.parametrize("held", [0, 13])
+@pytest.mark.parametrize("name", ["append_paged", "decode_attn_paged", "prefill_attn_window"])
+def test_a_refused_call_changes_nothing(calls, monkeypatch, budget, held, name):
+    """Whichever operator refuses a prompt, a chunk or a step, the cache is as it was, and one that has not begun takes
+    another batch."""
+    c = make(2, budget=budget)
+    if held:
+        append(c, [held, held])
+        append(c, [held, held], 1)
+    was = snapshot(c)
+    refuse(monkeypatch, name)
+    q, k = tensor(2, 4, 5, 128), tensor(2, 2, 5, 128)
+    tries = {"append_paged": ("append", "prompt", "step"), "decode_attn_paged": ("step",) + (("prompt",) if budget else ()),
+             "prefill_attn_window": ("prompt",)}[name]
+    for t in tries:
+        with pytest.raises(ValueError, match="refused here"):
+            if t == "append":
+                c.append(1, k, k)
+            elif t == "prompt":
+                c.prefill_attn(1, q, k, k, lens=[5, 2])
+            else:
+                c.append_decode_attn(1, q[:, :, 0], k[:, :, :1], k[:, :, :1])
+        assert snapshot(c) == was, t
+    monkeypatch.undo()
+    monkeypatch.setattr(M, "append_paged", lambda *a, **kw: None)
+    if held:
+        append(c, [1, 2], 1)
+        assert c.get_seq_lens(1) == [held + 1, held + 2]
+    else:
+        append(c, [4, 1, 7], heads=3)
+        assert c.get_seq_lens() == [4, 1, 7] and c._pools[0][0].shape[1] == 3
+
+
+def test_a_refused_first_call_fixes_no_batch(calls):
+    """Out of pages, or of max_seq_len, or with wrong lengths: the next call may bring another batch."""
+    for kw in (dict(num_pages=3), dict(max_seq_len=40)):
+        c = make(**kw)
+        with pytest.raises((RuntimeError, ValueError)):
+            append(c, [50, 50])
+        with pytest.raises(ValueError, match="token counts"):
+            append(c, [50, 50], seq=3)
+        assert snapshot(c) == ([[]], 0, [0], 0)
+        append(c, [30], heads=4)
+        assert c.get_seq_lens() == [30] and len(c._rows[0]) == 2
+    c = make(num_pages=3)
+    append(c, [], seq=5)  # no sequences: nothing to do, and nothing fixed
+    append(c, [48])
+    assert c._pools[0][0].shape[0] == 3
+
+
+def test_prompts_attend_before_they_append(calls):
+    c = make()
+    q, k = tensor(2, 4, 5, 128), tensor(2, 2, 5, 128)
+    c.prefill_attn(0, q, k, k)
+    assert [x[0] for x in calls] == ["prefill_attn_window", "append_paged"]
+    assert c.get_seq_lens() == [5, 5]
