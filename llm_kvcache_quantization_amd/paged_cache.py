@@ -306,8 +306,9 @@ class PagedKVCache(_EngineBase):
     def append_decode_attn(self, layer_id: int, q: Tensor, k: Tensor, v: Tensor, sm_scale: Optional[float] = None,
                            inv_tau: Optional[Tensor] = None) -> Tensor:
         """The decode step: appends one token a sequence, attends, and with a budget accumulates the weights and
-        evicts where a sequence has grown ``slack`` over it.  q [B, Hq, 128]; k, v [B, Hkv, 1, 128]; ``inv_tau`` as
-        given (the hook passes the engine's)."""
+        evicts where a sequence has grown ``slack`` over it.  q [B, Hq, 128], fp16 or bf16 whatever the pages (float pages
+        attend, and return, in their own type); k, v [B, Hkv, 1, 128] as ``append`` takes them; ``inv_tau`` as given
+        (the hook passes the engine's)."""
         if k.ndim != 4 or k.shape[2] != 1:
             raise ValueError(f"a decode step appends one token, got k {tuple(k.shape)}")
         if q.ndim != 3 or q.shape[0] != k.shape[0] or q.shape[1] % max(k.shape[1], 1):
@@ -318,8 +319,8 @@ class PagedKVCache(_EngineBase):
         if q.shape[2] != HEAD_DIM or q.shape[1] == 0 or q.device != k.device or \
                 q.dtype not in (torch.float16, torch.bfloat16):
             raise ValueError(f"q must be fp16 or bf16 [B, Hq, {HEAD_DIM}] on {k.device}, got {q.dtype} {tuple(q.shape)} on {q.device}")
-        if self.dtype != torch.int8:  # the hook hands q over in fp16, K and V in the model's type
-            q, k, v = q.to(self.dtype), k.to(self.dtype), v.to(self.dtype)
+        if self.dtype != torch.int8:  # q alone: what is stored has the pages' type already, or append refuses it
+            q = q.to(self.dtype)
         before = self._state(layer_id)
         self.append(layer_id, k, v)
         try:

@@ -151,3 +151,23 @@ def test_prompts_attend_before_they_append(calls):
     c.prefill_attn(0, q, k, k)
     assert [x[0] for x in calls] == ["prefill_attn_window", "append_paged"]
     assert c.get_seq_lens() == [5, 5]
+
+
+@pytest.mark.parametrize("pages", [torch.float16, torch.bfloat16, torch.int8])
+def test_a_step_takes_the_keys_that_append_takes(calls, pages):
+    """K and V of another type than the pages' are refused by a step as by an append; q is brought to float pages' type."""
+    for kt in (torch.float16, torch.bfloat16, torch.float32, torch.int32):
+        for qt in (torch.float16, torch.bfloat16):
+            c = make(dtype=pages)
+            q, k = tensor(2, 4, 128, dtype=qt), tensor(2, 2, 1, 128, dtype=kt)
+            if kt == pages or pages == torch.int8 and kt in (torch.float16, torch.bfloat16):
+                out = c.append_decode_attn(0, q, k, k)
+                assert out.dtype == (qt if pages == torch.int8 else pages)
+                stored = calls.named("append_paged")[-1][1]
+                assert stored[0].dtype == stored[1].dtype == kt
+            else:
+                for call in (lambda: c.append_decode_attn(0, q, k, k), lambda: c.append(0, k, k),
+                             lambda: c.append_decode_attn(0, q, tensor(2, 2, 1, 128, dtype=pages if pages != torch.int8 else torch.half), k)):
+                    with pytest.raises(ValueError, match="pages' type"):
+                        call()
+                    assert snapshot(c) == ([[]], 0, [0], 0)
