@@ -328,7 +328,7 @@ def _decode_attn_int8_torch_ref(q, k_int8, v_int8, k_scale, v_scale, context_len
 
 
 def _layer_inv_tau(engine, layer_idx: int, q_heads: int, device, dtype) -> Optional[torch.Tensor]:
-    """The engine's inv_tau[layer] in q's dtype, validated as the reference does
+    """The engine's inv_tau[layer] in `dtype`, validated as the reference does
     (src/engine/patch_model.py:711-746); None when temperature is off or absent."""
     inv_tau = getattr(engine, "inv_tau", None)
     if inv_tau is None or not getattr(engine, "use_attn_temperature", True):
@@ -382,7 +382,7 @@ def _fused_forward_impl(self, hidden_states, cache_wrapper, attention_mask=None,
         raise RuntimeError("Failed to obtain RoPE cos/sin for fused decode. "
                            "Check transformers version/model API (position_ids/position_embeddings).")
     q, k = _apply_rope(q, k, cos, sin)
-    tau = _layer_inv_tau(engine, layer_idx, q_heads, q.device, q.dtype)
+    tau = _layer_inv_tau(engine, layer_idx, q_heads, q.device, torch.float32 if _attends_prompts(engine) else q.dtype)
 
     sm_scale = float(getattr(self, "scaling", 1.0 / math.sqrt(head_dim)))
     decode_impl = getattr(engine, "decode_attn_impl", "triton_fused")
@@ -391,7 +391,9 @@ def _fused_forward_impl(self, hidden_states, cache_wrapper, attention_mask=None,
     q_kernel = q.squeeze(2)  # [B, Hq, D]
     try:
         if decode_impl in _HIP_IMPLS:
-            if q_kernel.dtype == torch.float16:
+            if _attends_prompts(engine):  # q as the prompts' is: in its own type, its temperature in fp32 in the kernel
+                out = engine.append_decode_attn(layer_idx, q_kernel, k, v, sm_scale=sm_scale, inv_tau=tau)
+            elif q_kernel.dtype == torch.float16:
                 out = engine.append_decode_attn(layer_idx, q_kernel, k, v, sm_scale=sm_scale, inv_tau=tau)
             else:
                 # the reference scales q in its own dtype, then the kernel casts it to fp16
@@ -492,7 +494,7 @@ def _prefill_forward_impl(self, hidden_states, cache_wrapper, attention_mask=Non
                            "Check transformers version/model API (position_ids/position_embeddings).")
     q, k = _apply_rope(q, k, cos, sin)
     out = engine.prefill_attn(layer_idx, q, k, v, sm_scale=float(getattr(self, "scaling", 1.0 / math.sqrt(head_dim))),
-                              inv_tau=_layer_inv_tau(engine, layer_idx, q_heads, q.device, q.dtype))
+                              inv_tau=_layer_inv_tau(engine, layer_idx, q_heads, q.device, torch.float32))
     attn_output = self.o_proj(out.transpose(1, 2).reshape(bsz, q_len, q_heads * head_dim).to(hidden_states.dtype))
     return (attn_output, None, cache_wrapper) if return_cache else (attn_output, None)
 

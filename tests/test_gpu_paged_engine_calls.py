@@ -63,3 +63,24 @@ def test_refused_batch_of_too_many_rows():
     assert c.get_seq_len() == 0
     c.append(0, one[:2], one[:2])
     assert c.get_seq_lens() == [1, 1]
+
+
+@pytest.mark.parametrize("pages", [BF16, torch.int8])
+def test_bf16_queries_of_a_step_beyond_fp16(pages):
+    """Queries of 2^20 against keys of 2^-20: a step attends as a prompt of the same token does."""
+    K = _k()
+    g = torch.Generator(device=DEV).manual_seed(3)
+    f = 2.0 ** 20 if pages == BF16 else 2.0 ** 10  # INT8 scales are fp16
+    q, k, v = (torch.randn(2, h, 40, D, generator=g, device=DEV) for h in (4, 2, 2))
+    q, k, v = (q * f * 2.0 ** 7).to(BF16), (k / f * 2.0 ** -7).to(BF16), v.to(BF16)
+    assert q.abs().max() > 65504
+    c = K.PagedKVCache(1, device=DEV, dtype=pages, page_size=16)
+    for i in range(40):
+        out = c.append_decode_attn(0, q[:, :, i], k[:, :, i : i + 1], v[:, :, i : i + 1], SM)
+    kd, vd = (x.double() for x in c.get_kv(0))
+    for h in range(4):
+        s = (kd[:, h // 2] * q[:, h, 39:40].double()).sum(-1) * SM
+        p = torch.softmax(s, -1)
+        want = (p.unsqueeze(-1) * vd[:, h // 2]).sum(1)
+        # the output's rounding (2^-8), P's in bf16 or fp16 and V's in fp16 (2^-8 at most each), all below |v| < 5
+        assert (out[:, h].double() - want).abs().max() <= 3 * 5 * 2.0 ** -8

@@ -99,3 +99,24 @@ def test_other_masks_are_refused(past):
         with pytest.raises(ValueError, match="padding"):
             prompt(mask, 7, past)
             raise AssertionError(f"mask {i} was taken")
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_steps_hand_over_what_prompts_do(dtype):
+    """q in the model's type, beyond fp16's range too, and the temperature beside it in fp32."""
+    tau = torch.rand(1, HQ) + 0.5
+    m = attention(dtype)
+    with torch.no_grad():
+        m.q_proj.weight.mul_(1e4 if dtype == torch.float16 else 1e6)
+    x = torch.randn(2, 1, 32).to(dtype)
+    rope = torch.ones(1, D), torch.zeros(1, D)
+    got = []
+    for forward in (P._prefill_forward_impl, P._fused_forward_impl):
+        engine = Engine(inv_tau=tau)
+        forward(m, x, types.SimpleNamespace(engine=engine, layer_idx=0), position_embeddings=rope)
+        got.append(engine.calls[0])
+    (q0, k0, v0, t0), (q1, k1, v1, t1) = got
+    assert q1.shape == (2, HQ, D) and q1.dtype == dtype and torch.equal(q1, q0[:, :, 0])
+    assert dtype == torch.float16 or q1.abs().max() > 65504 and torch.isfinite(q1).all()
+    assert torch.equal(k0, k1) and torch.equal(v0, v1)
+    assert t0.dtype == t1.dtype == torch.float32 and torch.equal(t0, tau[0]) and torch.equal(t1, tau[0])
