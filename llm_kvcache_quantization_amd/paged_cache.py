@@ -259,7 +259,13 @@ class PagedKVCache(_EngineBase):
         return list(self._held[layer_id])
 
     def get_paged_tensors(self, layer_id: int):
-        """(k_pages, v_pages, k_scale, v_scale, block_table, lens) as the operators take them."""
+        """(k_pages, v_pages, k_scale, v_scale, block_table, lens) as the operators take them: the pools themselves, the
+        table and the lengths as copies of the caller's own."""
+        *pool, table, lens = self._tensors(layer_id)
+        return (*pool, table.clone(), lens.clone())
+
+    def _tensors(self, layer_id: int) -> tuple:
+        """get_paged_tensors with the engine's own table and lengths, which other layers and calls share."""
         if not 0 <= layer_id < self.num_layers or not self._held[layer_id]:
             raise ValueError(f"Layer {layer_id} cache is empty")
         pool = self._pools[layer_id]
@@ -269,7 +275,7 @@ class PagedKVCache(_EngineBase):
     def get_kv(self, layer_id: int) -> Tuple[Tensor, Tensor]:
         """Dense K, V [B, Hkv, n, 128] of what is held (INT8: fp16 values), n the longest sequence's tokens; slots
         past a shorter sequence's end, and those of pages given back to the pool, are zero."""
-        kp, vp, ks, vs, table, _ = self.get_paged_tensors(layer_id)
+        kp, vp, ks, vs, table, _ = self._tensors(layer_id)
         held = self._held[layer_id]
         n = max(held, default=0)
         cols = -(-n // self.page_size)
@@ -292,7 +298,7 @@ class PagedKVCache(_EngineBase):
 
     def _attend_one(self, layer_id: int, q: Tensor, sm_scale: Optional[float], tau: Optional[Tensor],
                     weights: Optional[Tensor], held: Optional[List[int]] = None) -> Tensor:
-        kp, vp, ks, vs, table, lens = self.get_paged_tensors(layer_id)
+        kp, vp, ks, vs, table, lens = self._tensors(layer_id)
         if held is not None:
             lens = self._device_ints(held, q.device)
         return decode_attn_paged(q, kp, vp, table, lens, sm_scale, k_scale=ks, v_scale=vs, inv_tau=tau, window=self.window,
@@ -387,7 +393,7 @@ class PagedKVCache(_EngineBase):
         held = self._held[layer_id]
         if max(held, default=0) <= self.budget + slack:
             return
-        kp, vp, ks, vs, table, lens = self.get_paged_tensors(layer_id)
+        kp, vp, ks, vs, table, lens = self._tensors(layer_id)
         w = self._layer_weights(layer_id, kp.device)
         _, _, self._weights[layer_id] = evict_paged(kp, vp, table, lens, w, self.budget, sinks=self.sinks, recent=self.recent,
                                                     k_scale=ks, v_scale=vs)

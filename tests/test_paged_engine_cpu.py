@@ -171,3 +171,20 @@ def test_a_step_takes_the_keys_that_append_takes(calls, pages):
                     with pytest.raises(ValueError, match="pages' type"):
                         call()
                     assert snapshot(c) == ([[]], 0, [0], 0)
+
+
+def test_tensors_handed_out_are_the_callers(calls):
+    """Whoever counts on in the lengths, or edits the table, does not reach other layers' calls."""
+    c = make(2)
+    for layer in (0, 1):
+        append(c, [20, 7], layer)
+    *_, table, lens = c.get_paged_tensors(0)
+    want = table.clone()
+    lens += 1
+    table.fill_(-1)
+    for layer in (0, 1):
+        *_, t, n = c.get_paged_tensors(layer)
+        assert n.tolist() == [20, 7] and torch.equal(t, want)
+    c.decode_attn(1, tensor(2, 4, 128))
+    _, (_, _, _, t, n, _), _ = calls[-1]
+    assert n.tolist() == [20, 7] and torch.equal(t, want)
