@@ -727,6 +727,10 @@ __device__ __forceinline__ void add_weights(const DecArgs& a, int chunk, int h, 
   float* w = a.weights + b * a.wsb + h * a.wsh + tok;
   float p = 0.f;
   for (int k = 0; k < rep; ++k) p += fast_exp2(s[k * kTile] - lse[k]);
+  if (p != p) {  // a head's softmax is none: that is so for the tokens it sees, and adds nothing to the others of their tile
+    const int32_t page = a.c.table[b * a.c.table_stride + (tok >> a.c.lg)];
+    if ((uint32_t)page >= (uint32_t)a.c.num_pages || (tok < rt.lo && tok >= rt.sink_end)) return;
+  }
   *w += p;
 }
 
