@@ -18,10 +18,16 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float float2v __attribute__((ext_vector_type(2)));
 typedef float float16v __attribute__((ext_vector_type(16)));
 
-// 16-bit element types: conversions round to nearest even (two values a v_cvt_pk)
+// 16-bit element types: conversions round to nearest even (two values a v_cvt_pk).
+// kUp: where P = exp2(s - m) is rounded to the type, m lies this far below the largest score seen (log2 units; a score
+// 6 above that largest moves it).  P in fp16 then has room up to 2^15, and all its bits down to 23 below the largest score,
+// which is the sum's own precision.  With m at the largest, tokens 15 bits below it lose bits and those 25 below it are
+// lost to the product with V, and many of them are no small part (65536 tokens 25 bits below a first one: 2^-9).  bf16 has
+// fp32's range.
 struct TF16 {
   using elem = half_t;
   static constexpr uint32_t kInf = 0x7C00;
+  static constexpr float kUp = 9.f;
   __device__ __forceinline__ static float to_f(uint16_t b) { return (float)__builtin_bit_cast(half_t, b); }
   __device__ __forceinline__ static uint32_t pack(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((float2v{a, b}), half2v));
@@ -36,6 +42,7 @@ struct TF16 {
 struct TB16 {
   using elem = bf16_t;
   static constexpr uint32_t kInf = 0x7F80;
+  static constexpr float kUp = 0.f;
   __device__ __forceinline__ static float to_f(uint16_t b) { return __builtin_bit_cast(float, (uint32_t)b << 16); }
   __device__ __forceinline__ static uint32_t pack(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((float2v{a, b}), bf16x2));

@@ -171,8 +171,8 @@ struct Share {
   }
 };
 
-// A running softmax: maximum (log2 units; -inf before the first finite score), sum.  While the maximum is
-// -inf the sum is not a sum: 1 if a token was seen (all its scores were -inf, the result is NaN), else 0.
+// A running softmax: maximum (log2 units, kUp below the largest score; -inf before the first finite one), sum.  While the
+// maximum is -inf the sum is not a sum: 1 if a token was seen (all its scores were -inf, the result is NaN), else 0.
 __device__ __forceinline__ float shift_of(float m) { return m == kNegInf ? 0.f : m; }
 // the factor of a part with maximum m in a whole with maximum M
 __device__ __forceinline__ float part_of(float m, float M) { return fast_exp2(m - shift_of(M)); }
@@ -475,11 +475,11 @@ __global__ __launch_bounds__(WAVES * 64, 2) void paged_decode_kernel(DecArgs a) 
           *(float4v*)(so + 4) = float4v{s[4], s[5], s[6], s[7]};
         }
       }
-      // the maximum follows only where a score passes it by 2^6: P stays below 64, and the accumulators
-      // are seldom rescaled
+      // the maximum follows only where a score passes the largest before it by 2^6: P stays below 64 (2^15 in fp16),
+      // and the accumulators are seldom rescaled
       float mx = max8f(s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7]);
-      if (__any(mx > m + 6.f)) {
-        mx = fmaxf(wave_max_xor_groups(mx), m);
+      if (__any(mx > m + (6.f + M::kUp))) {
+        mx = fmaxf(wave_max_xor_groups(mx) - M::kUp, m);
         const float f = part_of(m, mx);
         l *= f;
 #pragma unroll

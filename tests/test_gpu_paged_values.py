@@ -50,3 +50,59 @@ def test_weights_of_tokens_that_are_not_seen(int8, slots):
             assert not nan.any() and (w[b][:, seen] > was[b][:, seen]).all()
         else:
             assert nan.all()
+
+
+def faint(n, bits, seed):
+    """K, V [1, n, 128] and q [2, 128] (float64): token 0 scores 0 and has no value, the others score `bits` (log2) below it, give
+    or take one, and have values around 1."""
+    g = torch.Generator().manual_seed(seed)
+    q = torch.ones(2, D, dtype=torch.float64)
+    f = math.log(2) / (D * SM)
+    k = (-(bits + 2 * torch.rand(n, 1, generator=g, dtype=torch.float64) - 1) * f).expand(n, D).clone()
+    v = 1 + 0.5 * torch.randn(n, D, generator=g, dtype=torch.float64)
+    k[0] = v[0] = 0
+    return q, k[None], v[None]
+
+
+def exact_and_tolerance(q, k, v, u_out, u_p, u_v, up):
+    """float64 attention of q [Hq, 128] over k, v [1, n, 128], and how far off a kernel may be, as derived in test_gpu_paged.py
+    but for P: in fp16 its steps below 2^-14 are 2^-24, and a score's P is 2^up times its share of the largest's at least, so
+    that it is off by 2^-25-up of it at most."""
+    s = q @ k[0].t() * SM
+    e = torch.exp(s - s.max())
+    p = e / e.sum(1, keepdim=True)
+    out, A = p @ v[0], p @ v[0].abs()
+    d = 130 * 2.0 ** -23 * float((q.abs() @ k[0].abs().t() * SM).max())
+    tol = u_out * out.abs() + (u_p + u_v + 2 * d + k.shape[1] * 2.0 ** -23 + 2.0 ** -20) * A
+    return out, tol + 2.0 ** (-25 - up) * v[0].abs().sum(0) / e.sum(1, keepdim=True) + 1e-12
+
+
+@pytest.mark.parametrize("dtype,int8", [(F16, 0), (F16, 32), (BF16, 128), (BF16, 0)])
+@pytest.mark.parametrize("n", [600, 65536])  # one work-group a row, and split
+@pytest.mark.parametrize("bits", [20, 25, 28])
+def test_decode_many_faint_tokens(dtype, int8, n, bits):
+    """A first token that takes nearly all the softmax and has no value: the result is what the many others add up to."""
+    K = _k()
+    print(f"[faint] decode {dtype} {int8} {n} {bits}", flush=True)
+    q, k, v = faint(n, bits, 7)
+    pool = Pool([n], 1, 64, dtype, int8)
+    T = pool.cols * 64
+    k, v = (torch.nn.functional.pad(x.to(dtype), (0, 0, 0, T - n)) for x in (k, v))
+    pool.dense_k, pool.dense_v = k[None], v[None]
+    if int8:
+        from test_gpu_paged import quantize
+
+        pool.ck, pool.sk = quantize(pool.dense_k, int8)
+        pool.cv, pool.sv = quantize(pool.dense_v, int8)
+    pool.fill(lambda b: visible(n, T, None, 0)).cuda()
+    w = torch.zeros(1, 1, T, device=DEV)
+    out = K.decode_attn_paged(q.to(dtype).to(DEV)[None], *pool.args(), torch.tensor([n], device=DEV), SM, **pool.scales(), weights=w)
+    kd, vd = (x[0, :, :n] for x in pool.values())
+    ref, tol = exact_and_tolerance(q, kd, vd, 2.0 ** -11 if dtype == F16 else 2.0 ** -8, 2.0 ** -8 if dtype == BF16 and not int8 else 2.0 ** -11,
+                                   2.0 ** -11 if int8 else 0, 100 if dtype == BF16 and not int8 else 9)
+    err = (out[0].double().cpu() - ref).abs()
+    assert (err <= tol).all(), (float((err / ref.abs()).max()), float((tol / ref.abs()).max()))
+    # the softmax itself is fp32 throughout
+    p = torch.softmax(q @ kd[0].t() * SM, 1).sum(0)
+    d = 130 * 2.0 ** -23 * float((q.abs() @ kd[0].abs().t() * SM).max())
+    assert ((w[0, 0, :n].double().cpu() - p).abs() <= p * (2 * d + n * 2.0 ** -23 + 2.0 ** -20)).all()
