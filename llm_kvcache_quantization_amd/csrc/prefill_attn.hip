@@ -250,13 +250,14 @@ struct Prefill {
     return s0 + s1;
   }
 
-  // While a lane's sum stays below 64 so does each of its P: the maximum follows only where it does not.
+  // While a lane's sum stays below 64 (2^15 in fp16) so does each of its P: the maximum, kUp below the largest score,
+  // follows only where it does not.
   __device__ __forceinline__ void add_sum(float sum, const float16v& sc, float mul, u32x4 (&pb)[2]) {
-    if (__any(!(sum <= 64.f) || m == kNegInf)) {
+    if (__any(!(sum <= 64.f * (1 << (int)T::kUp)) || m == kNegInf)) {
       float mx = kNegInf;
 #pragma unroll
       for (int j = 0; j < 16; ++j) mx = fmaxf(mx, sc[j] * mul);
-      mx = fmaxf(fmaxf(mx, xor32(mx)), m);
+      mx = fmaxf(fmaxf(mx, xor32(mx)) - T::kUp, m);
       const float f = fast_exp2(m - (mx == kNegInf ? 0.f : mx));
       l *= f;
 #pragma unroll

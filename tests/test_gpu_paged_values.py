@@ -67,14 +67,16 @@ def faint(n, bits, seed):
 def exact_and_tolerance(q, k, v, u_out, u_p, u_v, up):
     """float64 attention of q [Hq, 128] over k, v [1, n, 128], and how far off a kernel may be, as derived in test_gpu_paged.py
     but for P: in fp16 its steps below 2^-14 are 2^-24, and a score's P is 2^up times its share of the largest's at least, so
-    that it is off by 2^-25-up of it at most."""
+    that it is off by 2^-25-up of it at most.  An fp16 output below 2^-14 has steps of 2^-24 itself, so that rounding it is off by
+    up to 2^-25 whatever the kernel does: 2^-20 of a value around 1 lies there (bf16, of fp32's range, has no such end)."""
     s = q @ k[0].t() * SM
     e = torch.exp(s - s.max())
     p = e / e.sum(1, keepdim=True)
     out, A = p @ v[0], p @ v[0].abs()
     d = 130 * 2.0 ** -23 * float((q.abs() @ k[0].abs().t() * SM).max())
     tol = u_out * out.abs() + (u_p + u_v + 2 * d + k.shape[1] * 2.0 ** -23 + 2.0 ** -20) * A
-    return out, tol + 2.0 ** (-25 - up) * v[0].abs().sum(0) / e.sum(1, keepdim=True) + 1e-12
+    last = 2.0 ** -25 if u_out == 2.0 ** -11 else 0.0
+    return out, tol + 2.0 ** (-25 - up) * v[0].abs().sum(0) / e.sum(1, keepdim=True) + last + 1e-12
 
 
 @pytest.mark.parametrize("dtype,int8", [(F16, 0), (F16, 32), (BF16, 128), (BF16, 0)])
@@ -106,3 +108,20 @@ def test_decode_many_faint_tokens(dtype, int8, n, bits):
     p = torch.softmax(q @ kd[0].t() * SM, 1).sum(0)
     d = 130 * 2.0 ** -23 * float((q.abs() @ kd[0].abs().t() * SM).max())
     assert ((w[0, 0, :n].double().cpu() - p).abs() <= p * (2 * d + n * 2.0 ** -23 + 2.0 ** -20)).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("S,T", [(500, 500), (40, 700), (3, 40000)])  # whole, and split over the keys
+@pytest.mark.parametrize("bits", [20, 25, 28])
+def test_prompt_many_faint_tokens(dtype, S, T, bits):
+    K = _k()
+    print(f"[faint] prompt {dtype} {S} {T} {bits}", flush=True)
+    q, k, v = faint(T, bits, 8)
+    q, k, v = (x.to(dtype) for x in (q[:, None].expand(-1, S, -1), k, v))
+    out = K.prefill_attn_window(q[None].to(DEV), k[None].to(DEV), v[None].to(DEV), SM)[0].double().cpu()
+    for i in {0, 1, S // 2, S - 1}:
+        n = T - S + i + 1
+        ref, tol = exact_and_tolerance(q[:, i].double(), k[:, :n].double(), v[:, :n].double(), *[2.0 ** -11 if dtype == F16 else 2.0 ** -8] * 2,
+                                       0, 9 if dtype == F16 else 100)
+        err = (out[:, i] - ref).abs()
+        assert (err <= tol).all(), (i, float((err / ref.abs()).max()), float((tol / ref.abs()).max()))
