@@ -306,6 +306,8 @@ int evict(const kvq_paged_evict_params* p, hipStream_t st) {
     return fail(KVQ_ERR_INVALID, "paged evict: budget must be positive and hold sinks + recent");
   if ((int64_t)p->w_tokens < (int64_t)p->cache.max_pages * p->cache.page_size)
     return fail(KVQ_ERR_INVALID, "paged evict: fewer weights than token slots");
+  // places are counted on in 32 bits past the end by a work-group's share
+  if (p->budget > (1 << 30) || p->w_tokens > (1 << 30)) return fail(KVQ_ERR_UNSUPPORTED, "paged evict: a budget or weights of more than 2^30 tokens");
   if (B > 65535 || H > 65535) return fail(KVQ_ERR_UNSUPPORTED, "paged evict: too many rows or heads");
   if (B == 0) return KVQ_OK;
   if (!p->context_lens || !p->weights || !p->new_lens || !p->kept || !p->new_weights)

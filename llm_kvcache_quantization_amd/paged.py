@@ -357,8 +357,8 @@ def evict_paged(k_pages: Tensor, v_pages: Tensor, block_table: Tensor, context_l
     _no_grad(k_pages, v_pages, weights)
     if budget < 1 or sinks < 0 or recent < 0 or sinks + recent > budget:
         raise ValueError(f"budget must be positive and hold sinks + recent, got {budget}, {sinks} + {recent}")
-    if budget >= 1 << 31:
-        raise ValueError(f"budget too large: {budget}")
+    if budget > 1 << 30 or weights.shape[2] > 1 << 30:  # before an output of that size is made
+        raise ValueError(f"budget and weights may have at most 2^30 tokens, got {budget} and {weights.shape[2]}")
     new_lens = torch.empty_like(lens)
     kept = lens.new_empty((batch, heads, budget))
     new_weights = torch.empty_like(weights, memory_format=torch.contiguous_format)

@@ -1,0 +1,35 @@
+"""Limits of the paged operators that are refused on the host, on the CPU: sizes whose counters would leave 32 bits,
+lengths that do not fit int32, and what would carry a derivative."""
+import pytest
+import torch
+
+from test_paged_cpu import _cache, _evict, _lib, _refused
+
+
+class OnGpu(torch.Tensor):
+    """A CPU tensor that passes for one of a GPU: what is refused before anything is enqueued."""
+
+    is_cuda = True
+
+
+def gpu(x):
+    return x.as_subclass(OnGpu)
+
+
+def pages():
+    return gpu(torch.zeros(4, 2, 16, 128, dtype=torch.float16))
+
+
+def test_budgets_and_weights_past_2_30():
+    """A work-group's places pass the end by its share: they are counted in 32 bits."""
+    import llm_kvcache_quantization_amd as K
+
+    C, L = _lib()
+    c = _cache(C)
+    for over in (dict(budget=2 ** 31 - 1), dict(budget=2 ** 30 + 1), dict(w_tokens=2 ** 31 - 1), dict(w_tokens=2 ** 30 + 1)):
+        _refused(L, "kvq_paged_evict", _evict(C, c, **over))
+    k, table, lens = pages(), gpu(torch.zeros(1, 2, dtype=torch.int32)), gpu(torch.ones(1, dtype=torch.int32))
+    w = gpu(torch.zeros(1, 2, 32))
+    for budget in (2 ** 30 + 1, 2 ** 31 - 1, 2 ** 31, 2 ** 40):
+        with pytest.raises(ValueError, match="2.30"):
+            K.evict_paged(k, k, table, lens, w, budget)
