@@ -157,6 +157,8 @@ int append(const kvq_paged_append_params* p, hipStream_t st) {
   const int rc = paged_cache(p->cache, a.c);
   if (rc) return rc;
   if (p->seq_new < 0) return fail(KVQ_ERR_INVALID, "paged append: negative seq_new");
+  // a row holds no more, and places of a work-group's share past the end stay in 32 bits
+  if (p->seq_new > (1 << 30)) return fail(KVQ_ERR_UNSUPPORTED, "paged append: more than 2^30 new tokens");
   if (p->x_type != KVQ_PAGED_F16 && p->x_type != KVQ_PAGED_BF16) return fail(KVQ_ERR_INVALID, "paged append: unknown x_type");
   const int fmt = p->cache.format;
   if (fmt != KVQ_PAGED_INT8 && fmt != p->x_type) return fail(KVQ_ERR_INVALID, "paged append: the pages' type is another than the rows'");

@@ -3,7 +3,7 @@ lengths that do not fit int32, and what would carry a derivative."""
 import pytest
 import torch
 
-from test_paged_cpu import _cache, _evict, _lib, _refused
+from test_paged_cpu import _append, _cache, _evict, _lib, _refused
 
 
 class OnGpu(torch.Tensor):
@@ -33,3 +33,12 @@ def test_budgets_and_weights_past_2_30():
     for budget in (2 ** 30 + 1, 2 ** 31 - 1, 2 ** 31, 2 ** 40):
         with pytest.raises(ValueError, match="2.30"):
             K.evict_paged(k, k, table, lens, w, budget)
+
+
+def test_more_new_tokens_than_2_30():
+    """One row repeated 2^31 - 1 times is a view of 256 bytes: the places past its end wrapped to negative ones."""
+    C, L = _lib()
+    for n in (2 ** 30 + 1, 2 ** 31 - 1):
+        p = _append(C, _cache(C, batch=1, kv_heads=1), seq_new=n, k_stride_s=0, v_stride_s=0)
+        _refused(L, "kvq_paged_append", p)
+        assert b"2^30" in L.kvq_last_error()
