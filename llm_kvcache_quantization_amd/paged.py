@@ -44,6 +44,7 @@ from . import _capi as C
 
 HEAD_DIM = 128
 PAGE_SIZES = (16, 32, 64, 128, 256)
+_INTEGERS = (torch.int8, torch.uint8, torch.int16, torch.uint16, torch.int32, torch.uint32, torch.int64)
 _TYPES = {torch.float16: C.KVQ_PAGED_F16, torch.bfloat16: C.KVQ_PAGED_BF16}
 
 
@@ -88,8 +89,10 @@ def _i32(t: Tensor, name: str, batch: int, device: torch.device) -> Tensor:
     if t.ndim != 1 or t.shape[0] != batch:
         raise ValueError(f"{name} must be [B] = [{batch}], got {tuple(t.shape)}")
     if t.dtype != torch.int32 or t.device != device:
-        if t.is_floating_point() or t.dtype == torch.bool:
-            raise ValueError(f"{name} must be integers, got {t.dtype}")
+        if t.dtype not in _INTEGERS:
+            raise ValueError(f"{name} must be integers of at most 64 bits with a sign, got {t.dtype}")
+        if t.dtype in (torch.int64, torch.uint32):  # to int32's ends, which lie behind every table
+            t = t.to(torch.int64).clamp(-1 << 31, (1 << 31) - 1)
         t = t.to(device=device, dtype=torch.int32)
     return t.contiguous()
 

@@ -84,3 +84,23 @@ def test_bf16_queries_of_a_step_beyond_fp16(pages):
         want = (p.unsqueeze(-1) * vd[:, h // 2]).sum(1)
         # the output's rounding (2^-8), P's in bf16 or fp16 and V's in fp16 (2^-8 at most each), all below |v| < 5
         assert (out[:, h].double() - want).abs().max() <= 3 * 5 * 2.0 ** -8
+
+
+def test_lengths_in_64_bits():
+    """Lengths and positions of 2^32 and more are behind the table, not at their low 32 bits."""
+    K = _k()
+    g = torch.Generator(device=DEV).manual_seed(1)
+    k, v = (torch.randn(3, 2, 16, D, generator=g, device=DEV).half() for _ in range(2))
+    q = torch.randn(2, 4, D, generator=g, device=DEV).half()
+    table = torch.tensor([[2, 0], [1, 2]], dtype=torch.int32, device=DEV)
+    lens = torch.tensor([32, 9], device=DEV)
+    want = K.decode_attn_paged(q, k, v, table, lens.int())
+    far = torch.tensor([2 ** 32 + 5, 9], device=DEV)
+    assert torch.equal(K.decode_attn_paged(q, k, v, table, far), want)
+    assert not K.decode_attn_paged(q, k, v, table, far - 2 ** 40)[0].any()
+    x = torch.randn(2, 2, 4, D, generator=g, device=DEV).half()
+    was = k.clone()
+    K.append_paged(x, x, k, v, table, torch.tensor([2 ** 32, 2 ** 32 + 9], device=DEV))
+    assert torch.equal(k, was)
+    out = K.prefill_attn_window(x, x, x, q_lens=torch.tensor([2 ** 33, 2], device=DEV), kv_lens=torch.tensor([2 ** 32, 2], device=DEV))
+    assert torch.equal(out, K.prefill_attn_window(x, x, x, q_lens=torch.tensor([4, 2], device=DEV), kv_lens=torch.tensor([4, 2], device=DEV)))

@@ -42,3 +42,18 @@ def test_more_new_tokens_than_2_30():
         p = _append(C, _cache(C, batch=1, kv_heads=1), seq_new=n, k_stride_s=0, v_stride_s=0)
         _refused(L, "kvq_paged_append", p)
         assert b"2^30" in L.kvq_last_error()
+
+
+def test_lengths_that_do_not_fit_int32():
+    """They stand for what they say: behind every table, or in front of it."""
+    from llm_kvcache_quantization_amd.paged import _i32
+
+    cpu, far = torch.device("cpu"), [2 ** 32 + 5, -2 ** 40, 7, 2 ** 31, -2 ** 31 - 1, 2 ** 63 - 1]
+    got = _i32(torch.tensor(far), "lens", 6, cpu)
+    assert got.dtype == torch.int32 and got.tolist() == [2 ** 31 - 1, -2 ** 31, 7, 2 ** 31 - 1, -2 ** 31, 2 ** 31 - 1]
+    assert _i32(torch.tensor([2 ** 32 - 1, 5], dtype=torch.int64).to(torch.uint32), "lens", 2, cpu).tolist() == [2 ** 31 - 1, 5]
+    for t in (torch.int8, torch.uint8, torch.int16, torch.int32):
+        assert _i32(torch.tensor([3, 100], dtype=t), "lens", 2, cpu).tolist() == [3, 100]
+    for t in (torch.float32, torch.bool, torch.uint64, torch.complex64):
+        with pytest.raises(ValueError, match="integers"):
+            _i32(torch.zeros(2).to(t), "lens", 2, cpu)
