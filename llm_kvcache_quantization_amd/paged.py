@@ -24,7 +24,7 @@ tokens is not evicted.
 Everything is enqueued on the current stream of the tensors' device.  Scratch memory comes from torch's
 allocator, call by call, so that calls on several streams and captured graphs share none.  There is no
 backward pass: the operators serve inference, as the rest of this package does, and refuse tensors that
-require a gradient while gradients are recorded.
+require a gradient while gradients are recorded, and tensors with a tangent of forward differentiation.
 
 The reference has no counterpart: its caches are dense and unbounded (src/cache/int8_cache.py,
 src/cache/fp16_cache.py).
@@ -39,6 +39,7 @@ from typing import Optional, Tuple
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from . import _capi as C
 
@@ -67,10 +68,16 @@ _APPEND, _DECODE, _PREFILL, _EVICT = (_packer(c) for c in (
 
 
 def _no_grad(*tensors: Optional[Tensor]) -> None:
-    if torch.is_grad_enabled():
+    """Refuses tensors of a recorded graph, and those with a tangent: either derivative would be lost in silence."""
+    grad, dual = torch.is_grad_enabled(), forward_ad._current_level >= 0
+    if grad or dual:
         for t in tensors:
-            if t is not None and t.requires_grad:
+            if t is None:
+                continue
+            if grad and t.requires_grad:
                 raise NotImplementedError("the paged operators have no backward pass: call them under torch.no_grad()")
+            if dual and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError("the paged operators have no forward derivative: they take no tensor with a tangent")
 
 
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
@@ -225,7 +232,7 @@ def append_paged(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, block_t
         raise ValueError(f"k/v must lie on {device}, got {k.device} / {v.device}")
     if heads != k_pages.shape[1]:
         raise ValueError(f"k/v have {heads} heads, the pages {k_pages.shape[1]}")
-    _no_grad(k, v, k_pages, v_pages)
+    _no_grad(k, v, k_pages, v_pages, k_scale, v_scale)
     pos = _i32(write_pos, "write_pos", batch, device)
     lens = None if new_lens is None else _i32(new_lens, "new_lens", batch, device)
     k, v = _rows16(k), _rows16(v)
@@ -260,7 +267,7 @@ def decode_attn_paged(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_table: 
         raise ValueError(f"q must lie on {device}, got {q.device}")
     if q_heads == 0 or q_heads % heads:
         raise ValueError(f"q_heads={q_heads} must be a multiple of kv_heads={heads}")
-    _no_grad(q, k_pages, v_pages, inv_tau, weights)
+    _no_grad(q, k_pages, v_pages, k_scale, v_scale, inv_tau, weights)
     lens = _i32(context_lens, "context_lens", batch, device)
     window, sinks = _window(window, sinks)
     w = (0, 0, 0)
@@ -357,7 +364,7 @@ def evict_paged(k_pages: Tensor, v_pages: Tensor, block_table: Tensor, context_l
                          f"got {weights.dtype} {tuple(weights.shape)} on {weights.device}")
     if weights.shape[2] > 1 and weights.stride(2) != 1:
         raise ValueError("weights must be contiguous over the tokens")
-    _no_grad(k_pages, v_pages, weights)
+    _no_grad(k_pages, v_pages, k_scale, v_scale, weights)
     if budget < 1 or sinks < 0 or recent < 0 or sinks + recent > budget:
         raise ValueError(f"budget must be positive and hold sinks + recent, got {budget}, {sinks} + {recent}")
     if budget > 1 << 30 or weights.shape[2] > 1 << 30:  # before an output of that size is made

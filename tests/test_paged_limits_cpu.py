@@ -57,3 +57,40 @@ def test_lengths_that_do_not_fit_int32():
     for t in (torch.float32, torch.bool, torch.uint64, torch.complex64):
         with pytest.raises(ValueError, match="integers"):
             _i32(torch.zeros(2).to(t), "lens", 2, cpu)
+
+
+def test_tensors_with_a_tangent():
+    """Forward differentiation, whether or not gradients are recorded."""
+    from torch.autograd import forward_ad
+
+    import llm_kvcache_quantization_amd as K
+
+    k, table, lens = pages(), gpu(torch.zeros(1, 2, dtype=torch.int32)), gpu(torch.ones(1, dtype=torch.int32))
+    q, x, w, tau = (torch.randn(s) for s in ((1, 4, 128), (1, 2, 3, 128), (1, 2, 32), (4,)))
+    q, x = q.half(), x.half()
+    with forward_ad.dual_level():
+        dual = lambda t: gpu(forward_ad.make_dual(t, torch.ones_like(t)))  # noqa: E731
+        x0, q0 = gpu(x), gpu(q)
+        for call in (lambda: K.append_paged(dual(x), x0, k, k, table, lens),
+                     lambda: K.decode_attn_paged(dual(q), k, k, table, lens),
+                     lambda: K.decode_attn_paged(q0, k, k, table, lens, inv_tau=dual(tau)),
+                     lambda: K.decode_attn_paged(q0, dual(torch.zeros(4, 2, 16, 128).half()), k, table, lens),
+                     lambda: K.prefill_attn_window(gpu(x.repeat(1, 2, 1, 1)), dual(x), x0),
+                     lambda: K.evict_paged(k, k, table, lens, dual(w), 1)):
+            for recorded in (True, False):
+                with torch.set_grad_enabled(recorded), pytest.raises(NotImplementedError, match="tangent"):
+                    call()
+
+
+def test_scales_that_want_a_gradient():
+    import llm_kvcache_quantization_amd as K
+
+    i8 = gpu(torch.zeros(4, 2, 16, 128, dtype=torch.int8))
+    table, lens = gpu(torch.zeros(1, 2, dtype=torch.int32)), gpu(torch.ones(1, dtype=torch.int32))
+    q, x, w = (gpu(torch.zeros(s).half()) for s in ((1, 4, 128), (1, 2, 3, 128), (1, 2, 32)))
+    for side in ("k_scale", "v_scale"):
+        sc = {n: gpu(torch.ones(4, 2, 16, 4).half().requires_grad_(n == side)) for n in ("k_scale", "v_scale")}
+        for call in (lambda: K.append_paged(x, x, i8, i8, table, lens, **sc), lambda: K.decode_attn_paged(q, i8, i8, table, lens, **sc),
+                     lambda: K.evict_paged(i8, i8, table, lens, w.float(), 1, **sc)):
+            with pytest.raises(NotImplementedError, match="backward"):
+                call()
