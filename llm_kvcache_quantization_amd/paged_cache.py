@@ -29,8 +29,10 @@ class PagedKVCache(_EngineBase):
     """A paged cache of fp16, bf16 or INT8 pages (``dtype``; INT8 with fp16 scales per (token, ``group_size``)).
 
     ``num_pages`` fixes the pool (``RuntimeError`` when it is used up); without it the pool grows by doubling.
-    ``max_seq_len`` bounds the tokens held of a sequence.  Layers share the block table: call them in the same
-    order with the same token counts, as a model's forward does.  K and V are fp16 or bf16; float pages have their
+    ``max_seq_len`` bounds the tokens held of a sequence.  Layers share the
+    block table: call them in the same order with the same token counts, as a model's forward does (those in use: a
+    layer that never appends needs no pages, and one that begins late takes pages of its own for what the others
+    gave back).  K and V are fp16 or bf16; float pages have their
     type, INT8 pages take either.  What the engine keeps (pools, table, lengths) belongs to the stream it was made on:
     use it on one stream, or make the other wait before and after.
     """
@@ -85,6 +87,10 @@ class PagedKVCache(_EngineBase):
         self._held: List[List[int]] = [[] for _ in range(n)]   # tokens held of each sequence, per layer
         self._seen: List[List[int]] = [[] for _ in range(n)]   # tokens appended to each sequence, per layer
         self._rows: List[List[int]] = [[] for _ in range(self._batch)]  # pages of each sequence, -1: given back
+        self._gone: dict = {}                                  # sequence: its pages before this, but the sinks', are given back,
+        self._holes: dict = {}                                 # and some before this
+        self._lost: List[dict] = [{} for _ in range(n)]        # the same of a layer's tokens, whoever has taken pages there since
+        self._lead: Optional[int] = None                       # the layer that a step begins with
         self._free: List[int] = list(range(self._total - 1, -1, -1))
         self._table: Optional[Tensor] = None
         self._lens: dict = {}                                  # device copies of token counts, by value
@@ -124,27 +130,49 @@ class PagedKVCache(_EngineBase):
         return t
 
     def _give_back(self) -> None:
-        """Returns pages that no layer needs: behind the longest held length, or out of the window's sight."""
-        least = [min(h[b] for h in self._held if h) for b in range(self._batch)] if any(self._held) else []
-        most = [max(h[b] for h in self._held if h) for b in range(self._batch)] if any(self._held) else []
-        if any(not h for h in self._held):
-            return  # a layer has not begun
+        """Returns pages that no layer in use needs: behind the longest held length, or out of the window's sight.  (A layer
+        that begins later takes its own.)"""
+        begun = [h for h in self._held if h]
+        if not begun:
+            return
+        least = most = begun[0]
+        if any(h != least for h in begun):
+            least, most = [min(x) for x in zip(*begun)], [max(x) for x in zip(*begun)]
         ps, changed = self.page_size, False
-        for row, lo, hi in zip(self._rows, least, most):
+        for row, hi in zip(self._rows, most):
             while len(row) > -(-hi // ps):
                 page = row.pop()
                 changed = True
                 if page >= 0:
                     self._free.append(page)
-            if self.window is not None:
+        if self.window is not None:
+            keep = -(-self.sinks // ps)
+            for b, (row, lo) in enumerate(zip(self._rows, least)):
                 # the next query stands at lo or later and sees no token before lo + 1 - window but the sinks
-                for i in range(-(-self.sinks // ps), max(lo + 1 - self.window, 0) // ps):
+                end = max(lo + 1 - self.window, 0) // ps
+                for i in range(max(self._gone.get(b, 0), keep), end):
                     if row[i] >= 0:
                         self._free.append(row[i])
                         row[i] = -1
                         changed = True
+                if end > max(self._gone.get(b, 0), keep):
+                    self._gone[b] = end
+                    self._holes[b] = max(self._holes.get(b, 0), end)
+                    for held, lost in zip(self._held, self._lost):
+                        if held:
+                            lost[b] = max(lost.get(b, 0), end)
         if changed:
             self._table = None
+
+    def _needs(self, held: List[int], target: List[int]) -> List[Tuple[int, int]]:
+        """(sequence, place) of the pages that tokens held .. target - 1 lack: at the end of a row, and where a layer begins
+        in pages that were given back."""
+        ps, out = self.page_size, []
+        for b, (row, h, t) in enumerate(zip(self._rows, held, target)):
+            if h // ps < self._holes.get(b, 0):
+                out += [(b, i) for i in range(h // ps, min(len(row), -(-t // ps))) if row[i] < 0]
+            out += [(b, i) for i in range(len(row), -(-t // ps))]
+        return out
 
     def _reserve(self, layer_id: int, counts: List[int], device) -> None:
         """Pages for `counts` more tokens of each sequence."""
@@ -152,18 +180,23 @@ class PagedKVCache(_EngineBase):
         target = [h + c for h, c in zip(held, counts)]
         if self.max_seq_len is not None and max(target, default=0) > self.max_seq_len:
             raise ValueError(f"target_len {max(target)} exceeds max_seq_len {self.max_seq_len} for layer {layer_id}")
-        need = [max(0, -(-t // self.page_size) - len(r)) for t, r in zip(target, self._rows)]
-        if sum(need) > len(self._free):
+        need = self._needs(held, target)
+        if len(need) > len(self._free):
             self._give_back()
-            need = [max(0, -(-t // self.page_size) - len(r)) for t, r in zip(target, self._rows)]
-        short = sum(need) - len(self._free)
+            need = self._needs(held, target)
+        short = len(need) - len(self._free)
         if short > 0:
             if self.num_pages is not None:
-                raise RuntimeError(f"out of pages: {sum(need)} needed, {len(self._free)} of {self.num_pages} free")
+                raise RuntimeError(f"out of pages: {len(need)} needed, {len(self._free)} of {self.num_pages} free")
             self._grow(self._total + max(short, self._total))
-        if sum(need):
-            for row, n in zip(self._rows, need):
-                row.extend(self._free.pop() for _ in range(n))
+        for b, i in need:
+            row = self._rows[b]
+            if i == len(row):
+                row.append(self._free.pop())
+            else:
+                row[i] = self._free.pop()
+                self._gone[b] = min(self._gone.get(b, 0), i)
+        if need:
             self._table = None
 
     def _grow(self, total: int) -> None:
@@ -240,7 +273,9 @@ class PagedKVCache(_EngineBase):
             if self.num_pages is not None:
                 self._total = self.num_pages
                 self._free = list(range(self._total - 1, -1, -1))
-        if layer_id == 0 and (self.window is not None or self.budget is not None):
+        if self._lead is None:
+            self._lead = layer_id
+        if layer_id == self._lead and (self.window is not None or self.budget is not None):
             self._give_back()
         self._reserve(layer_id, counts, k.device)
         held = self._held[layer_id] or [0] * batch
@@ -254,8 +289,8 @@ class PagedKVCache(_EngineBase):
         self._seq_len = max(self._layer_seq_lens)
 
     def get_seq_lens(self, layer_id: int = 0) -> List[int]:
-        """Tokens held of each sequence (``get_seq_len`` counts all that the longest was given, the position of
-        its next token)."""
+        """Token slots of each sequence, those of pages given back among them (``get_seq_len`` counts all that the
+        longest was given, the position of its next token)."""
         return list(self._held[layer_id])
 
     def get_paged_tensors(self, layer_id: int):
@@ -283,6 +318,9 @@ class PagedKVCache(_EngineBase):
         slot = torch.arange(cols * self.page_size, device=t.device)
         there = (t >= 0).repeat_interleave(self.page_size, dim=1) & \
             (slot < self._device_ints(held, t.device).unsqueeze(1))
+        if self._lost[layer_id]:  # a layer that began later may have pages where this one gave its own back
+            lost = self._device_ints([self._lost[layer_id].get(b, 0) * self.page_size for b in range(self._batch)], t.device)
+            there &= (slot >= lost.unsqueeze(1)) | (slot < -(-self.sinks // self.page_size) * self.page_size)
 
         def dense(pages, scale):
             x = pages[t.clamp(min=0)]

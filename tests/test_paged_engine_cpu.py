@@ -188,3 +188,124 @@ def test_tensors_handed_out_are_the_callers(calls):
     c.decode_attn(1, tensor(2, 4, 128))
     _, (_, _, _, t, n, _), _ = calls[-1]
     assert n.tolist() == [20, 7] and torch.equal(t, want)
+
+
+# ---------------------------------------------------------------- pages given back
+
+
+def write(k, v, kp, vp, table, pos, lens=None, **kw):
+    """append_paged, token by token."""
+    for b in range(k.shape[0]):
+        for i in range(k.shape[2] if lens is None else int(lens[b])):
+            t = int(pos[b]) + i
+            page = int(table[b, t // kp.shape[2]])
+            assert page >= 0, "a token is written to a page that is not there"
+            kp[page, :, t % kp.shape[2]], vp[page, :, t % kp.shape[2]] = k[b, :, i], v[b, :, i]
+
+
+class Filled:
+    """A cache of layers whose token t of sequence b is (layer, b, t), and what each should still hold of them."""
+
+    def __init__(self, monkeypatch, layers, **kw):
+        monkeypatch.setattr(M, "append_paged", write)
+        self.c = make(layers, **kw)
+        self.n = [[0, 0, 0] for _ in range(layers)]
+
+    def append(self, layer, counts):
+        k = torch.zeros(3, 1, max(counts), 128)
+        for b, m in enumerate(counts):
+            k[b, 0, :m, 0], k[b, 0, :m, 1] = layer, b
+            k[b, 0, :m, 2] = torch.arange(self.n[layer][b], self.n[layer][b] + m)
+            self.n[layer][b] += m
+        k = k.half().as_subclass(OnGpu)
+        self.c.append(layer, k, -k, counts)
+        self.check()
+
+    def check(self):
+        c = self.c
+        owned = [p for r in c._rows for p in r if p >= 0]
+        assert len(owned) == len(set(owned)) and sorted(owned + c._free) == list(range(c._total))
+        for layer, lens in enumerate(self.n):
+            if not any(lens):
+                continue
+            assert c.get_seq_lens(layer) == lens
+            k, v = c.get_kv(layer)
+            assert torch.equal(k, -v)
+            for b, n in enumerate(lens):
+                t = torch.arange(k.shape[2])
+                there = k[b, 0, :, 0] + k[b, 0, :, 1] + k[b, 0, :, 2] != 0
+                right = (t < n) & (k[b, 0, :, 0] == layer) & (k[b, 0, :, 1] == b) & (k[b, 0, :, 2] == t)
+                # nothing but the tokens themselves, or zeros where pages were given back; what the next query sees is all there
+                assert (right | ~there).all(), (layer, b)
+                seen = (t < n) & ((t >= n + 1 - c.window) | (t < c.sinks)) if c.window else t < n
+                assert right[seen].all(), (layer, b)
+
+    def pages(self):
+        return [sum(p >= 0 for p in r) for r in self.c._rows]
+
+
+def test_layers_that_are_not_used_hold_no_pages_back(calls, monkeypatch):
+    """Only layers 1 and 3 of 4 append: the window gives pages back all the same, and a budget's eviction does."""
+    f = Filled(monkeypatch, 4, window=20, sinks=4)
+    for n in ([30, 5, 40], [30, 30, 0], [1, 1, 1], [100, 1, 60], [1, 1, 1]):
+        for layer in (1, 3):
+            f.append(layer, n)
+    # the next query sees the sinks' page and 20 tokens that end inside a page: 4 pages at most, and the last append's
+    assert max(f.pages()) <= 1 + 2 + 8 and f.pages()[1] <= 5
+    f.append(1, [1, 1, 1])
+    f.append(3, [1, 1, 1])
+    assert max(f.pages()) <= 4
+    c = make(4, budget=16, recent=4, slack=0)
+    for _ in range(3):
+        append(c, [60, 8], 2)
+        c._evict(2, 0)
+    append(c, [1, 1], 2)
+    assert [len(r) for r in c._rows] == [2, 2]
+
+
+def test_layers_one_after_the_other(calls, monkeypatch):
+    """Every chunk of a layer before the next layer's first: later layers take pages of their own where the first gave
+    back, in a fixed pool too."""
+    f = Filled(monkeypatch, 3, window=24, sinks=20, num_pages=40)
+    chunks = ([20, 50, 3], [40, 7, 0], [33, 33, 33], [1, 0, 1], [60, 2, 64], [1, 1, 1])
+    for layer in range(3):
+        for n in chunks:
+            f.append(layer, n)
+    for _ in range(40):
+        for layer in range(3):
+            f.append(layer, [1, 1, 1])
+    assert max(f.pages()) <= 2 + 3
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_pages_whatever_the_order(calls, monkeypatch, seed):
+    """Chunks and steps of three layers in orders of all kinds, layers that begin late among them."""
+    g = torch.Generator().manual_seed(seed)
+    pick = lambda n: int(torch.randint(0, n, (1,), generator=g))  # noqa: E731
+    f = Filled(monkeypatch, 3, window=(1, 5, 16, 33, 40, 7)[seed], sinks=(0, 3, 16, 17, 1, 40)[seed])
+    plan = [[pick(40), pick(40), pick(40)] if pick(2) else [1, 1, 1] for _ in range(25)]
+    plan = [n if max(n) else [1, 0, 0] for n in plan]
+    at = [0, 0, 0]
+    while min(at) < len(plan):
+        layer = pick(3) if seed % 2 else min(range(3), key=lambda x: (at[x] + (5 * x if at[x] == 0 and at[0] < 8 * x else 0), x))
+        if at[layer] < len(plan):
+            f.append(layer, plan[at[layer]])
+            at[layer] += 1
+
+
+def test_giving_back_looks_at_new_pages_only(calls):
+    """A step's bookkeeping does not grow with the tokens that a window has left behind."""
+    c = make(window=20)
+    append(c, [2000, 1, 1])
+    append(c, [1, 1, 1])
+    looked = []
+
+    class Row(list):
+        def __getitem__(self, i):
+            looked.append(i)
+            return list.__getitem__(self, i)
+
+    c._rows = [Row(r) for r in c._rows]
+    for _ in range(64):
+        append(c, [1, 1, 1])
+    assert 0 < len(looked) <= 2 * 3 * (64 // 16 + 1), looked  # whether a page is there, and which
