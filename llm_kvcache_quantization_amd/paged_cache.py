@@ -129,9 +129,9 @@ class PagedKVCache(_EngineBase):
             t = self._lens[key] = torch.tensor(values, dtype=torch.int32, device=device)
         return t
 
-    def _give_back(self) -> None:
-        """Returns pages that no layer in use needs: behind the longest held length, or out of the window's sight.  (A layer
-        that begins later takes its own.)"""
+    def _give_back(self, counts: Optional[List[int]] = None) -> None:
+        """Returns pages that no layer in use needs: behind the longest held length, or out of the window's sight now that
+        every sequence, or every one with `counts`, takes a token.  (A layer that begins later takes its own.)"""
         begun = [h for h in self._held if h]
         if not begun:
             return
@@ -149,7 +149,7 @@ class PagedKVCache(_EngineBase):
             keep = -(-self.sinks // ps)
             for b, (row, lo) in enumerate(zip(self._rows, least)):
                 # the next query stands at lo or later and sees no token before lo + 1 - window but the sinks
-                end = max(lo + 1 - self.window, 0) // ps
+                end = max(lo + (1 if counts is None or counts[b] else 0) - self.window, 0) // ps
                 for i in range(max(self._gone.get(b, 0), keep), end):
                     if row[i] >= 0:
                         self._free.append(row[i])
@@ -182,7 +182,7 @@ class PagedKVCache(_EngineBase):
             raise ValueError(f"target_len {max(target)} exceeds max_seq_len {self.max_seq_len} for layer {layer_id}")
         need = self._needs(held, target)
         if len(need) > len(self._free):
-            self._give_back()
+            self._give_back(counts)
             need = self._needs(held, target)
         short = len(need) - len(self._free)
         if short > 0:
@@ -276,7 +276,7 @@ class PagedKVCache(_EngineBase):
         if self._lead is None:
             self._lead = layer_id
         if layer_id == self._lead and (self.window is not None or self.budget is not None):
-            self._give_back()
+            self._give_back(counts)
         self._reserve(layer_id, counts, k.device)
         held = self._held[layer_id] or [0] * batch
         kp, vp, ks, vs = self._pool(layer_id, k.device)
@@ -344,6 +344,10 @@ class PagedKVCache(_EngineBase):
 
     def decode_attn(self, layer_id: int, q: Tensor, sm_scale: Optional[float] = None) -> Tensor:
         """Attention of q [B, Hq, 128] over the layer's cache as it is, with the engine's ``inv_tau``."""
+        if self.window is not None and 0 <= layer_id < self.num_layers:
+            for b, end in self._lost[layer_id].items():  # another layer's next token may have come already
+                if end * self.page_size > max(self._held[layer_id][b] - self.window, 0):
+                    raise RuntimeError(f"sequence {b} sees tokens whose pages were given back for its next one: append that first")
         tau = self.inv_tau[layer_id] if self.use_attn_temperature and self.inv_tau is not None else None
         return self._attend_one(layer_id, q, sm_scale, tau, None)
 

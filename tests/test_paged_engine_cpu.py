@@ -293,6 +293,23 @@ def test_pages_whatever_the_order(calls, monkeypatch, seed):
             at[layer] += 1
 
 
+def test_a_sequence_that_takes_nothing_keeps_what_it_sees(calls, monkeypatch):
+    """A row of a padded batch with no new token still sees `window` tokens: they stay, and one whose next token another
+    layer has taken already is refused."""
+    f = Filled(monkeypatch, 2, window=16)
+    for layer in (0, 1):
+        f.append(layer, [47, 47, 47])
+    f.append(0, [0, 1, 1])
+    # row 0 sees token 31, the last of page 1; the others' next query saw token 32 first
+    assert f.c._rows[0][0] < 0 <= f.c._rows[0][1] and f.c._rows[1][1] < 0
+    with pytest.raises(RuntimeError, match="sequence 1 "):
+        f.c.decode_attn(1, tensor(3, 2, 128))
+    f.c.decode_attn(0, tensor(3, 2, 128))
+    f.append(1, [0, 1, 1])
+    for layer in (0, 1):
+        f.c.decode_attn(layer, tensor(3, 2, 128))
+
+
 def test_giving_back_looks_at_new_pages_only(calls):
     """A step's bookkeeping does not grow with the tokens that a window has left behind."""
     c = make(window=20)
