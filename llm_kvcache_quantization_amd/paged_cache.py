@@ -29,7 +29,7 @@ class PagedKVCache(_EngineBase):
     """A paged cache of fp16, bf16 or INT8 pages (``dtype``; INT8 with fp16 scales per (token, ``group_size``)).
 
     ``num_pages`` fixes the pool (``RuntimeError`` when it is used up); without it the pool grows by doubling.
-    ``max_seq_len`` bounds the tokens held of a sequence.  Layers share the
+    ``max_seq_len`` bounds the tokens that a sequence holds (those of pages given back no longer count).  Layers share the
     block table: call them in the same order with the same token counts, as a model's forward does (those in use: a
     layer that never appends needs no pages, and one that begins late takes pages of its own for what the others
     gave back).  K and V are fp16 or bf16; float pages have their
@@ -178,8 +178,11 @@ class PagedKVCache(_EngineBase):
         """Pages for `counts` more tokens of each sequence."""
         held = self._held[layer_id] or [0] * self._batch
         target = [h + c for h, c in zip(held, counts)]
-        if self.max_seq_len is not None and max(target, default=0) > self.max_seq_len:
-            raise ValueError(f"target_len {max(target)} exceeds max_seq_len {self.max_seq_len} for layer {layer_id}")
+        if self.max_seq_len is not None:
+            keep, lost = -(-self.sinks // self.page_size), self._lost[layer_id]
+            most = max((t - max(lost.get(b, 0) - keep, 0) * self.page_size for b, t in enumerate(target)), default=0)
+            if most > self.max_seq_len:
+                raise ValueError(f"target_len {most} exceeds max_seq_len {self.max_seq_len} for layer {layer_id}")
         need = self._needs(held, target)
         if len(need) > len(self._free):
             self._give_back(counts)

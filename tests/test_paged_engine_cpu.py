@@ -310,6 +310,23 @@ def test_a_sequence_that_takes_nothing_keeps_what_it_sees(calls, monkeypatch):
         f.c.decode_attn(layer, tensor(3, 2, 128))
 
 
+def test_max_seq_len_counts_what_is_held(calls, monkeypatch):
+    """A stream through a window goes on past max_seq_len; a chunk that would have more than it in pages is refused."""
+    f = Filled(monkeypatch, 2, window=20, sinks=4, max_seq_len=96)
+    for _ in range(8):
+        for layer in (0, 1):
+            f.append(layer, [40, 1, 0])
+    assert f.c.get_seq_lens() == [320, 8, 0]
+    with pytest.raises(ValueError, match="max_seq_len"):
+        append(f.c, [90, 1, 1], heads=1)
+    with pytest.raises(ValueError, match="max_seq_len"):
+        append(f.c, [1, 95, 1], heads=1)
+    c = make(max_seq_len=96)
+    append(c, [96])
+    with pytest.raises(ValueError, match="max_seq_len"):
+        append(c, [1])
+
+
 def test_giving_back_looks_at_new_pages_only(calls):
     """A step's bookkeeping does not grow with the tokens that a window has left behind."""
     c = make(window=20)
