@@ -313,17 +313,21 @@ class PagedKVCache(_EngineBase):
     def get_kv(self, layer_id: int) -> Tuple[Tensor, Tensor]:
         """Dense K, V [B, Hkv, n, 128] of what is held (INT8: fp16 values), n the longest sequence's tokens; slots
         past a shorter sequence's end, and those of pages given back to the pool, are zero."""
-        kp, vp, ks, vs, table, _ = self._tensors(layer_id)
+        *_, table, _ = self._tensors(layer_id)
         held = self._held[layer_id]
-        n = max(held, default=0)
-        cols = -(-n // self.page_size)
-        t = table[:, :cols].long()
-        slot = torch.arange(cols * self.page_size, device=t.device)
-        there = (t >= 0).repeat_interleave(self.page_size, dim=1) & \
-            (slot < self._device_ints(held, t.device).unsqueeze(1))
+        table = table[:, : -(-max(held, default=0) // self.page_size)]
         if self._lost[layer_id]:  # a layer that began later may have pages where this one gave its own back
-            lost = self._device_ints([self._lost[layer_id].get(b, 0) * self.page_size for b in range(self._batch)], t.device)
-            there &= (slot >= lost.unsqueeze(1)) | (slot < -(-self.sinks // self.page_size) * self.page_size)
+            place = torch.arange(table.shape[1], device=table.device)
+            lost = self._device_ints([self._lost[layer_id].get(b, 0) for b in range(self._batch)], table.device)
+            table = table.masked_fill((place < lost.unsqueeze(1)) & (place >= -(-self.sinks // self.page_size)), -1)
+        return self._dense(layer_id, table, held)
+
+    def _dense(self, layer_id: int, table: Tensor, lens: List[int]) -> Tuple[Tensor, Tensor]:
+        """Dense K, V [B, Hkv, max(lens), 128] of the pages that a table [B, cols] names, sequence b's first lens[b] slots; the
+        others, and pages that are not there, are zero."""
+        t = table.long()
+        slot = torch.arange(t.shape[1] * self.page_size, device=t.device)
+        there = (t >= 0).repeat_interleave(self.page_size, dim=1) & (slot < self._device_ints(lens, t.device).unsqueeze(1))
 
         def dense(pages, scale):
             x = pages[t.clamp(min=0)]
@@ -331,8 +335,9 @@ class PagedKVCache(_EngineBase):
                 g = scale[t.clamp(min=0)].float().unsqueeze(-1)
                 x = (x.float().unflatten(-1, (-1, self.group_size)) * g).flatten(-2).half()
             x = x.permute(0, 2, 1, 3, 4).flatten(2, 3)
-            return x.masked_fill(~there[:, None, :, None], 0.0)[:, :, :n]
+            return x.masked_fill(~there[:, None, :, None], 0.0)[:, :, : max(lens, default=0)]
 
+        kp, vp, ks, vs = self._pools[layer_id]
         return dense(kp, ks), dense(vp, vs)
 
     # ---------------------------------------------------------------- attention
@@ -396,7 +401,7 @@ class PagedKVCache(_EngineBase):
         held = list(self._held[layer_id]) or [0] * batch
         kk, vv = k, v
         if any(held):
-            kk, vv = self._with_past(layer_id, k, v, held, counts)
+            kk, vv, held = self._with_past(layer_id, k, v, held, counts)
         ragged = lens is not None or len(set(held)) > 1
         out = prefill_attn_window(
             q, kk, vv, sm_scale, window=self.window, sinks=self.sinks, inv_tau=inv_tau,
@@ -416,11 +421,24 @@ class PagedKVCache(_EngineBase):
             self._evict(layer_id, 0)
         return out
 
-    def _with_past(self, layer_id: int, k: Tensor, v: Tensor, held: List[int], counts: List[int]) -> Tuple[Tensor, Tensor]:
-        """What each sequence holds, then its new tokens, dense [B, Hkv, max, 128]."""
+    def _with_past(self, layer_id: int, k: Tensor, v: Tensor, held: List[int],
+                   counts: List[int]) -> Tuple[Tensor, Tensor, List[int]]:
+        """What each sequence holds, then its new tokens, dense [B, Hkv, max, 128], and how many of the first there are.
+
+        Through a window that is the sinks' pages and those that the first new token sees: tokens between them are seen
+        by none of the queries, and those behind them lie as far from the queries as they did, so that the same window
+        and sinks hold."""
+        table, ps = self._block_table(k.device), self.page_size
+        if self.window is not None:
+            keep = -(-self.sinks // ps)
+            left_out = [max(max(h + 1 - self.window, 0) // ps - keep, 0) for h in held]
+            held = [h - n * ps for h, n in zip(held, left_out)]
+            place = torch.arange(-(-max(held) // ps), device=k.device)
+            place = place + (place >= keep) * self._device_ints(left_out, k.device).unsqueeze(1)
+            table = table.gather(1, place.clamp(max=table.shape[1] - 1))
         total = max(h + c for h, c in zip(held, counts))
         out = []
-        for past, new in zip(self.get_kv(layer_id), (k, v)):
+        for past, new in zip(self._dense(layer_id, table[:, : -(-max(held) // ps)], held), (k, v)):
             x = new.new_zeros((new.shape[0], new.shape[1], total, HEAD_DIM))
             if len(set(held)) == 1 and len(set(counts)) == 1:
                 x[:, :, : held[0]] = past.to(new.dtype)
@@ -430,7 +448,7 @@ class PagedKVCache(_EngineBase):
                     x[b, :, :h] = past[b, :, :h].to(new.dtype)
                     x[b, :, h : h + c] = new[b, :, :c]
             out.append(x)
-        return out[0], out[1]
+        return out[0], out[1], held
 
     def _evict(self, layer_id: int, slack: int) -> None:
         if self.budget is None:

@@ -104,3 +104,27 @@ def test_lengths_in_64_bits():
     assert torch.equal(k, was)
     out = K.prefill_attn_window(x, x, x, q_lens=torch.tensor([2 ** 33, 2], device=DEV), kv_lens=torch.tensor([2 ** 32, 2], device=DEV))
     assert torch.equal(out, K.prefill_attn_window(x, x, x, q_lens=torch.tensor([4, 2], device=DEV), kv_lens=torch.tensor([4, 2], device=DEV)))
+
+
+@pytest.mark.parametrize("dtype", [F16, torch.int8])
+def test_a_windowed_chunk_takes_memory_for_the_window(dtype):
+    """A chunk after 40000 tokens gives what it gives after the last of them alone, in memory that does not follow the
+    history."""
+    K = _k()
+    g = torch.Generator(device=DEV).manual_seed(5)
+    c, short = (K.PagedKVCache(1, device=DEV, dtype=dtype, page_size=64, window=200) for _ in range(2))
+    k, v = (torch.randn(2, 2, 40000, D, generator=g, device=DEV).half() for _ in range(2))
+    c.append(0, k, v)
+    short.append(0, k[:, :, 39936 - 256 :], v[:, :, 39936 - 256 :])  # a whole number of pages fewer
+    for S in (70, 300):
+        q, kn, vn = (torch.randn(2, h, S, D, generator=g, device=DEV).half() for h in (4, 2, 2))
+        want = short.prefill_attn(0, q, kn, vn, SM)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        out = c.prefill_attn(0, q, kn, vn, SM)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        # K and V of 200 + 63 + S tokens in a few copies (INT8: one in fp32), and what the attention itself takes
+        rows = 2 * 2 * (264 + S) * D
+        assert torch.cuda.max_memory_allocated() - before <= 16 * 4 * rows + (8 << 20), S

@@ -343,3 +343,71 @@ def test_giving_back_looks_at_new_pages_only(calls):
     for _ in range(64):
         append(c, [1, 1, 1])
     assert 0 < len(looked) <= 2 * 3 * (64 // 16 + 1), looked  # whether a page is there, and which
+
+
+# ---------------------------------------------------------------- chunks
+
+
+def attend(q, k, v, sm=None, window=None, sinks=0, q_lens=None, kv_lens=None, inv_tau=None):
+    """prefill_attn_window in float64 (heads alike)."""
+    out = torch.zeros(q.shape, dtype=torch.float64)
+    for b in range(q.shape[0]):
+        m = q.shape[2] if q_lens is None else int(q_lens[b])
+        n = k.shape[2] if kv_lens is None else int(kv_lens[b])
+        if not m:
+            continue
+        pos, key = torch.arange(n - m, n)[:, None], torch.arange(n)[None]
+        vis = key <= pos
+        if window:
+            vis &= (key > pos - window) | (key < sinks)
+        s = (q[b, :, :m].double() @ k[b, :, :n].double().transpose(1, 2)).masked_fill(~vis, -float("inf"))
+        out[b, :, :m] = torch.softmax(s, -1) @ v[b, :, :n].double()
+    return out.as_subclass(torch.Tensor)
+
+
+@pytest.mark.parametrize("window,sinks", [(None, 0), (1, 0), (1, 3), (16, 0), (17, 16), (40, 5), (33, 40), (500, 4)])
+@pytest.mark.parametrize("late", [False, True])
+def test_chunks_through_a_window_touch_the_window(calls, monkeypatch, window, sinks, late):
+    """What a chunk attends over is the sinks' pages, the window's and its own tokens, however much was held, and what comes
+    out is the attention over all tokens."""
+    monkeypatch.setattr(M, "append_paged", write)
+    seen = []
+
+    def stand_in(q, k, v, *args, **kw):
+        seen.append(k.shape[2])
+        return attend(q, k, v, *args, **kw)
+
+    monkeypatch.setattr(M, "prefill_attn_window", stand_in)
+    g = torch.Generator().manual_seed(1)
+    c = make(2, window=window, sinks=sinks)
+    plans = ([200, 200, 200], [1, 1, 1], [30, 30, 30], [33, 7, 50], [20, 0, 300], [15, 15, 15]), ([64, 64, 64], [16, 16, 16], [8, 8, 8])
+    for plan in plans:
+        lens = [[0, 0, 0], [0, 0, 0]]
+        kept = [[[torch.zeros(1, 0, 128).half() for _ in range(2)] for _ in range(3)] for _ in range(2)]
+        order = [(n, layer) for layer in (0, 1) for n in plan] if late else [(n, layer) for n in plan for layer in (0, 1)]
+        for counts, layer in order:
+            S = max(counts)
+            q, k, v = (torch.randn(3, 1, S, 128, generator=g).mul(0.3).half().as_subclass(OnGpu) for _ in range(3))
+            out = c.prefill_attn(layer, q, k, v, lens=None if len(set(counts)) == 1 else counts)
+            bound = S + (max(lens[layer]) if window is None else -(-sinks // 16) * 16 + window + 15)
+            assert seen[-1] <= max(bound, S), (counts, layer)
+            for b, n in enumerate(counts):
+                both = [torch.cat([kept[layer][b][i], torch.Tensor(x[b, :, :n]).half()], 1) for i, x in enumerate((k, v))]
+                kept[layer][b] = both
+                lens[layer][b] += n
+                if n:
+                    want = attend(q[b : b + 1, :, :n], both[0][None], both[1][None], window=window, sinks=sinks)[0]
+                    assert torch.allclose(out[b, :, :n], want, rtol=0, atol=1e-12), (counts, layer, b)
+        assert c.get_seq_lens(1) == lens[1]
+        c.clear()
+
+
+def test_a_chunk_leaves_the_cache_as_an_append_does(calls, monkeypatch):
+    f = Filled(monkeypatch, 1, window=20, sinks=4)
+    f.append(0, [50, 3, 0])
+    x = torch.zeros(3, 1, 7, 128).half().as_subclass(OnGpu)
+    for b in range(3):
+        x[b, 0, :, 1], x[b, 0, :, 2] = b, torch.arange(f.n[0][b], f.n[0][b] + 7)
+    f.c.prefill_attn(0, x, x, -x, lens=[7, 5, 1])
+    f.n[0] = [57, 8, 1]
+    f.check()
