@@ -128,3 +128,164 @@ def test_a_windowed_chunk_takes_memory_for_the_window(dtype):
         # K and V of 200 + 63 + S tokens in a few copies (INT8: one in fp32), and what the attention itself takes
         rows = 2 * 2 * (264 + S) * D
         assert torch.cuda.max_memory_allocated() - before <= 16 * 4 * rows + (8 << 20), S
+
+
+# ---------------------------------------------------------------- bounds that bind, in several layers
+
+
+@pytest.mark.parametrize("dtype,int8", [(F16, 0), (BF16, 0), (F16, 32)])
+@pytest.mark.parametrize("kw", [dict(window=40, sinks=3), dict(budget=48, sinks=4, recent=12, slack=8)], ids=["window", "budget"])
+def test_bounds_in_three_layers(dtype, int8, kw):
+    """Layers with keys of their own share one table while pages go back and rows are cut down: each layer's every step is
+    the attention over what that layer should hold."""
+    from test_gpu_paged import check, reference, visible
+    from test_gpu_paged_engine import Model, draws, same_rows
+
+    K = _k()
+    print(f"[layers] {dtype} {int8} {kw}", flush=True)
+    B, hq, hkv, L = 2, 4, 2, 3
+    window = kw.get("window")
+    c = K.PagedKVCache(L, device=DEV, dtype=torch.int8 if int8 else dtype, page_size=16, group_size=int8 or 32, **kw)
+    m = [Model(B, hkv, int8, **{n: x for n, x in kw.items() if n != "window"}) for _ in range(L)]
+    g = torch.Generator(device=DEV).manual_seed(11)
+    lens = [75, 30]
+    for layer in range(L):
+        q, k, v = draws(g, B, hq, hkv, 75, dtype)
+        c.prefill_attn(layer, q, k, v, SM, lens=lens)
+        m[layer].append(k, v, lens)
+        if not window:
+            for b, n in enumerate(lens):
+                m[layer].weigh(b, q[b, :, n - 1].cpu(), SM)
+            m[layer].evict(0)
+    for step in range(50):
+        for layer in range(L):
+            q, k, v = draws(g, B, hq, hkv, 1, dtype)
+            out = c.append_decode_attn(layer, q[:, :, 0], k, v, SM)
+            m[layer].append(k, v, [1] * B)
+            for b, n in enumerate(m[layer].held()):
+                if step % 5 == layer:
+                    ref, tol, _, _ = reference(q[b, :, 0].cpu(), torch.stack(m[layer].k[b]), torch.stack(m[layer].v[b]),
+                                               visible(n, n, window, kw["sinks"] if window else 0), SM, dtype, F16 if int8 else dtype, int8)
+                    check(out[b], ref, tol, (step, layer, b))
+                if not window:
+                    m[layer].weigh(b, q[b, :, 0].cpu(), SM)
+            m[layer].evict(kw.get("slack", 0))
+            assert c.get_seq_lens(layer) == m[layer].held(), (step, layer)
+    assert max(sum(p >= 0 for p in r) for r in c._rows) <= 5
+    if not window:
+        same_rows(c, m[0], int8)
+    assert c.get_seq_len() == 125
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_hook_generates_through_a_window_that_binds(dtype):
+    """Prompt, chunk and steps through the patched model with a window of 24 and 4 sinks give the tokens of the unpatched
+    model under the mask that says so."""
+    from test_gpu_paged_engine import _generate, _tiny_lm
+
+    K = _k()
+    print(f"[hook window] {dtype}", flush=True)
+    m = _tiny_lm(dtype)
+    ids = torch.randint(0, 211, (2, 70), generator=torch.Generator().manual_seed(9)).to(DEV)
+
+    def plain(window):
+        cur, toks = ids, []
+        for _ in range(12):
+            n = cur.shape[1]
+            i, j = torch.arange(n, device=DEV)[:, None], torch.arange(n, device=DEV)[None]
+            seen = (j <= i) & ((j > i - window) | (j < 4))
+            mask = torch.zeros(n, n, device=DEV, dtype=dtype).masked_fill(~seen, torch.finfo(dtype).min)
+            with torch.no_grad():
+                toks.append(m(input_ids=cur, attention_mask=mask.expand(2, 1, n, n)).logits[:, -1].argmax(-1))
+            cur = torch.cat([cur, toks[-1].view(-1, 1)], 1)
+        return torch.stack(toks, 1)
+
+    want = plain(24)
+    assert not torch.equal(want, plain(1000))  # the window matters
+    engine = K.PagedKVCache(2, device=DEV, dtype=dtype, page_size=16, window=24, sinks=4)
+    got = _generate(m, engine, ids, 12)
+    assert torch.equal(got, want), (got.tolist(), want.tolist())
+    # the prompt in two chunks
+    engine = K.PagedKVCache(2, device=DEV, dtype=dtype, page_size=16, window=24, sinks=4)
+    cache = K.INT8CacheWrapperContainer(engine, 2)
+    K.apply_int8_fused_patch(m)
+    try:
+        with torch.no_grad():
+            m(input_ids=ids[:, :41], past_key_values=cache, use_cache=True)
+            logits = m(input_ids=ids[:, 41:], past_key_values=cache, use_cache=True).logits
+    finally:
+        K.remove_int8_fused_patch(m)
+    assert torch.equal(logits[:, -1].argmax(-1), want[:, 0]) and engine.get_seq_len() == 70
+
+
+class Simulated:
+    """An engine in float64 with a budget, as PagedKVCache has one."""
+
+    decode_attn_impl, inv_tau = "hip_fused", None
+
+    def __init__(self, layers, heads, batch, budget, sinks, recent, slack):
+        from test_gpu_paged_engine import Model
+
+        self.num_layers = layers
+        self.m = [Model(batch, heads, 0, budget, sinks, recent, slack) for _ in range(layers)]
+        self._layer_seq_lens = [0] * layers
+        self.slack = slack
+
+    def get_paged_tensors(self, layer):
+        raise NotImplementedError
+
+    def get_seq_len(self):
+        return max(self._layer_seq_lens)
+
+    def prefill_attn(self, layer, q, k, v, sm_scale=None, inv_tau=None):
+        m, S = self.m[layer], q.shape[2]
+        m.append(k, v, [S] * q.shape[0])
+        self._layer_seq_lens[layer] += S
+        out = torch.zeros(q.shape, dtype=torch.float64)
+        for b in range(q.shape[0]):
+            kk, vv = torch.stack(m.k[b]), torch.stack(m.v[b])
+            n, rep = kk.shape[1], q.shape[1] // kk.shape[0]
+            hidden = torch.ones(S, n, dtype=torch.bool).triu(n - S + 1)
+            for h in range(q.shape[1]):
+                s = (q[b, h].cpu().double() @ kk[h // rep].t() * sm_scale).masked_fill(hidden, -math.inf)
+                out[b, h] = torch.softmax(s, 1) @ vv[h // rep]
+            m.weigh(b, q[b, :, -1].cpu(), sm_scale)
+        m.evict(0 if S > 1 else self.slack)
+        return out.to(q)
+
+    def append_decode_attn(self, layer, q, k, v, sm_scale=None, inv_tau=None):
+        return self.prefill_attn(layer, q.unsqueeze(2), k, v, sm_scale).squeeze(2)
+
+
+def test_hook_generates_through_a_budget_that_binds():
+    """The tokens are those of a float64 simulation of the budget in the same hook, and not those of a cache without one."""
+    from test_gpu_paged_engine import _generate, _tiny_lm
+
+    K = _k()
+    print("[hook budget]", flush=True)
+    m = _tiny_lm(F16)
+    ids = torch.randint(0, 211, (2, 70), generator=torch.Generator().manual_seed(9)).to(DEV)
+    kw = dict(budget=24, sinks=4, recent=8, slack=4)
+    want = _generate(m, Simulated(2, 2, 2, **kw), ids, 12)
+    engine = K.PagedKVCache(2, device=DEV, dtype=F16, page_size=16, **kw)
+    got = _generate(m, engine, ids, 12)
+    assert torch.equal(got, want), (got.tolist(), want.tolist())
+    assert max(engine.get_seq_lens(1)) <= 28 and engine.get_seq_len() == 81
+    assert not torch.equal(got, _generate(m, K.PagedKVCache(2, device=DEV, dtype=F16, page_size=16), ids, 12))
+
+
+def test_repeated_calls_give_the_same_bits():
+    """Split and whole prompts, weights and eviction: the same inputs give the same results, every time."""
+    from test_gpu_paged_engine import _operands, _step
+
+    K = _k()
+    g = torch.Generator(device=DEV).manual_seed(4)
+    q, k, v = (torch.randn(2, h, 3000, D, generator=g, device=DEV).half() for h in (4, 2, 2))
+    for S in (3000, 50):
+        outs = [K.prefill_attn_window(q[:, :, -S:], k, v, SM, window=700, sinks=4) for _ in range(4)]
+        assert all(torch.equal(o, outs[0]) for o in outs)
+    steps = []
+    for _ in range(4):
+        ops = _operands(7)
+        steps.append([*_step(*ops), ops[3], torch.nan_to_num(ops[0].k), torch.nan_to_num(ops[0].v)])
+    assert all(torch.equal(a, b) for s in steps for a, b in zip(s, steps[0]))
