@@ -53,6 +53,16 @@ def _reset_fused_state() -> None:
 # ---------------------------------------------------------------- HF cache duck types
 
 
+def _append_and_read(engine, layer_idx, key_states, value_states):
+    """What the original forward gets from a cache: all that is held, dense.  It would attend tokens outside an engine's own
+    window, and the zeros in the place of pages that were given back."""
+    if getattr(engine, "window", None) is not None:
+        raise ValueError(f"a {type(engine).__name__} with a window attends its tokens itself: patch the model "
+                         "(apply_int8_fused_patch)")
+    engine.append(layer_idx, key_states, value_states)
+    return engine.get_kv(layer_idx)
+
+
 class INT8CacheWrapper:
     """One layer's view of a quantized cache engine, in the shape HF attention expects
     (src/engine/patch_model.py:95-131).  The fused path reads ``engine`` and
@@ -63,8 +73,7 @@ class INT8CacheWrapper:
         self.layer_idx = layer_idx
 
     def update(self, key_states, value_states, layer_idx, cache_kwargs=None):
-        self.engine.append(layer_idx, key_states, value_states)
-        return self.engine.get_kv(layer_idx)
+        return _append_and_read(self.engine, layer_idx, key_states, value_states)
 
     def get_seq_length(self, layer_idx: int = 0) -> int:
         return self.engine.get_seq_len()
@@ -144,8 +153,7 @@ class INT8CacheWrapperContainer:
         return cached + current, 0
 
     def update(self, key_states, value_states, layer_idx, cache_kwargs=None):
-        self.engine.append(layer_idx, key_states, value_states)
-        return self.engine.get_kv(layer_idx)
+        return _append_and_read(self.engine, layer_idx, key_states, value_states)
 
 
 # ---------------------------------------------------------------- RoPE and head metadata

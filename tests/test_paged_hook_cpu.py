@@ -120,3 +120,22 @@ def test_steps_hand_over_what_prompts_do(dtype):
     assert dtype == torch.float16 or q1.abs().max() > 65504 and torch.isfinite(q1).all()
     assert torch.equal(k0, k1) and torch.equal(v0, v1)
     assert t0.dtype == t1.dtype == torch.float32 and torch.equal(t0, tau[0]) and torch.equal(t1, tau[0])
+
+
+def test_an_unpatched_model_gets_no_windowed_cache():
+    """`update` hands out all that is held, which a window does not see: refused before anything is appended."""
+    import llm_kvcache_quantization_amd as K
+
+    x = torch.zeros(1, 2, 3, 128, dtype=torch.float16)
+    for kw, refused in ((dict(window=20), True), (dict(), False), (dict(budget=20), False)):
+        engine = K.PagedKVCache(1, device="cpu", **kw)
+        log = []
+        engine.append = lambda layer, k, v: log.append(layer)
+        engine.get_kv = lambda layer: (x, x)
+        for cache in (P.INT8CacheWrapper(engine, 0), P.INT8CacheWrapperContainer(engine, 1)):
+            if refused:
+                with pytest.raises(ValueError, match="window"):
+                    cache.update(x, x, 0)
+            else:
+                assert cache.update(x, x, 0) == (x, x)
+        assert len(log) == (0 if refused else 2)
