@@ -276,8 +276,6 @@ class PagedKVCache(_EngineBase):
             if self.num_pages is not None:
                 self._total = self.num_pages
                 self._free = list(range(self._total - 1, -1, -1))
-        if self._lead is None:
-            self._lead = layer_id
         if layer_id == self._lead and (self.window is not None or self.budget is not None):
             self._give_back(counts)
         self._reserve(layer_id, counts, k.device)
@@ -286,6 +284,8 @@ class PagedKVCache(_EngineBase):
         table = self._block_table(k.device)
         append_paged(k, v, kp, vp, table, self._device_ints(held, k.device),
                      self._device_ints(counts, k.device) if ragged else None, k_scale=ks, v_scale=vs)
+        if self._lead is None:
+            self._lead = layer_id
         self._held[layer_id] = [h + c for h, c in zip(held, counts)]
         self._seen[layer_id] = [s + c for s, c in zip(self._seen[layer_id] or [0] * batch, counts)]
         self._layer_seq_lens[layer_id] = max(self._seen[layer_id], default=0)

@@ -411,3 +411,15 @@ def test_a_chunk_leaves_the_cache_as_an_append_does(calls, monkeypatch):
     f.c.prefill_attn(0, x, x, -x, lens=[7, 5, 1])
     f.n[0] = [57, 8, 1]
     f.check()
+
+
+def test_a_refused_layer_does_not_lead(calls):
+    """After clear() another layer than the one that was refused begins the steps: pages still go back."""
+    c = make(2, window=20, max_seq_len=200)
+    append(c, [5])
+    c.clear()
+    with pytest.raises(ValueError, match="max_seq_len"):
+        append(c, [300])
+    for _ in range(3):
+        append(c, [64], 1)
+    assert sum(p >= 0 for p in c._rows[0]) <= 2 + 4
