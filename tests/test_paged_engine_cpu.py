@@ -415,7 +415,7 @@ def test_a_chunk_leaves_the_cache_as_an_append_does(calls, monkeypatch):
 
 def test_a_refused_layer_does_not_lead(calls):
     """After clear() another layer than the one that was refused begins the steps: pages still go back."""
-    c = make(2, window=20, max_seq_len=200)
+    c = make(2, window=20, max_seq_len=200, num_pages=100)  # never short of pages
     append(c, [5])
     c.clear()
     with pytest.raises(ValueError, match="max_seq_len"):
