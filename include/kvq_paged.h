@@ -11,7 +11,8 @@
  * numbers are device memory that the host does not read: lengths are clamped to the table's
  * columns, and a page number outside [0, num_pages) stands for a page that is not there (its
  * tokens are left out of the attention, nothing is written to it, and a row that has one is not
- * evicted).  No counterpart in the reference, whose caches are dense.
+ * evicted).  Pages that are written (append, eviction) need memory of their own: a stride of 0 between
+ * them, or between heads, is refused.  No counterpart in the reference, whose caches are dense.
  */
 #ifndef KVQ_PAGED_H_
 #define KVQ_PAGED_H_

@@ -108,6 +108,15 @@ inline int paged_cache(const kvq_paged_cache& p, PagedCache& c) {
   return KVQ_OK;
 }
 
+// Of a cache that is written: its pages and heads have memory of their own.
+inline int paged_written(const PagedCache& c) {
+  const int64_t pages[4] = {c.ksp, c.vsp, c.kssp, c.vssp}, heads[4] = {c.ksh, c.vsh, c.kssh, c.vssh};
+  for (int i = 0; i < (c.ks ? 4 : 2); ++i)
+    if ((c.num_pages > 1 && pages[i] == 0) || (c.kv_heads > 1 && heads[i] == 0))
+      return fail(KVQ_ERR_INVALID, "paged: pages that are written must have memory of their own, got a stride of 0");
+  return KVQ_OK;
+}
+
 inline int launched() {
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? KVQ_OK : fail(KVQ_ERR_LAUNCH, std::string("launch: ") + hipGetErrorString(e));

@@ -154,8 +154,8 @@ __global__ __launch_bounds__(kAppThreads) void paged_append_long_kernel(AppArgs 
 int append(const kvq_paged_append_params* p, hipStream_t st) {
   if (!p) return fail(KVQ_ERR_INVALID, "paged append: NULL params");
   AppArgs a{};
-  const int rc = paged_cache(p->cache, a.c);
-  if (rc) return rc;
+  int rc = paged_cache(p->cache, a.c);
+  if (rc || (rc = paged_written(a.c))) return rc;
   if (p->seq_new < 0) return fail(KVQ_ERR_INVALID, "paged append: negative seq_new");
   // a row holds no more, and places of a work-group's share past the end stay in 32 bits
   if (p->seq_new > (1 << 30)) return fail(KVQ_ERR_UNSUPPORTED, "paged append: more than 2^30 new tokens");

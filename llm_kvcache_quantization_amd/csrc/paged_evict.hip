@@ -300,7 +300,7 @@ int evict(const kvq_paged_evict_params* p, hipStream_t st) {
   if (!p) return fail(KVQ_ERR_INVALID, "paged evict: NULL params");
   EvictArgs a{};
   int rc = paged_cache(p->cache, a.c);
-  if (rc) return rc;
+  if (rc || (rc = paged_written(a.c))) return rc;
   const int B = a.c.batch, H = a.c.kv_heads;
   if (p->budget <= 0 || p->sinks < 0 || p->recent < 0 || (int64_t)p->sinks + p->recent > p->budget)
     return fail(KVQ_ERR_INVALID, "paged evict: budget must be positive and hold sinks + recent");

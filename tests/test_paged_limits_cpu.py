@@ -94,3 +94,23 @@ def test_scales_that_want_a_gradient():
                      lambda: K.evict_paged(i8, i8, table, lens, w.float(), 1, **sc)):
             with pytest.raises(NotImplementedError, match="backward"):
                 call()
+
+
+def test_written_pages_have_memory_of_their_own():
+    """Expanded pages or heads may be read; who writes them would write one place from several work-groups."""
+    C, L = _lib()
+    for over in (dict(k_stride_p=0), dict(v_stride_p=0), dict(k_stride_h=0), dict(v_stride_h=0)):
+        for int8 in (False, True):
+            c = _cache(C, int8, **over)
+            _refused(L, "kvq_paged_append", _append(C, c))
+            assert b"stride of 0" in L.kvq_last_error()
+            _refused(L, "kvq_paged_evict", _evict(C, c))
+            assert b"stride of 0" in L.kvq_last_error()
+    for over in (dict(ks_stride_p=0), dict(vs_stride_p=0), dict(ks_stride_h=0), dict(vs_stride_h=0)):
+        _refused(L, "kvq_paged_append", _append(C, _cache(C, True, **over)))
+        assert b"stride of 0" in L.kvq_last_error()
+    # one page, one head: their strides mean nothing
+    c = _cache(C, num_pages=1, kv_heads=1, k_stride_p=0, v_stride_p=0, k_stride_h=0, v_stride_h=0)
+    import ctypes
+
+    assert L.kvq_paged_append(ctypes.byref(_append(C, c, seq_new=0)), None) == 0
