@@ -372,6 +372,8 @@ def evict_paged(k_pages: Tensor, v_pages: Tensor, block_table: Tensor, context_l
     new_lens = torch.empty_like(lens)
     kept = lens.new_empty((batch, heads, budget))
     new_weights = torch.empty_like(weights, memory_format=torch.contiguous_format)
+    if weights.shape[2] == 0:  # no slots: no tokens
+        return new_lens.zero_(), kept.fill_(-1), new_weights
     if batch:
         _call(C.lib().kvq_paged_evict, _EVICT.pack(
             *cache, lens.data_ptr(), weights.data_ptr(), *weights.stride()[:2], new_lens.data_ptr(), kept.data_ptr(),

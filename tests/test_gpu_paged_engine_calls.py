@@ -289,3 +289,24 @@ def test_repeated_calls_give_the_same_bits():
         ops = _operands(7)
         steps.append([*_step(*ops), ops[3], torch.nan_to_num(ops[0].k), torch.nan_to_num(ops[0].v)])
     assert all(torch.equal(a, b) for s in steps for a, b in zip(s, steps[0]))
+
+
+def test_tables_without_a_column():
+    """No slots: nothing is written, seen or kept."""
+    K = _k()
+    for dtype in (F16, torch.int8):
+        k = torch.ones(3, 2, 16, D, device=DEV, dtype=dtype)
+        sc = dict(k_scale=torch.ones(3, 2, 16, 2, device=DEV).half(), v_scale=torch.ones(3, 2, 16, 2, device=DEV).half()) if dtype == torch.int8 else {}
+        table, lens = torch.zeros(2, 0, device=DEV, dtype=torch.int32), torch.tensor([5, 0], device=DEV)
+        q, x = torch.ones(2, 4, D, device=DEV).half(), torch.zeros(2, 2, 4, D, device=DEV).half()
+        for w in (None, torch.ones(2, 2, 0, device=DEV), torch.ones(2, 2, 7, device=DEV)):
+            assert not K.decode_attn_paged(q, k, k, table, lens, **sc, weights=w).any()
+            assert w is None or (w == 1).all()
+            if w is not None:
+                new, kept, weights = K.evict_paged(k, k.clone(), table, lens, w, 3, **sc)
+                torch.cuda.synchronize()
+                assert new.tolist() == [0, 0] and kept.shape == (2, 2, 3) and (kept == -1).all()
+                assert weights.shape == w.shape and not weights.any()
+        K.append_paged(x, x, k, k.clone(), table, lens, **sc)
+        torch.cuda.synchronize()
+        assert (k == 1).all()
