@@ -1,7 +1,7 @@
 // Eviction from a paged cache by accumulated weight (kvq_paged_evict), in two launches.
 //
 // paged_select_kernel: a work-group a (row, KV head); every wave has a segment of the tokens, with their
-// weights in registers where the pages can hold at most 32768 tokens a row.  The threshold, the need-th largest
+// weights in registers where the pages can hold 16384 to 32768 tokens a row.  The threshold, the need-th largest
 // weight of the tokens that are not protected, by three passes of a radix select (11, 11 and 10 bits of a key
 // that orders as the floats do) with LDS histograms; then every wave counts what it keeps of its segment, and
 // writes it from the sum of the segments before it.
@@ -320,12 +320,15 @@ int evict(const kvq_paged_evict_params* p, hipStream_t st) {
   a.slices = (i8 ? 128 : 256) / kSlice;
   a.scale_bytes = i8 ? 256 / p->cache.group_size : 0;
   const int64_t cap = (int64_t)p->cache.max_pages * p->cache.page_size;
-  // Few token slots: a small work-group with short loops.  The variant that keeps weights in registers is a long
-  // straight line, which an empty instruction cache pays for: 640 tokens 12.4 us, 8.5 so; but 32768 tokens 27.2 us
-  // against 35.0 fetched each time.
-  if (cap <= 4096) select<256, false>(a, st);
-  else if (cap <= 1024 * kSelKeys) select<1024, true>(a, st);
-  else select<1024, false>(a, st);
+  // By the token slots of a row, us a call (its move is the same), 256 threads that fetch weights in every pass / 1024 that
+  // do / 1024 that keep them in registers, which is a long straight line that an empty instruction cache pays for:
+  //   1 row x 2 heads     512 12.1 / 12.5 / 19.3, 2048 15.0 / 15.3 / 20.7, 4096 21.4 / 17.7 / 23.3, 8192 35.0 / 23.5 / 27.5,
+  //                       16384 61.6 / 37.8 / 38.0, 32768 115 / 66.4 / 58.5
+  //   64 rows x 8 heads   512 23.7 / 26.5 / 43.6, 2048 45.7 / 49.5 / 64.1, 4096 91.7 / 90.1 / 105, 8192 219 / 212 / 224,
+  //                       16384 483 / 464 / 470, 32768 965 / 929 / 926
+  if (cap <= 2048) select<256, false>(a, st);
+  else if (cap <= 512 * kSelKeys || cap > 1024 * kSelKeys) select<1024, false>(a, st);
+  else select<1024, true>(a, st);
   if ((rc = launched())) return rc;
   hipLaunchKernelGGL(paged_move_kernel, dim3((unsigned)H, (unsigned)B, (unsigned)(2 * a.slices)), dim3(kMoveThreads), 0, st, a);
   return launched();

@@ -125,3 +125,13 @@ def test_prompt_many_faint_tokens(dtype, S, T, bits):
                                        0, 9 if dtype == F16 else 100)
         err = (out[:, i] - ref).abs()
         assert (err <= tol).all(), (i, float((err / ref.abs()).max()), float((tol / ref.abs()).max()))
+
+
+@pytest.mark.parametrize("slots", [2048, 2064, 16384, 16400, 32768, 32784])
+def test_evict_at_the_variants_ends(slots):
+    """Tables on either side of where the selection changes, full and nearly empty rows in each."""
+    from test_gpu_paged import run_evict
+
+    run_evict([slots, 700, slots - 1], 1, 16, F16, 0, 600, 4, 100, slots=slots)
+    zeros = lambda w, g: torch.where(torch.rand(w.shape, generator=g) < 0.9, 0.0, w)  # noqa: E731
+    run_evict([slots - 5, 601], 2, 16, F16, 64, 600, 0, 7, slots=slots, w=zeros)
