@@ -122,7 +122,8 @@ int64_t kvq_prefill_workspace_bytes(const kvq_prefill_params* p);
  * the lower token).  Kept tokens move, in order, to slots 0 .. budget - 1; slots behind are left as they
  * were.  new_lens [B], kept [B, kv_heads, budget] (old token of each slot, -1 behind the row's last) and
  * new_weights [B, kv_heads, w_tokens] dense (0 behind the row's last) are written.  Rows of at most
- * budget tokens, and rows with a page that is not there, keep their tokens; no page may serve two rows. */
+ * budget tokens, and rows with a page that is not there, keep their tokens; no page may serve two rows, or
+ * two places of one.  budget and w_tokens are at most 2^30. */
 typedef struct kvq_paged_evict_params {
   kvq_paged_cache cache;
   const int32_t* context_lens;

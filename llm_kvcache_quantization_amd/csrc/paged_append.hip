@@ -5,8 +5,8 @@
 // 16 lanes.
 //
 // What bounds it: the launch for a step's rows (one token of 2 heads 2.3 us in the kernel); for prompts HBM and the
-// chain length, page, row (4 padded prompts of up to 4095 tokens, 8 heads, bf16 to INT8 of groups of 32: 19.6 us, where
-// a copy of their bytes takes 11.8).
+// chain length, page, row (4 padded prompts of up to 4095 tokens, 8 heads, bf16 to INT8 of groups of 32: 18.3 us a call,
+// where a copy of their bytes takes 11.8; as they are 15.1, 5.0 TB/s, where a copy takes 15.4).
 #include "paged.h"
 
 #pragma clang fp contract(off)
@@ -124,7 +124,8 @@ __global__ __launch_bounds__(kAppThreads) void paged_append_kernel(AppArgs a) {
 }
 
 // kAppTokens and more: a work-group takes as many consecutive tokens of a sequence and head, four rows a thread with
-// their loads side by side (the prompts above 19.6 us; in one line 21.4; two or eight rows a thread 19.7 and 23.8).
+// their loads side by side (the kernel alone on the prompts above 19.6 us; in one line 21.4; two or eight rows a thread
+// 19.7 and 23.8).
 template <class T, int GS>
 __global__ __launch_bounds__(kAppThreads) void paged_append_long_kernel(AppArgs a) {
   constexpr int R = kAppTokens / kAppRows;

@@ -3,9 +3,9 @@
 //   out[b,h] = sum_t p_t v_t,  p = softmax over the visible t of sm_scale inv_tau_h q.k_t
 //
 // One pass over K and V with a running maximum and sum.  What bounds it: HBM; every visible K and V row
-// is read once for all query heads of its KV head.  Measured: 8 rows x 8 KV heads x 32768 tokens in fp16 pages of 16 175 us (6.2 TB/s); 8
-// ragged rows of up to 65536 tokens in INT8, groups of 32, 108 us (5.9 TB/s); below 2048 tokens a row the chain
-// launch, length, page, K, V, join: 9 to 12 us.
+// is read once for all query heads of its KV head.  Measured, us a call: 8 rows x 8 KV heads x 32768 tokens in fp16 pages of 16
+// 175 (6.1 TB/s), of 64 165 (6.5 TB/s); 8 ragged rows of up to 65536 tokens in INT8, groups of 32, 110 (5.8 TB/s); below
+// 2048 tokens a row the chain launch, length, page, K, V, join: 9 to 13.
 //
 // Work: a row's visible tokens are cut into tiles of 32 token slots, and the tiles of all rows of a KV
 // head are shared out over the work-groups (Share; long rows of a ragged batch are split, short ones are

@@ -11,9 +11,9 @@
 // same bytes of all rows (a slice of one side of one (row, head)) needs one barrier a block and nothing from
 // the others.  Kept tokens are fetched two blocks ahead, their pages one, so that a block costs one latency.
 //
-// What bounds it: the select is a chain of passes within a work-group (8 x 8 rows of 32768 tokens 27 us, one of
-// 640 8.5); the move is HBM (4096 kept of each, INT8: 37 us for 143 MB read and written), or a launch's latency
-// where the budget is small (5 us).  Four rows a thread in flight: eight take 41 us, with fewer work-groups a CU.
+// What bounds it, the kernels alone: the select is a chain of passes within a work-group (8 x 8 rows of 32768 tokens 27
+// us, 1 x 2 of 640 8.9); the move is HBM (4096 kept of each, INT8: 37 us for 143 MB read and written), or a launch's
+// latency where the budget is small (5 us).  Four rows a thread in flight: eight take 41 us, with fewer work-groups a CU.
 #include "paged.h"
 
 namespace kvq {

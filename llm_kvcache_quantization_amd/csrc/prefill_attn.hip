@@ -22,9 +22,10 @@
 // work-group's result is not finite it runs again with such rows taken out of the products and added query by
 // query.
 //
-// What bounds it: the matrix units (42% busy) and the vector units (43%, half of it exponentials), in turn in each
-// wave.  Measured: 16384 tokens through a window of 4096, 28 heads, bf16, 938 us (898 TFLOP/s); 8192 tokens
-// without a window 506 us (950 TFLOP/s); a tile of 64 keys takes 1.75 us on a CU of its own, 2.3 where two share one.
+// What bounds it: the matrix units (busy for 42% of the CUs' busy cycles) and the vector units (43%, half of it
+// exponentials), in turn in each wave.  Measured, us a call: 16384 tokens through a window of 4096, 28 heads, bf16, 958 (879
+// TFLOP/s; 912 to 1005 from card to card); 8192 tokens without a window 510 (943 TFLOP/s); a tile of 64 keys takes 1.75 us
+// on a CU of its own, 2.3 where two share one.
 #include "paged.h"
 
 namespace kvq {
@@ -96,9 +97,9 @@ __device__ __forceinline__ Row unit_of(const PreArgs& a, int64_t unit64) {
 // share K and V in its L2.  It takes them by the place of their queries, the last and longest first, so that short
 // ones are left for the end.  An XCD's work-groups go round its shader engines in turn, whatever those have left to
 // do: the (row, head)s shift by one from place to place, or long and short rows would each have engines of their own.
-// us, a (row, head) at a time / without the shift / so: 4 padded prompts of up to 2047 tokens, 40 heads, window 1024
-// 168 / 209 / 149; 8192 tokens, 28 heads, no window 717 / - / 516; 4 x 32 heads of 4096 tokens with K and V of their
-// own 780 / - / 680.
+// us, a (row, head) at a time / without the shift / so, all three before padded queries and halves of tiles were left out:
+// 4 padded prompts of up to 2047 tokens, 40 heads, window 1024 168 / 209 / 149 (116 since); 8192 tokens, 28 heads, no
+// window 717 / - / 516; 4 x 32 heads of 4096 tokens with K and V of their own 780 / - / 680.
 __device__ __forceinline__ int64_t unit_at(const PreArgs& a, uint32_t at) {
   const uint32_t xcd = at & 7, k = at >> 3, depth = (uint32_t)a.blocks * (uint32_t)a.splits;
   const uint32_t per = (uint32_t)((a.units + 7) / 8), start = xcd * per, columns = (per + depth - 1) / depth;
@@ -352,7 +353,7 @@ struct Prefill {
     const TileLoad<true> load_v(v, a.vss, r.kv_len);
     const int i0 = r.i0 + 32 * wave, i = i0 + (lane & 31);
     // this lane's position; padded queries are the last one again, or all of a wave's tiles would take the masked path
-    // (509 queries over 16381 keys: 210 us, so 145), and are written as zeros
+    // (509 queries over 16381 keys: 219 us, so 157), and are written as zeros
     const int p = r.off + min(i, r.q_len - 1);
     const int pw0 = r.off + i0, pw1 = r.off + min(i0 + 31, r.q_len - 1);
 #pragma unroll

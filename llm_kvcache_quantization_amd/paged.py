@@ -219,7 +219,7 @@ def append_paged(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, block_t
     65,500 up read back as infinite.
 
     Slots past the table's end, and pages that are not there, are not written.  Pages that two sequences
-    share may be read but not appended to.
+    share, or one has twice, may be read but not appended to.
     """
     if k.ndim != 4 or k.shape[3] != HEAD_DIM or k.shape != v.shape:
         raise ValueError(f"k and v must be [B, Hkv, S, {HEAD_DIM}] alike, got {tuple(k.shape)} / {tuple(v.shape)}")
@@ -353,7 +353,7 @@ def evict_paged(k_pages: Tensor, v_pages: Tensor, block_table: Tensor, context_l
     lengths, the old token of every slot (-1 behind the last), and the kept tokens' weights (0 behind the last).
 
     Sequences of at most ``budget`` tokens stay as they are.  So do sequences with a page that is not there
-    (``kept`` is -1 for them).  Pages must not be shared between sequences.
+    (``kept`` is -1 for them).  No page may serve two sequences, or two places of one.
     """
     cache = _cache_fields(k_pages, v_pages, k_scale, v_scale, block_table)
     device, heads, batch = k_pages.device, k_pages.shape[1], block_table.shape[0]
