@@ -130,8 +130,9 @@ class PagedKVCache(_EngineBase):
         return t
 
     def _give_back(self, counts: Optional[List[int]] = None) -> None:
-        """Returns pages that no layer in use needs: behind the longest held length, or out of the window's sight now that
-        every sequence, or every one with `counts`, takes a token.  (A layer that begins later takes its own.)"""
+        """Returns pages that no layer in use needs: behind the longest held length, or out of the window's sight, that of
+        the next token where a sequence takes one (`counts`; None: all do), else of its last.  (A layer that begins later
+        takes pages of its own.)"""
         begun = [h for h in self._held if h]
         if not begun:
             return
@@ -148,7 +149,7 @@ class PagedKVCache(_EngineBase):
         if self.window is not None:
             keep = -(-self.sinks // ps)
             for b, (row, lo) in enumerate(zip(self._rows, least)):
-                # the next query stands at lo or later and sees no token before lo + 1 - window but the sinks
+                # the next token's query stands at lo or later and sees no token before lo + 1 - window but the sinks
                 end = max(lo + (1 if counts is None or counts[b] else 0) - self.window, 0) // ps
                 for i in range(max(self._gone.get(b, 0), keep), end):
                     if row[i] >= 0:
@@ -185,7 +186,7 @@ class PagedKVCache(_EngineBase):
                 raise ValueError(f"target_len {most} exceeds max_seq_len {self.max_seq_len} for layer {layer_id}")
         need = self._needs(held, target)
         if len(need) > len(self._free):
-            self._give_back(counts)
+            self._give_back(counts)  # short of pages: all that the new tokens do not see
             need = self._needs(held, target)
         short = len(need) - len(self._free)
         if short > 0:
@@ -277,7 +278,7 @@ class PagedKVCache(_EngineBase):
                 self._total = self.num_pages
                 self._free = list(range(self._total - 1, -1, -1))
         if layer_id == self._lead and (self.window is not None or self.budget is not None):
-            self._give_back(counts)
+            self._give_back([0] * batch)  # the call may yet be refused: what the last token sees stays
         self._reserve(layer_id, counts, k.device)
         held = self._held[layer_id] or [0] * batch
         kp, vp, ks, vs = self._pool(layer_id, k.device)

@@ -295,19 +295,36 @@ def test_pages_whatever_the_order(calls, monkeypatch, seed):
 
 def test_a_sequence_that_takes_nothing_keeps_what_it_sees(calls, monkeypatch):
     """A row of a padded batch with no new token still sees `window` tokens: they stay, and one whose next token another
-    layer has taken already is refused."""
-    f = Filled(monkeypatch, 2, window=16)
+    layer has taken already, for want of pages, is refused."""
+    f = Filled(monkeypatch, 2, window=16, num_pages=9)
     for layer in (0, 1):
         f.append(layer, [47, 47, 47])
-    f.append(0, [0, 1, 1])
+    assert not f.c._free
+    f.append(0, [0, 50, 1])
     # row 0 sees token 31, the last of page 1; the others' next query saw token 32 first
     assert f.c._rows[0][0] < 0 <= f.c._rows[0][1] and f.c._rows[1][1] < 0
     with pytest.raises(RuntimeError, match="sequence 1 "):
         f.c.decode_attn(1, tensor(3, 2, 128))
     f.c.decode_attn(0, tensor(3, 2, 128))
-    f.append(1, [0, 1, 1])
+    f.append(1, [0, 50, 1])
     for layer in (0, 1):
         f.c.decode_attn(layer, tensor(3, 2, 128))
+
+
+@pytest.mark.parametrize("held", range(40, 60))
+def test_a_refused_step_keeps_what_the_last_token_sees(calls, monkeypatch, held):
+    f = Filled(monkeypatch, 1, window=16)
+    f.append(0, [held, 20, 1])
+    refuse(monkeypatch, "decode_attn_paged")
+    x = torch.zeros(3, 1, 1, 128).half().as_subclass(OnGpu)
+    with pytest.raises(ValueError, match="refused here"):
+        f.c.append_decode_attn(0, tensor(3, 2, 128), x, x)
+    k, _ = f.c.get_kv(0)
+    for b, n in enumerate(f.n[0]):
+        t = torch.arange(max(n - 16, 0), n)
+        assert torch.equal(k[b, 0, t, 2].float(), t.float()) and (k[b, 0, t, 1] == b).all()
+    monkeypatch.setattr(M, "decode_attn_paged", lambda q, *a, **kw: q)
+    f.c.decode_attn(0, tensor(3, 2, 128))
 
 
 def test_max_seq_len_counts_what_is_held(calls, monkeypatch):
