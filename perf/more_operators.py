@@ -162,6 +162,10 @@ def prepare(case, seed):
         st["dst"] = (perm(pairs) if other else order[pairs : 2 * pairs]).int()
         st["lens"] = (torch.randint(1, case["slots"] + 1, (pairs,), generator=g, device=DEV).int() if case["slots"]
                       else None)
+        if own:  # a beam search copies pages at every step, always of the same pools
+            import llm_kvcache_quantization_amd as kvq
+
+            st["handles"] = [None if x is None else kvq.PagePools(x) for x in (st["pools"], st["into"])]
         return st
     hq, sizes, prompts = case["q_heads"], _sizes(case), _prompts(case)
     rows = sum(sizes)
@@ -263,7 +267,8 @@ def run(st):
     import llm_kvcache_quantization_amd as kvq
 
     if c["op"] == "copy":
-        kvq.copy_paged(st["pools"], st["src"], st["dst"], st["lens"], into=st["into"])
+        pools, into = st["handles"]
+        kvq.copy_paged(pools, st["src"], st["dst"], st["lens"], into=into)
         return st["pools"] if st["into"] is None else st["into"]
     if c["op"] == "shared":
         return kvq.decode_attn_shared(st["q"], st["k_pages"], st["v_pages"], st["table"], st["lens"], st["prefix"], SM,
