@@ -33,6 +33,8 @@ from .cache import (  # noqa: F401
     load_per_layer_bits_from_policy,
 )
 from .paged import append_paged, decode_attn_paged, evict_paged, prefill_attn_window  # noqa: F401
+from .shared import PagePools, SharedPrefix, copy_paged, decode_attn_shared  # noqa: F401
+from .scoring import TokenLogprobs, token_logprobs  # noqa: F401
 from .paged_cache import PagedKVCache  # noqa: F401
 from .patch import (  # noqa: F401
     INT8CacheWrapper,
@@ -68,6 +70,12 @@ __all__ = [
     "decode_attn_paged",
     "prefill_attn_window",
     "evict_paged",
+    "PagePools",
+    "SharedPrefix",
+    "copy_paged",
+    "decode_attn_shared",
+    "TokenLogprobs",
+    "token_logprobs",
     "INT8CacheWrapper",
     "INT8CacheWrapperContainer",
     "apply_int8_fused_patch",

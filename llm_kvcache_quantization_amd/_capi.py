@@ -37,6 +37,10 @@ KVQ_PAGED_F16 = 0
 KVQ_PAGED_BF16 = 1
 KVQ_PAGED_INT8 = 2
 
+KVQ_LOGITS_F16 = 0
+KVQ_LOGITS_BF16 = 1
+KVQ_LOGITS_F32 = 2
+
 KVQ_LAYOUT_ROWS = 0
 KVQ_LAYOUT_TILE32 = 1
 
@@ -186,6 +190,45 @@ class PagedEvictParams(ctypes.Structure):
     ]
 
 
+class PagePool(ctypes.Structure):
+    _fields_ = [
+        ("base", c_vp), ("stride_p", c_i64), ("stride_h", c_i64), ("stride_t", c_i64),
+        ("row_bytes", c_i32), ("reserved", c_i32),
+    ]
+
+
+class CopyPagesParams(ctypes.Structure):
+    _fields_ = [
+        ("from_", c_vp), ("to", c_vp), ("src", c_vp), ("dst", c_vp), ("lens", c_vp),
+        ("n_pools", c_i32), ("pairs", c_i32), ("page_size", c_i32), ("heads", c_i32),
+        ("from_pages", c_i32), ("to_pages", c_i32),
+    ]
+
+
+class SharedPlanInfo(ctypes.Structure):
+    _fields_ = [("rows", c_i32), ("units", c_i32), ("slots", c_i32), ("words", c_i32)]
+
+
+class SharedDecodeParams(ctypes.Structure):
+    _fields_ = [
+        ("cache", PagedCache),
+        ("q", c_vp), ("q_stride_b", c_i64), ("q_stride_h", c_i64), ("out", c_vp),
+        ("context_lens", c_vp), ("inv_tau", c_vp), ("plan_words", c_vp),
+        ("workspace", c_vp), ("workspace_bytes", c_i64), ("plan", SharedPlanInfo),
+        ("sm_scale", c_f32), ("q_heads", c_i32), ("q_type", c_i32), ("reserved", c_i32),
+    ]
+
+
+class TokenLogprobsParams(ctypes.Structure):
+    _fields_ = [
+        ("logits", c_vp), ("row_stride", c_i64), ("tokens", c_vp),
+        ("logprobs", c_vp), ("entropy", c_vp), ("top_logprobs", c_vp), ("top_tokens", c_vp),
+        ("workspace", c_vp), ("workspace_bytes", c_i64), ("rows", c_i64),
+        ("vocab", c_i32), ("top", c_i32), ("logits_type", c_i32), ("tokens64", c_i32),
+        ("inv_temperature", c_f32), ("reserved", c_i32),
+    ]
+
+
 # include/kvq_paged.h
 PAGED_SYMBOLS = (
     "kvq_paged_append",
@@ -195,6 +238,17 @@ PAGED_SYMBOLS = (
     "kvq_prefill_workspace_bytes",
     "kvq_paged_evict",
 )
+
+# include/kvq_shared.h
+SHARED_SYMBOLS = (
+    "kvq_copy_pages",
+    "kvq_shared_plan",
+    "kvq_shared_decode",
+    "kvq_shared_decode_workspace_bytes",
+)
+
+# include/kvq_logprobs.h
+LOGPROBS_SYMBOLS = ("kvq_token_logprobs", "kvq_token_logprobs_workspace_bytes")
 
 EXPORTED_SYMBOLS = (
     "kvq_decode_attn",
@@ -278,6 +332,19 @@ def lib() -> ctypes.CDLL:
                              ("kvq_prefill_workspace_bytes", PrefillParams)):
             getattr(L, name).argtypes = [ctypes.POINTER(params)]
             getattr(L, name).restype = c_i64
+        # several answers from one prompt (include/kvq_shared.h)
+        for name in ("kvq_copy_pages", "kvq_shared_decode"):
+            getattr(L, name).argtypes = [c_vp, c_vp]
+            getattr(L, name).restype = c_i32
+        L.kvq_shared_plan.argtypes = [c_vp, c_vp, c_i32, c_i32, c_i32, ctypes.POINTER(SharedPlanInfo), c_vp, c_i64]
+        L.kvq_shared_plan.restype = c_i32
+        L.kvq_shared_decode_workspace_bytes.argtypes = [ctypes.POINTER(SharedDecodeParams)]
+        L.kvq_shared_decode_workspace_bytes.restype = c_i64
+        # log probabilities (include/kvq_logprobs.h)
+        L.kvq_token_logprobs.argtypes = [c_vp, c_vp]
+        L.kvq_token_logprobs.restype = c_i32
+        L.kvq_token_logprobs_workspace_bytes.argtypes = [ctypes.POINTER(TokenLogprobsParams)]
+        L.kvq_token_logprobs_workspace_bytes.restype = c_i64
         ver = L.kvq_abi_version()
         if ver != ABI_VERSION:
             raise ImportError(f"{LIB_PATH} has ABI {ver}, this package needs {ABI_VERSION}; rebuild it")

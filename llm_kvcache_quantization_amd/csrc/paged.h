@@ -55,6 +55,25 @@ struct TB16 {
   }
 };
 
+// A running softmax: maximum (log2 units, kUp below the largest score; -inf before the first finite one), sum.  While the
+// maximum is -inf the sum is not a sum: 1 if a token was seen (all its scores were -inf, the result is NaN), else 0.
+__device__ __forceinline__ float shift_of(float m) { return m == kNegInf ? 0.f : m; }
+// the factor of a part with maximum m in a whole with maximum M
+__device__ __forceinline__ float part_of(float m, float M) { return fast_exp2(m - shift_of(M)); }
+// 1 / denominator; 0 where nothing was seen (a zero row), NaN where only -inf was
+__device__ __forceinline__ float inverse_of(float M, float L) {
+  return M == kNegInf ? (L > 0.f ? __builtin_nanf("") : 0.f) : 1.0f / L;
+}
+// sum of a part as it enters a whole with maximum M
+__device__ __forceinline__ float sum_in(float m, float l, float M) {
+  return l * (M == kNegInf ? 1.f : part_of(m, M));
+}
+
+// 4 int8 codes (offset by 128 already) -> two dwords of fp16 pairs; 1024 + u is exact in fp16
+__device__ __forceinline__ uint32_t code_pair(uint32_t u, uint32_t sel) {
+  return as_u32(as_h2(perm_b32(0x64646464u, u, sel)) - half2v{(half_t)1152.f, (half_t)1152.f});
+}
+
 // The cache as the kernels take it: the page size as a shift.
 struct PagedCache {
   uint8_t* k;

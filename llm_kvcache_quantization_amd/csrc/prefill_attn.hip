@@ -9,10 +9,6 @@
 // (its column) of both, so the softmax is lane-local but for one exchange between the half-waves, made
 // only where the maximum moves, and P^T's operand is the lane's own scores, rounded to 16 bits.
 //
-// Lane (q, hh) = (lane % 32, lane / 32) of a 32 x 32 result holds rows 8 (i / 4) + 4 hh + i % 4 of column
-// q, i < 16.  The 8 reduction slots that P^T's operand takes from it are keys 16 mm + {4 hh + r, 8 + 4 hh +
-// r}, r < 4; V^T's operand has the same keys from two transposing LDS reads of 4 keys each.
-//
 // K and V tiles go straight from memory into LDS, two buffers each, the next tile's loads under the present
 // one's products.  Rows are XOR-swizzled in 16-byte chunks (by the lanes' choice of what they load), so that
 // the operands' reads spread over all banks.
@@ -26,13 +22,12 @@
 // exponentials), in turn in each wave.  Measured, us a call: 16384 tokens through a window of 4096, 28 heads, bf16, 958 (879
 // TFLOP/s; 912 to 1005 from card to card); 8192 tokens without a window 510 (943 TFLOP/s); a tile of 64 keys takes 1.75 us
 // on a CU of its own, 2.3 where two share one.
-#include "paged.h"
+#include "attn_tile.h"
 
 namespace kvq {
 namespace {
 
 constexpr int kBM = 128;      // queries a work-group
-constexpr int kBN = 64;       // keys a tile
 constexpr int kThreads = 256;
 
 struct PreArgs {
@@ -114,20 +109,12 @@ __device__ __forceinline__ int64_t unit_at(const PreArgs& a, uint32_t at) {
 __device__ __forceinline__ bool sees(int p, int key, int window, int sinks) {
   return key <= p && (window <= 0 || key > p - window || key < sinks);
 }
-__device__ __forceinline__ float xor32(float x) { return __shfl_xor(x, 32, 64); }
-// A tile in LDS.  K: [key][16 chunks of 8 channels], chunk ^ (key % 16); V: the same, chunk ^ 4 (key % 4).
-typedef u32x4 LdsTile[kBN * 16];
 // The buffers are variables of their own, and the loop is written out for both: only so does the compiler know
 // that the operands' reads of one need not wait for the loads into the other.
 struct Lds {
   LdsTile &k0, &v0, &k1, &v1;
   uint32_t (&bad)[2];  // keys of the tile whose V row is not finite
 };
-
-typedef __attribute__((address_space(3))) uint8_t lds_u8;
-typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
-typedef const __attribute__((address_space(1))) void* gptr;
-typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 // One side's tiles of rows key0 .. key0 + 63 into LDS.  A wave instruction loads four rows; a lane takes the
 // chunk that belongs at its place, 16 bytes from those of its neighbours.
@@ -161,9 +148,16 @@ struct TileLoad {
 };
 
 template <class T>
-struct Prefill {
-  float16v acc[4];
-  float m, l;
+struct Prefill : AttnTile<T> {
+  using AttnTile<T>::acc;
+  using AttnTile<T>::m;
+  using AttnTile<T>::l;
+  using AttnTile<T>::read_k;
+  using AttnTile<T>::read_v;
+  using AttnTile<T>::scores;
+  using AttnTile<T>::exps;
+  using AttnTile<T>::add_sum;
+  using AttnTile<T>::add_values;
   bool seen;
 
   // V of the second run: rows with an Inf or NaN as zeros, their keys marked
@@ -186,43 +180,6 @@ struct Prefill {
     }
   }
 
-  // K's operands of keys 32 u .. of the tile.
-  static __device__ __forceinline__ void read_k(const LdsTile& ks, int u, u32x4 (&kf)[8]) {
-    const int lane = threadIdx.x & 63, ql = lane & 31, hh = lane >> 5;
-#pragma unroll
-    for (int kk = 0; kk < 8; ++kk) kf[kk] = ks[(32 * u + ql) * 16 + ((2 * kk + hh) ^ (ql & 15))];
-  }
-
-  // V^T's operands of keys 32 u + 16 mm .., channels 32 ct .., in vf[4 mm + ct].  16 lanes of a transposing read
-  // take 4 keys of 16 channels: lane i brings 4 channels of key i / 4.
-  static __device__ __forceinline__ void read_v(const LdsTile& vs, int u, u32x4 (&vf)[8]) {
-    const int lane = threadIdx.x & 63, hh = lane >> 5, i = lane & 15;
-    const lds_u8* const vt = (const lds_u8*)&vs[0];
-    const int vrow = 32 * u + 4 * hh + (i >> 2);
-    const int vcol = 32 * ((lane >> 4) & 1) + 8 * (i & 3);  // bytes from the 32 channels' first
-#pragma unroll
-    for (int mm = 0; mm < 2; ++mm)
-#pragma unroll
-      for (int ct = 0; ct < 4; ++ct)
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          const int row = 16 * mm + 8 * w + vrow;  // row % 4 = i / 4
-          const int at = row * 256 + ((64 * ct + vcol) ^ ((i >> 2) << 6));
-          const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(vt + at)));
-          vf[4 * mm + ct][2 * w] = x[0];
-          vf[4 * mm + ct][2 * w + 1] = x[1];
-        }
-  }
-
-  static __device__ __forceinline__ float16v scores(const u32x4 (&kf)[8], const u32x4 (&q)[8]) {
-    float16v sc;
-#pragma unroll
-    for (int j = 0; j < 16; ++j) sc[j] = 0.f;
-#pragma unroll
-    for (int kk = 0; kk < 8; ++kk) sc = T::mfma32(kf[kk], q[kk], sc);
-    return sc;
-  }
-
   // Scaled scores with -inf where this lane's query does not see the key.
   __device__ __forceinline__ void mask(float16v& sc, const PreArgs& a, float scale, int key0, int u, int p) {
     // key = first + c, c < 32 a constant: c against this lane's last key, first key and end of the sinks
@@ -235,45 +192,6 @@ struct Prefill {
       seen |= vis;
       sc[j] = vis ? sc[j] * scale : kNegInf;
     }
-  }
-
-  // P of 32 keys, in 16 bits, from the scores times mul; returns this lane's sum of it.
-  __device__ __forceinline__ float exps(const float16v& sc, float mul, u32x4 (&pb)[2]) const {
-    const float mm = -(m == kNegInf ? 0.f : m);
-    float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-    for (int j = 0; j < 16; j += 2) {
-      const float e0 = fast_exp2(fmaf(sc[j], mul, mm)), e1 = fast_exp2(fmaf(sc[j + 1], mul, mm));
-      s0 += e0;
-      s1 += e1;
-      pb[j >> 3][(j >> 1) & 3] = T::pack(e0, e1);
-    }
-    return s0 + s1;
-  }
-
-  // While a lane's sum stays below 64 (2^15 in fp16) so does each of its P: the maximum, kUp below the largest score,
-  // follows only where it does not.
-  __device__ __forceinline__ void add_sum(float sum, const float16v& sc, float mul, u32x4 (&pb)[2]) {
-    if (__any(!(sum <= 64.f * (1 << (int)T::kUp)) || m == kNegInf)) {
-      float mx = kNegInf;
-#pragma unroll
-      for (int j = 0; j < 16; ++j) mx = fmaxf(mx, sc[j] * mul);
-      mx = fmaxf(fmaxf(mx, xor32(mx)) - T::kUp, m);
-      const float f = fast_exp2(m - (mx == kNegInf ? 0.f : mx));
-      l *= f;
-#pragma unroll
-      for (int ct = 0; ct < 4; ++ct) acc[ct] *= f;
-      m = mx;
-      sum = exps(sc, mul, pb);
-    }
-    l += sum;
-  }
-
-  __device__ __forceinline__ void add_values(const u32x4 (&vf)[8], const u32x4 (&pb)[2]) {
-#pragma unroll
-    for (int mm = 0; mm < 2; ++mm)
-#pragma unroll
-      for (int ct = 0; ct < 4; ++ct) acc[ct] = T::mfma32(vf[4 * mm + ct], pb[mm], acc[ct]);
   }
 
   // A tile's products, 32 keys at a time.  Operands are read from LDS a step before they are used: V's under
