@@ -69,6 +69,16 @@ __device__ __forceinline__ float sum_in(float m, float l, float M) {
   return l * (M == kNegInf ? 1.f : part_of(m, M));
 }
 
+__device__ __forceinline__ int scan64(int x) {  // inclusive, over the lanes
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // 1, 2, 4, 8 lanes up in rows of 16
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // lane 15 to the row above, lane 31 to the half above
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+  return x;
+}
+
 // 4 int8 codes (offset by 128 already) -> two dwords of fp16 pairs; 1024 + u is exact in fp16
 __device__ __forceinline__ uint32_t code_pair(uint32_t u, uint32_t sel) {
   return as_u32(as_h2(perm_b32(0x64646464u, u, sel)) - half2v{(half_t)1152.f, (half_t)1152.f});

@@ -98,16 +98,6 @@ struct Rows {
   }
 };
 
-__device__ __forceinline__ int scan64(int x) {  // inclusive, over the lanes
-  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // 1, 2, 4, 8 lanes up in rows of 16
-  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // lane 15 to the row above, lane 31 to the half above
-  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
-  return x;
-}
-
 // every thread of the work-group calls it
 template <int THREADS>
 __device__ __forceinline__ Rows scan_rows(const DecArgs& a, int* lds, int* wsum) {

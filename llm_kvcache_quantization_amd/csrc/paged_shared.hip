@@ -27,7 +27,7 @@ constexpr int kThreads = 256;
 constexpr int kCols = 128;      // columns a work-group
 constexpr int kMaxRows = 4096;  // rows of a call
 constexpr int kMaxRep = 128;    // query heads of a KV head
-constexpr int kMaxChunks = 64;  // work-groups of a tail
+constexpr int kMaxChunks = 64;  // work-groups of a tail, where there are more rows than lanes
 
 // A prefix's work-group: columns col0 .. of the group whose first row is row0, tiles t0 .. t1 of its first len tokens; its
 // parts are slot .. slot + cols - 1 of a KV head's.
@@ -59,28 +59,71 @@ struct ShArgs {
   int32_t q_heads, rep;
   const Unit* units;
   const RowPlan* rows;
-  int32_t chunks;        // of a tail, at most
-  int32_t prefix_slots;  // parts of the prefixes of a KV head; then those of the tails, [row][chunk][head]
-  uint32_t tails;        // work-groups of tails, the launch's first
+  int32_t chunks;        // of a tail, at most, where there are more than 64 rows, else 0
+  int32_t fill;          // work-groups that the tails of a KV head are shared out over (and one more a row, at most)
+  int32_t prefix_slots;  // parts of the prefixes of a KV head; then those of the tails, [work-group][head]
+  uint32_t tails;        // work-groups of tails, the launch's last
+  int4* places;          // [batch] Tails
   int64_t slots;         // parts of a KV head
   float2* ml;            // [kv_heads][slots]
   float* acc;            // [kv_heads][slots][128]
 };
 
-constexpr int kTailTiles = 2;  // least tiles of a tail's work-group
+constexpr int kTailTiles = 3;  // least tiles of a tail's work-group
 
 // The tiles of a row's own tokens lo .. hi - 1.
 struct Tail {
-  int lo, hi, first, count, chunks;
-  __device__ __forceinline__ Tail(const ShArgs& a, const RowPlan& r, int b) {
+  int lo, hi, first, count;
+  bool shares;  // the row takes part in its group's prefix
+  __device__ __forceinline__ Tail(const ShArgs& a, int len, int n) {
     const int64_t cap = (int64_t)a.c.max_pages << a.c.lg;
-    hi = (int)min((int64_t)max(((const_i32)a.lens)[b], 0), cap);
-    lo = hi >= r.len ? r.len : 0;
+    hi = (int)min((int64_t)max(n, 0), cap);
+    shares = hi >= len;
+    lo = shares ? len : 0;
     first = lo / kBN;
     count = hi > lo ? (hi + kBN - 1) / kBN - first : 0;
-    chunks = min(a.chunks, (count + kTailTiles - 1) / kTailTiles);
   }
-  __device__ __forceinline__ int begin(int i) const { return first + (int)((uint32_t)count * (uint32_t)i / (uint32_t)chunks); }
+  // of `chunks` even runs of tiles, the i-th's first
+  __device__ __forceinline__ int begin(int i, int chunks) const { return first + (int)((uint32_t)count * (uint32_t)i / (uint32_t)chunks); }
+};
+
+// Which row a tail's work-group is of, and which of its chunks; and, of each row, what the join needs: {first
+// work-group, work-groups, whether it shares}.  Up to 64 rows are in a wave's lanes: the tiles of all are shared out
+// evenly, whatever their lengths.  More have as many chunks each.
+struct Tails {
+  int row, chunk, chunks;
+  __device__ __forceinline__ Tails(const ShArgs& a, int at, bool write) {
+    const int B = a.c.batch;
+    row = -1;
+    if (a.chunks) {
+      if (at < B * a.chunks) {
+        const int b = at / a.chunks;
+        chunk = at % a.chunks;
+        const Tail t(a, plan_of_row(a.rows, b).len, ((const_i32)a.lens)[b]);
+        chunks = min(a.chunks, (t.count + kTailTiles - 1) / kTailTiles);
+        if (write && chunk == 0 && threadIdx.x == 0) a.places[b] = {b * a.chunks, chunks, t.shares, 0};
+        if (chunk < chunks) row = b;
+      }
+      return;
+    }
+    const int lane = threadIdx.x & 63;
+    int count = 0;
+    bool shares = false;
+    if (lane < B) {
+      const Tail t(a, a.rows[lane].len, a.lens[lane]);
+      count = t.count;
+      shares = t.shares;
+    }
+    const int total = __builtin_amdgcn_readlane(scan64(count), 63);
+    const int per = max((total + a.fill - 1) / a.fill, kTailTiles);
+    const int mine = (count + per - 1) / per, before = scan64(mine) - mine;
+    if (write && at == 0 && threadIdx.x < (uint32_t)B) a.places[lane] = {before, mine, shares, 0};
+    const uint64_t here = __ballot(lane < B && before <= at && at < before + mine);
+    if (!here) return;
+    row = __builtin_ctzll(here);
+    chunk = at - __builtin_amdgcn_readlane(before, row);
+    chunks = __builtin_amdgcn_readlane(mine, row);
+  }
 };
 
 __device__ const u32x4 zero_row[16] = {};
@@ -90,18 +133,18 @@ struct Source {
   const uint8_t *k, *v, *ks, *vs;
   const_i32 table;
   int lo, hi;
+  // every token of a tile is there and seen (ok: there())
+  __device__ __forceinline__ bool whole(int key0, uint32_t ok) const { return ok == 15 && key0 >= lo && key0 + kBN <= hi; }
 };
 
-struct Pages {
-  int32_t n[4];  // of 16 tokens each
-};
+typedef int32_t Pages __attribute__((ext_vector_type(4)));  // of a tile's tokens, 16 each (a vector: registers, whatever picks from it)
 
 __device__ __forceinline__ Pages pages_of(const PagedCache& c, const Source& s, int tile) {
   Pages p;
 #pragma unroll
   for (int u = 0; u < 4; ++u) {
     const int i = (tile * kBN + 16 * u) >> c.lg;
-    p.n[u] = i < c.max_pages ? s.table[i] : -1;
+    p[u] = i < c.max_pages ? s.table[i] : -1;
   }
   return p;
 }
@@ -110,34 +153,38 @@ __device__ __forceinline__ Pages pages_of(const PagedCache& c, const Source& s, 
 __device__ __forceinline__ uint32_t there(const PagedCache& c, const Pages& p) {
   uint32_t ok = 0;
 #pragma unroll
-  for (int u = 0; u < 4; ++u) ok |= (uint32_t)((uint32_t)p.n[u] < (uint32_t)c.num_pages) << u;
+  for (int u = 0; u < 4; ++u) ok |= (uint32_t)((uint32_t)p[u] < (uint32_t)c.num_pages) << u;
   return ok;
+}
+
+// Where 16 consecutive tokens of a page begin, of one side.  All of it is scalar, and on a wave's way from tile to tile: page
+// strides below 2^32 bytes (the host's check) take two instructions to multiply where 64 bits take five.
+__device__ __forceinline__ const uint8_t* block_of(const PagedCache& c, const uint8_t* x, int64_t page_stride, int64_t row_stride, int32_t page, int token) {
+  return x + (uint64_t)(uint32_t)page * (uint32_t)page_stride + (uint32_t)(token & c.page_mask) * (uint32_t)row_stride;
 }
 
 // A tile's rows from 16-bit pages straight into LDS.  A wave instruction loads four rows of 16; a lane takes the chunk
 // that belongs at its place.
 struct Direct {
   uint32_t k_off, v_off;
-  int row, chunk;
-  __device__ __forceinline__ Direct(const PagedCache& c) {
+  int wave, row, chunk;
+  __device__ __forceinline__ Direct(const PagedCache& c, int wave_) : wave(wave_) {
     const int lane = threadIdx.x & 63;
-    row = 4 * (threadIdx.x >> 6) + (lane >> 4);
+    row = 4 * wave + (lane >> 4);
     chunk = lane & 15;
     k_off = (uint32_t)row * (uint32_t)c.kst + (uint32_t)(chunk ^ row) * 16;
     v_off = (uint32_t)row * (uint32_t)c.vst + (uint32_t)(chunk ^ ((row & 3) << 2)) * 16;
   }
+  template <bool ALL>
   __device__ __forceinline__ void load(const PagedCache& c, const Source& s, int key0, const Pages& p, uint32_t ok, LdsTile& kt,
                                        LdsTile& vt) const {
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const bool all = ok == 15 && key0 >= s.lo && key0 + kBN <= s.hi;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int at = 16 * u + 4 * wave;  // the wave's first row
-      const uint32_t slot = (uint32_t)((key0 + 16 * u) & c.page_mask);
-      const int64_t page = (ok >> u & 1) ? p.n[u] : 0;
-      const uint8_t* kp = s.k + page * c.ksp + slot * (uint32_t)c.kst + k_off;
-      const uint8_t* vp = s.v + page * c.vsp + slot * (uint32_t)c.vst + v_off;
-      if (!all) {
+      const int32_t page = ALL || (ok >> u & 1) ? p[u] : 0;
+      const uint8_t* kp = block_of(c, s.k, c.ksp, c.kst, page, key0 + 16 * u) + k_off;
+      const uint8_t* vp = block_of(c, s.v, c.vsp, c.vst, page, key0 + 16 * u) + v_off;
+      if constexpr (!ALL) {
         const int key = key0 + 16 * u + row;
         const bool there = (ok >> u & 1) && key >= s.lo && key < s.hi;
         kp = there ? kp : (const uint8_t*)(zero_row + chunk);
@@ -147,71 +194,191 @@ struct Direct {
       __builtin_amdgcn_global_load_lds((gptr)vp, (__attribute__((address_space(3))) void*)(&vt[at * 16]), 16, 0, 0);
     }
   }
+  __device__ __forceinline__ void operator()(const PagedCache& c, const Source& s, int key0, const Pages& p, uint32_t ok, LdsTile& kt,
+                                             LdsTile& vt) const {
+    if (s.whole(key0, ok)) load<true>(c, s, key0, p, ok, kt, vt);
+    else load<false>(c, s, key0, p, ok, kt, vt);
+  }
 };
 
-// A tile's rows from INT8 pages: 16 codes of a row a piece, two pieces of K and of V a thread, in registers while the
-// tile before it is worked on, then code x scale in fp16 (the framework's own dequantization) into LDS.
+// A tile of INT8 pages as it is, straight into LDS: K's codes [64][128]; V's with the scales [64][G] of both sides.
+typedef u32x4 KCodes[kBN * 8];
+template <int G>
+struct VCodes {
+  u32x4 v[kBN * 8];
+  uint32_t ks[G == 1 ? 64 : kBN * G / 2], vs[G == 1 ? 64 : kBN * G / 2];  // at least a wave's load
+};
+
+// A thread's places in a tile of INT8 pages.  A wave instruction loads eight rows of 8 pieces of 16 codes, and a dword of
+// scales a lane (half a token's, one or two tokens'); waves 0 and 1 take K's scales, 2 and 3 V's, twice where one has all.
 template <int GS>
 struct Coded {
   static constexpr int G = 128 / GS;
-  u32x4 k[2], v[2];
-  uint16_t ks[2], vs[2];
-  __device__ __forceinline__ void load(const PagedCache& c, const Source& s, int key0, const Pages& p, uint32_t ok) {
-    const int piece = threadIdx.x & 7, half = __builtin_amdgcn_readfirstlane(threadIdx.x >> 7);
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int row = (threadIdx.x >> 3) + 32 * e, key = key0 + row;  // of tokens 16 (2 e + half) ..
-      const bool up = half != 0, good = (ok >> (2 * e + half)) & 1;
-      const int64_t page = good ? (up ? p.n[2 * e + 1] : p.n[2 * e]) : 0;
-      const uint32_t slot = (uint32_t)(key & c.page_mask);
-      const bool there = good && key >= s.lo && key < s.hi;
-      const uint8_t* kp = s.k + page * c.ksp + slot * (uint32_t)c.kst + piece * 16;
-      const uint8_t* vp = s.v + page * c.vsp + slot * (uint32_t)c.vst + piece * 16;
-      const uint8_t* ksp = s.ks + page * c.kssp + slot * (2 * G) + piece * 16 / GS * 2;
-      const uint8_t* vsp = s.vs + page * c.vssp + slot * (2 * G) + piece * 16 / GS * 2;
-      const uint8_t* const zero = (const uint8_t*)zero_row;
-      k[e] = ld_stream<u32x4>(there ? kp : zero);
-      v[e] = ld_stream<u32x4>(there ? vp : zero);
-      ks[e] = *(const uint16_t*)(there ? ksp : zero);
-      vs[e] = *(const uint16_t*)(there ? vsp : zero);
-    }
+  uint32_t k_off, v_off;  // of the wave's rows from the first of their 16
+  int wave, row, s_row;   // in the tile: the first piece's (the second's is 32 behind), the scale dword's
+  uint32_t k_at, v_at;    // LDS: the first piece's operands
+  __device__ __forceinline__ Coded(const PagedCache& c, int wave_) : wave(wave_) {
+    const int tid = threadIdx.x, lane = tid & 63;
+    row = tid >> 3;
+    const uint32_t piece = tid & 7;
+    k_off = (uint32_t)(row & 15) * (uint32_t)c.kst + piece * 16;
+    v_off = (uint32_t)(row & 15) * (uint32_t)c.vst + piece * 16;
+    const int i = (G == 4 ? tid & 64 : 0) + lane;
+    s_row = min(i * 2 / G, kBN - 1);
+    k_at = (uint32_t)row * 256 + ((2 * piece) ^ (uint32_t)(row & 15)) * 16;
+    v_at = (uint32_t)row * 256 + ((2 * piece) ^ (uint32_t)((row & 3) << 2)) * 16;
   }
-  static __device__ __forceinline__ void put(u32x4 x, uint16_t scale, u32x4* lo, u32x4* hi) {
-    const half2v s = as_h2(scale * 0x00010001u);
+
+  // The codes of one side: the wave's rows lie in one block of 16 for each piece.
+  template <bool V>
+  __device__ __forceinline__ void load(const PagedCache& c, const Source& s, int key0, const Pages& p, uint32_t ok, u32x4* to) const {
+    const bool upper = wave >= 2;
+    if (s.whole(key0, ok)) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      u32x4 y;
+      for (int e = 0; e < 2; ++e)
+        put<V>(c, s, upper ? p[2 * e + 1] : p[2 * e], key0 + 32 * e + (upper ? 16 : 0), true, to + 256 * e + 64 * wave);
+    } else {
 #pragma unroll
-      for (int d = 0; d < 2; ++d) {
-        const uint32_t u = x[2 * h + d] ^ 0x80808080u;
-        y[2 * d] = as_u32(as_h2(code_pair(u, 0x04010400u)) * s);
-        y[2 * d + 1] = as_u32(as_h2(code_pair(u, 0x04030402u)) * s);
+      for (int e = 0; e < 2; ++e) {
+        const bool good = ok >> (2 * e + upper) & 1;
+        const int key = key0 + row + 32 * e;
+        put<V>(c, s, good ? (upper ? p[2 * e + 1] : p[2 * e]) : 0, key0 + 32 * e + (upper ? 16 : 0),
+               good && key >= s.lo && key < s.hi, to + 256 * e + 64 * wave);
       }
-      *(h ? hi : lo) = y;
     }
   }
-  __device__ __forceinline__ void store(LdsTile& kt, LdsTile& vt) const {
-    const int piece = threadIdx.x & 7;
+  template <bool V>
+  __device__ __forceinline__ void put(const PagedCache& c, const Source& s, int32_t page, int token, bool there, u32x4* to) const {
+    const uint8_t* x = V ? block_of(c, s.v, c.vsp, c.vst, page, token) + v_off : block_of(c, s.k, c.ksp, c.kst, page, token) + k_off;
+    if (!there) x = (const uint8_t*)zero_row;
+    __builtin_amdgcn_global_load_lds((gptr)x, (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+  }
+  __device__ __forceinline__ void load_scales(const PagedCache& c, const Source& s, int key0, const Pages& p, uint32_t ok, VCodes<G>& to) const {
+    const bool v = wave >= 2;
+    const uint8_t* const x = v ? s.vs : s.ks;
+    const uint32_t page_stride = (uint32_t)(v ? c.vssp : c.kssp);
+    uint32_t* const lds = (v ? to.vs : to.ks) + (G == 4 ? 64 * (wave & 1) : 0);
+    const uint32_t in_token = G == 4 ? 4 * (threadIdx.x & 1) : 0;
+    if (ok == 15 && c.lg >= 6) {  // a tile of one page
+      const uint32_t at = (uint32_t)((key0 & c.page_mask) + s_row) * (2 * G) / 4 * 4 + in_token;
+      __builtin_amdgcn_global_load_lds((gptr)(x + (uint64_t)(uint32_t)p[0] * page_stride + at), (__attribute__((address_space(3))) void*)lds, 4, 0, 0);
+    } else {
+      const int u = s_row >> 4;
+      const int32_t n = u < 2 ? (u ? p[1] : p[0]) : u == 2 ? p[2] : p[3];
+      const uint32_t at = (uint32_t)((key0 + s_row) & c.page_mask) * (2 * G) / 4 * 4 + in_token;
+      const uint8_t* y = x + (uint64_t)(uint32_t)n * page_stride + at;
+      if (!(ok >> u & 1)) y = (const uint8_t*)zero_row;
+      __builtin_amdgcn_global_load_lds((gptr)y, (__attribute__((address_space(3))) void*)lds, 4, 0, 0);
+    }
+  }
+
+  // K's operands from its codes: the codes themselves, exact in fp16, whose scales come to the scores.
+  __device__ __forceinline__ void decode_k(const KCodes& from, LdsTile& kt) const {
+    lds_u8* const to = (lds_u8*)&kt[0];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const int row = (threadIdx.x >> 3) + 32 * e;
-      put(k[e], ks[e], &kt[row * 16 + ((2 * piece) ^ (row & 15))], &kt[row * 16 + ((2 * piece + 1) ^ (row & 15))]);
-      put(v[e], vs[e], &vt[row * 16 + ((2 * piece) ^ ((row & 3) << 2))], &vt[row * 16 + ((2 * piece + 1) ^ ((row & 3) << 2))]);
+      const u32x4 x = from[threadIdx.x + 256 * e];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        u32x4 k;
+#pragma unroll
+        for (int d = 0; d < 2; ++d) {
+          const uint32_t a = x[2 * h + d] ^ 0x80808080u;
+          k[2 * d] = code_pair(a, 0x04010400u);
+          k[2 * d + 1] = code_pair(a, 0x04030402u);
+        }
+        *(lds_u32x4*)(to + (k_at ^ (16 * h)) + 8192 * e) = k;
+      }
+    }
+  }
+  // V's operands: code x scale in fp16, the framework's own dequantization, 0 for tokens that nobody sees.
+  __device__ __forceinline__ void decode_v(const Source& s, int key0, uint32_t ok, const VCodes<G>& from, LdsTile& vt) const {
+    lds_u8* const to = (lds_u8*)&vt[0];
+    const bool all = s.whole(key0, ok);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      uint32_t scale = ((const uint16_t*)from.vs)[(row + 32 * e) * G + (threadIdx.x & 7) * 16 / GS];
+      if (!all) {
+        const int at = row + 32 * e, key = key0 + at;
+        if (!((ok >> (at >> 4) & 1) && key >= s.lo && key < s.hi)) scale = 0;
+      }
+      const half2v f = as_h2(scale * 0x00010001u);
+      const u32x4 x = from.v[threadIdx.x + 256 * e];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        u32x4 v;
+#pragma unroll
+        for (int d = 0; d < 2; ++d) {
+          const uint32_t a = x[2 * h + d] ^ 0x80808080u;
+          v[2 * d] = as_u32(as_h2(code_pair(a, 0x04010400u)) * f);
+          v[2 * d + 1] = as_u32(as_h2(code_pair(a, 0x04030402u)) * f);
+        }
+        *(lds_u32x4*)(to + v_at + 16 * h + 8192 * e) = v;
+      }
     }
   }
 };
 
-template <class M>
+__device__ __forceinline__ float half_of(uint32_t w, int up) {
+  return (float)__builtin_bit_cast(half_t, (uint16_t)(up ? w >> 16 : w));
+}
+
+// G: groups of an INT8 row's scales; 0 where K's values come as they are.
+template <class M, int G>
 struct Shared : AttnTile<M> {
   using AttnTile<M>::acc;
   using AttnTile<M>::m;
   using AttnTile<M>::l;
   bool seen;
 
-  // A tile's tokens 32 u0 .. 32 u1 - 1.
+  // Scores of codes: of each group by itself, times the tokens' scales.  Two groups at a time, whose scales are read for them:
+  // all four have no room.
+  static __device__ __forceinline__ float16v code_scores(const u32x4 (&kf)[8], const u32x4 (&q)[8], const uint32_t* scales, int u) {
+    const uint16_t* const first = (const uint16_t*)scales + (32 * u + 4 * ((threadIdx.x & 63) >> 5)) * G;
+    float16v sc;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) sc[j] = 0.f;
+    constexpr int N = G < 2 ? G : 2;
+#pragma unroll
+    for (int g0 = 0; g0 < G; g0 += N) {
+      if (g0) __builtin_amdgcn_sched_barrier(0);
+      uint32_t w[16];  // token j's, of groups g0 and g0 + 1
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const uint16_t* const x = first + (8 * (j >> 2) + (j & 3)) * G + g0;
+        if constexpr (G == 1) w[j] = *x;
+        else w[j] = *(const uint32_t*)x;
+      }
+#pragma unroll
+      for (int g = g0; g < g0 + N; ++g) {
+        float16v d;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) d[j] = 0.f;
+#pragma unroll
+        for (int kk = 8 * g / G; kk < 8 * (g + 1) / G; ++kk) d = M::mfma32(kf[kk], q[kk], d);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) sc[j] = fmaf(d[j], half_of(w[j], g - g0), sc[j]);
+      }
+    }
+    return sc;
+  }
+
+  // Scaled scores with -inf for the tokens of a half that nobody sees.
+  __device__ __forceinline__ void mask(float16v& sc, const Source& s, float scale, int key0, uint32_t ok, int u) {
+    const int first = 32 * u + 4 * ((threadIdx.x & 63) >> 5);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const int at = first + 8 * (j >> 2) + (j & 3);  // in the tile
+      const bool vis = key0 + at >= s.lo && key0 + at < s.hi && (ok >> (at >> 4) & 1);
+      seen |= vis;
+      sc[j] = vis ? sc[j] * scale : kNegInf;
+    }
+  }
+
+  // A tile's tokens 32 u0 .. 32 u1 - 1: values as they are.
   __device__ __forceinline__ void tile(const LdsTile& ks, const LdsTile& vs, const Source& s, const u32x4 (&q)[8], float scale,
                                        int key0, uint32_t ok, int u0, int u1) {
-    const bool full = ok == 15 && key0 >= s.lo && key0 + kBN <= s.hi;
+    const bool full = s.whole(key0, ok);
     const float mul = full ? scale : 1.f;
     seen |= full;
     u32x4 kf[8], vf[8], pb[2];
@@ -222,28 +389,66 @@ struct Shared : AttnTile<M> {
       float16v sc = this->scores(kf, q);
       this->read_v(vs, u, vf);
       __builtin_amdgcn_sched_barrier(0);
-      if (!full) {
-        const int first = 32 * u + 4 * ((threadIdx.x & 63) >> 5);
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const int at = first + 8 * (j >> 2) + (j & 3);  // in the tile
-          const bool vis = key0 + at >= s.lo && key0 + at < s.hi && (ok >> (at >> 4) & 1);
-          seen |= vis;
-          sc[j] = vis ? sc[j] * scale : kNegInf;
-        }
-      }
+      if (!full) mask(sc, s, scale, key0, ok, u);
       this->add_sum(this->exps(sc, mul, pb), sc, mul, pb);
       if (u + 1 < u1) this->read_k(ks, u + 1, kf);
       __builtin_amdgcn_sched_barrier(0);
       this->add_values(vf, pb);
     }
   }
+
+  // The same of codes, up to P, and the product with V, pb[half].
+  __device__ __forceinline__ void code_probs(const LdsTile& ks, const uint32_t* scales, const Source& s, const u32x4 (&q)[8], float scale,
+                                             int key0, uint32_t ok, int u0, int u1, u32x4 (&pb)[2][2]) {
+    const bool full = s.whole(key0, ok);
+    const float mul = full ? scale : 1.f;
+    seen |= full;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int u = u0 + i;
+      if (u >= u1) break;
+      u32x4 kf[8];
+      this->read_k(ks, u, kf);
+      float16v sc = code_scores(kf, q, scales, u);
+      __builtin_amdgcn_sched_barrier(0);
+      if (!full) mask(sc, s, scale, key0, ok, u);
+      const float before = m;
+      this->add_sum(this->exps(sc, mul, pb[i]), sc, mul, pb[i]);
+      if (i == 1 && __any(m != before)) {  // the first half's P stand at the maximum before this one
+        const float f = fast_exp2(before - shift_of(m));
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int d = 0; d < 4; ++d)
+            pb[0][x][d] = M::pack(M::to_f((uint16_t)pb[0][x][d]) * f, M::to_f((uint16_t)(pb[0][x][d] >> 16)) * f);
+      }
+    }
+  }
+  __device__ __forceinline__ void code_values(const LdsTile& vs, int u0, int u1, const u32x4 (&pb)[2][2]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (u0 + i >= u1) break;
+      u32x4 vf[8];
+      this->read_v(vs, u0 + i, vf);
+      this->add_values(vf, pb[i]);
+    }
+  }
 };
+
+// A barrier of the work-group for its LDS alone: loads that are under way stay so.
+__device__ __forceinline__ void barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 template <class T, bool I8, int GS>
 __global__ __launch_bounds__(kThreads, 2) void shared_decode_kernel(ShArgs a) {
   using M = typename std::conditional<I8, TF16, T>::type;  // the matrix instructions' type
-  __shared__ LdsTile k0, v0, k1, v1;
+  constexpr int G = I8 ? 128 / GS : 0;
+  // 16-bit pages: two buffers; INT8: one for the operands, two for codes.  Each is a variable of its own, so that the
+  // compiler does not wait for what is being loaded into one where another is read.
+  __shared__ LdsTile k0, v0;
+  __shared__ typename std::conditional<I8, KCodes, LdsTile>::type k1;
+  __shared__ typename std::conditional<I8, VCodes<I8 ? G : 1>, LdsTile>::type v1;
+  __shared__ typename std::conditional<I8, KCodes, u32x4[1]>::type k2;
+  __shared__ typename std::conditional<I8, VCodes<I8 ? G : 1>, u32x4[1]>::type v2;
   __shared__ float2 half_ml[2][32];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ql = lane & 31, hh = lane >> 5, rep = a.rep;
@@ -254,21 +459,24 @@ __global__ __launch_bounds__(kThreads, 2) void shared_decode_kernel(ShArgs a) {
   int64_t slot;
   Source s;
   {
+    // the prefixes first: their runs are the longest
+    const uint32_t prefixes = gridDim.x - a.tails;
     uint32_t at = blockIdx.x;
-    if (at < a.tails) {
+    if (at >= prefixes) {
+      at -= prefixes;
       h = (int)(at % (uint32_t)H);
       at /= (uint32_t)H;
-      const int chunk = (int)(at % (uint32_t)a.chunks), b = (int)(at / (uint32_t)a.chunks);
+      const Tails mine(a, (int)at, h == 0);
+      const int b = __builtin_amdgcn_readfirstlane(mine.row);
+      if (b < 0) return;
       const RowPlan r = plan_of_row(a.rows, b);
-      const Tail tail(a, r, b);
-      if (chunk >= tail.chunks) return;
+      const Tail tail(a, r.len, ((const_i32)a.lens)[b]);
       row0 = b; col0 = 0; cols = rep;
-      t = tail.begin(chunk); t1 = tail.begin(chunk + 1);
+      t = tail.begin(mine.chunk, mine.chunks); t1 = tail.begin(mine.chunk + 1, mine.chunks);
       s.lo = tail.lo; s.hi = tail.hi;
-      s.table = (const_i32)(pc.table + (tail.lo == r.len ? b : r.row0) * pc.table_stride);
-      slot = a.prefix_slots + ((int64_t)b * a.chunks + chunk) * rep;
+      s.table = (const_i32)(pc.table + (tail.shares ? b : r.row0) * pc.table_stride);
+      slot = a.prefix_slots + (int64_t)at * rep;
     } else {
-      at -= a.tails;
       h = (int)(at % (uint32_t)H);
       const const_i32 w = (const_i32)(a.units + at / (uint32_t)H);
       const Unit u{w[0], w[1], w[2], w[3], w[4], w[5], w[6], 0};
@@ -300,7 +508,7 @@ __global__ __launch_bounds__(kThreads, 2) void shared_decode_kernel(ShArgs a) {
     if (a.inv_tau) scale *= a.inv_tau[head];
   }
 
-  Shared<M> f;
+  Shared<M, G> f;
 #pragma unroll
   for (int ct = 0; ct < 4; ++ct)
 #pragma unroll
@@ -312,18 +520,18 @@ __global__ __launch_bounds__(kThreads, 2) void shared_decode_kernel(ShArgs a) {
   Pages p = pages_of(pc, s, t);
   uint32_t ok = there(pc, p);
   if constexpr (!I8) {
-    const Direct d(pc);
+    const Direct d(pc, wave);
     auto arrived = [&]() {  // this wave's loads have, and then every wave's; the other buffer is free
       __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
       __syncthreads();
     };
-    d.load(pc, s, t * kBN, p, ok, k0, v0);
+    d(pc, s, t * kBN, p, ok, k0, v0);
     p = pages_of(pc, s, min(t + 1, t1 - 1));
     for (; t < t1; t += 2) {
       arrived();
       uint32_t ok1 = there(pc, p);
       if (t + 1 < t1) {
-        d.load(pc, s, (t + 1) * kBN, p, ok1, k1, v1);
+        d(pc, s, (t + 1) * kBN, p, ok1, k1, v1);
         p = pages_of(pc, s, min(t + 2, t1 - 1));
       }
       if (active) f.tile(k0, v0, s, q, scale, t * kBN, ok, u0, u1);
@@ -331,15 +539,26 @@ __global__ __launch_bounds__(kThreads, 2) void shared_decode_kernel(ShArgs a) {
       arrived();
       ok = there(pc, p);
       if (t + 2 < t1) {
-        d.load(pc, s, (t + 2) * kBN, p, ok, k0, v0);
+        d(pc, s, (t + 2) * kBN, p, ok, k0, v0);
         p = pages_of(pc, s, min(t + 3, t1 - 1));
       }
       if (active) f.tile(k1, v1, s, q, scale, (t + 1) * kBN, ok1, u0, u1);
     }
   } else {
-    Coded<GS> d;
-    d.load(pc, s, t * kBN, p, ok);
-    p = pages_of(pc, s, min(t + 1, t1 - 1));
+    // Tiles past the run's end are loaded like any, from the zeros: the waits are the same in every turn.
+    const Coded<GS> d(pc, wave);
+    u32x4 pb[2][2];
+    Pages p1 = pages_of(pc, s, min(t + 1, t1 - 1));
+    uint32_t ok1 = t + 1 < t1 ? there(pc, p1) : 0;
+    auto load_v = [&](int tile, const Pages& at, uint32_t good, VCodes<G>& to) {
+      d.template load<true>(pc, s, tile * kBN, at, good, to.v);
+      d.load_scales(pc, s, tile * kBN, at, good, to);
+    };
+    d.template load<false>(pc, s, t * kBN, p, ok, k1);
+    load_v(t, p, ok, v1);
+    d.template load<false>(pc, s, (t + 1) * kBN, p1, ok1, k2);
+    load_v(t + 1, p1, ok1, v2);
+    p = pages_of(pc, s, min(t + 2, t1 - 1));
     if constexpr (std::is_same<T, TB16>::value) {
       // bf16 values in fp16: exact once the column's largest is scaled to [1, 2) by a power of two (what lies 2^24
       // and more below it loses bits that are below the sum's)
@@ -360,26 +579,37 @@ __global__ __launch_bounds__(kThreads, 2) void shared_decode_kernel(ShArgs a) {
         for (int j = 0; j < 4; ++j)
           q[kk][j] = TF16::pack(TB16::to_f((uint16_t)q[kk][j]) * g, TB16::to_f((uint16_t)(q[kk][j] >> 16)) * g);
     }
-    d.store(k0, v0);
-    for (; t < t1; t += 2) {
-      __syncthreads();
-      uint32_t ok1 = there(pc, p);
-      if (t + 1 < t1) {
-        d.load(pc, s, (t + 1) * kBN, p, ok1);
-        p = pages_of(pc, s, min(t + 2, t1 - 1));
-      }
-      if (active) f.tile(k0, v0, s, q, scale, t * kBN, ok, u0, u1);
-      if (t + 1 == t1) break;
-      d.store(k1, v1);
-      __syncthreads();
-      ok = there(pc, p);
-      if (t + 2 < t1) {
-        d.load(pc, s, (t + 2) * kBN, p, ok);
-        p = pages_of(pc, s, min(t + 3, t1 - 1));
-      }
-      if (active) f.tile(k1, v1, s, q, scale, (t + 1) * kBN, ok1, u0, u1);
-      if (t + 2 < t1) d.store(k0, v0);
+    __builtin_amdgcn_s_waitcnt(0x0F78);  // vmcnt(8): the first K
+    barrier();
+    d.decode_k(k1, k0);
+    // A wave has two loads of K's codes and three of V's codes and scales under way while it awaits those before them.
+    auto arrived = [&]() {
+      __builtin_amdgcn_s_waitcnt(0x0F75);  // vmcnt(5)
+      barrier();
+    };
+    arrived();
+    // One tile: its scores while V is decoded, its product with V while the next tile's K is.
+    auto turn = [&](KCodes& kc, VCodes<G>& vc, const KCodes& next) {
+      const uint32_t ok2 = t + 2 < t1 ? there(pc, p) : 0;
+      d.template load<false>(pc, s, (t + 2) * kBN, p, ok2, kc);
+      d.decode_v(s, t * kBN, ok, vc, v0);
+      if (active) f.code_probs(k0, vc.ks, s, q, scale, t * kBN, ok, u0, u1, pb);
+      arrived();  // the next K
+      load_v(t + 2, p, ok2, vc);
+      p = pages_of(pc, s, min(t + 3, t1 - 1));
+      d.decode_k(next, k0);
+      if (active) f.code_values(v0, u0, u1, pb);
+      arrived();  // the next V
+      ok = ok1;
+      ok1 = ok2;
+      ++t;
+    };
+    while (t + 1 < t1) {  // no way out of its middle: the compiler would wait for all loads at its start
+      turn(k1, v1, k2);
+      turn(k2, v2, k1);
     }
+    if (t < t1) turn(k1, v1, k2);
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): no load may come after the work-group
   }
 
   // a sum whose maximum is -inf is none: 1 where something was seen, else 0
@@ -388,7 +618,7 @@ __global__ __launch_bounds__(kThreads, 2) void shared_decode_kernel(ShArgs a) {
   if (f.m == kNegInf && f.l == f.l) f.l = f.seen ? 1.f : 0.f;
   if (halves) {
     __syncthreads();  // the buffers are free
-    float4v* const other = (float4v*)(block ? k1 : k0);  // [16][64]
+    float4v* const other = (float4v*)(block ? v0 : k0);  // [16][64]
     if (active && u0 == 1) {
       if (hh == 0) half_ml[block][ql] = float2{f.m, f.l};
 #pragma unroll
@@ -430,25 +660,37 @@ __global__ __launch_bounds__(kThreads) void shared_join_kernel(ShArgs a) {
   const int rep = a.rep, cc = threadIdx.x & 15, sl = threadIdx.x >> 4;
   const int head = blockIdx.x, b = blockIdx.y, h = head / rep;
   const RowPlan r = plan_of_row(a.rows, b);
-  const Tail tail(a, r, b);
-  const int splits = tail.lo == r.len ? r.splits : 0;
+  const const_i32 place = (const_i32)(a.places + b);
+  const int chunks = place[1], splits = place[2] ? r.splits : 0;
   const int c = (b - r.row0) * rep + head % rep, c0 = c / max(r.per, 1) * r.per, width = min(r.per, r.cols - c0);
   const int64_t first = h * a.slots + r.slot + (int64_t)c0 * r.splits + (c - c0);
-  const int64_t own = h * a.slots + a.prefix_slots + (int64_t)b * a.chunks * rep + head % rep;
+  const int64_t own = h * a.slots + a.prefix_slots + (int64_t)place[0] * rep + head % rep;
   float m = kNegInf, l = 0.f, o[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) o[k] = 0.f;
-  for (int w = sl; w < splits + tail.chunks; w += 16) {
-    const int64_t slot = w < splits ? first + (int64_t)w * width : own + (int64_t)(w - splits) * rep;
-    const float2 p = a.ml[slot];
-    const float4v x = *(const float4v*)(a.acc + slot * 128 + cc * 8), y = *(const float4v*)(a.acc + slot * 128 + cc * 8 + 4);
-    const float top = fmaxf(m, p.x), f0 = part_of(m, top), f1 = part_of(p.x, top);
-    l = sum_in(m, l, top) + sum_in(p.x, p.y, top);
-    m = top;
+  const int parts = splits + chunks;
+  for (int w = sl; w < parts; w += 64) {  // four parts' loads side by side; past the end the last one again, without weight
+    float2 p[4];
+    float4v x[4], y[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      o[k] = o[k] * f0 + x[k] * f1;
-      o[4 + k] = o[4 + k] * f0 + y[k] * f1;
+    for (int u = 0; u < 4; ++u) {
+      const int i = min(w + 16 * u, parts - 1);
+      const int64_t slot = i < splits ? first + (int64_t)i * width : own + (int64_t)(i - splits) * rep;
+      p[u] = a.ml[slot];
+      x[u] = *(const float4v*)(a.acc + slot * 128 + cc * 8);
+      y[u] = *(const float4v*)(a.acc + slot * 128 + cc * 8 + 4);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (w + 16 * u >= parts) break;
+      const float top = fmaxf(m, p[u].x), f0 = part_of(m, top), f1 = part_of(p[u].x, top);
+      l = sum_in(m, l, top) + sum_in(p[u].x, p[u].y, top);
+      m = top;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        o[k] = o[k] * f0 + x[u][k] * f1;
+        o[4 + k] = o[4 + k] * f0 + y[u][k] * f1;
+      }
     }
   }
 #pragma unroll
@@ -471,8 +713,11 @@ __global__ __launch_bounds__(kThreads) void shared_join_kernel(ShArgs a) {
 
 // ---------------------------------------------------------------- host
 
-constexpr int kTarget = 512;     // work-groups that fill the GPU: two a CU
-constexpr int kMinTiles = 2;     // least tiles of a prefix's work-group
+constexpr int kTarget = 512;        // work-groups that fill the GPU: two a CU
+constexpr int kPrefixTarget = 384;  // those of them for the prefixes, and where that leaves each more than kLong tiles
+constexpr int kLongTarget = 448;
+constexpr int kLong = 12;
+constexpr int kMinTiles = 3;        // least tiles of a prefix's work-group
 constexpr int kMaxSplits = 256;
 
 int plan(const int32_t* sizes, const int32_t* lens, int32_t groups, int32_t q_heads, int32_t kv_heads, kvq_shared_plan_info* info,
@@ -489,10 +734,8 @@ int plan(const int32_t* sizes, const int32_t* lens, int32_t groups, int32_t q_he
     if (rows > kMaxRows) return fail(KVQ_ERR_UNSUPPORTED, "shared plan: more than 4096 rows");
     work += (sizes[g] * rep + kCols - 1) / kCols * (((int64_t)lens[g] + kBN - 1) / kBN);
   }
-  // tiles a work-group: what fills the GPU beside one work-group of each row and KV head for the tails
-  int64_t target = kTarget - rows * kv_heads;
-  if (target < kTarget / 2) target = kTarget / 2;
-  int64_t quota = (work * kv_heads + target - 1) / target;
+  int64_t quota = (work * kv_heads + kPrefixTarget - 1) / kPrefixTarget;  // tiles a work-group
+  if (quota > kLong) quota = (work * kv_heads + kLongTarget - 1) / kLongTarget;
   if (quota < kMinTiles) quota = kMinTiles;
   int64_t units = 0, slots = 0, row = 0;
   const auto put = [&](int64_t at, const int32_t (&w)[8]) {
@@ -534,13 +777,16 @@ int check(const kvq_shared_decode_params* p, PagedCache& c) {
   if (p->q_heads / c.kv_heads > kMaxRep) return fail(KVQ_ERR_UNSUPPORTED, "shared decode: more than 128 query heads a KV head");
   if (p->q_heads > 65535) return fail(KVQ_ERR_UNSUPPORTED, "shared decode: too many heads");
   if (c.batch > kMaxRows) return fail(KVQ_ERR_UNSUPPORTED, "shared decode: more than 4096 rows");
+  const int64_t strides[4] = {c.ksp, c.vsp, c.kssp, c.vssp};
+  for (int64_t x : strides)
+    if (x < 0 || x >> 32) return fail(KVQ_ERR_UNSUPPORTED, "shared decode: page stride out of range");
   if (p->plan.rows != c.batch || p->plan.units < 0 || p->plan.slots < 0) return fail(KVQ_ERR_INVALID, "shared decode: the plan is of another batch");
   return KVQ_OK;
 }
 
 struct Launch {
-  int chunks;             // of a tail
-  int64_t slots, acc, bytes;
+  int chunks, fill;
+  int64_t slots, places, acc, bytes;
   int64_t tails, grid;
 };
 
@@ -548,15 +794,27 @@ Launch launch_of(const kvq_shared_decode_params& p) {
   Launch w{};
   const int64_t B = p.cache.batch, H = p.cache.kv_heads, rep = p.q_heads / H;
   const int64_t tiles = ((int64_t)p.cache.max_pages * p.cache.page_size + kBN - 1) / kBN;
-  int64_t chunks = kTarget / (B > 0 ? B * H : 1);
-  const int64_t most = (tiles + kTailTiles - 1) / kTailTiles;
-  if (chunks > kMaxChunks) chunks = kMaxChunks;
-  if (chunks > most) chunks = most;
-  w.chunks = (int)(chunks < 1 ? 1 : chunks);
-  w.slots = p.plan.slots + B * w.chunks * rep;
-  w.acc = (8 * H * w.slots + 63) / 64 * 64;
+  const int64_t most = (tiles + kTailTiles - 1) / kTailTiles;  // of a row
+  int64_t groups;  // work-groups of tails, a KV head
+  if (B <= 64) {
+    int64_t fill = kTarget / H - p.plan.units;  // what the prefixes leave
+    if (fill < (kTarget - kPrefixTarget) / H) fill = (kTarget - kPrefixTarget) / H;
+    if (fill < B) fill = B;
+    w.fill = (int)fill;
+    groups = fill + B < B * most ? fill + B : B * most;
+    if (groups < 1) groups = 1;  // who writes the places
+  } else {
+    int64_t chunks = kTarget / (B * H);
+    if (chunks > kMaxChunks) chunks = kMaxChunks;
+    if (chunks > most) chunks = most;
+    w.chunks = (int)(chunks < 1 ? 1 : chunks);
+    groups = B * w.chunks;
+  }
+  w.slots = p.plan.slots + groups * rep;
+  w.places = (8 * H * w.slots + 63) / 64 * 64;
+  w.acc = w.places + (16 * B + 63) / 64 * 64;
   w.bytes = w.acc + 512 * H * w.slots;
-  w.tails = B * H * w.chunks;
+  w.tails = H * groups;
   w.grid = w.tails + H * p.plan.units;
   return w;
 }
@@ -592,11 +850,12 @@ int decode(const kvq_shared_decode_params* p, hipStream_t st) {
   a.q_heads = p->q_heads; a.rep = p->q_heads / a.c.kv_heads;
   a.rows = (const RowPlan*)p->plan_words;
   a.units = (const Unit*)(p->plan_words + 8 * (int64_t)p->plan.rows);
-  a.chunks = w.chunks;
+  a.chunks = w.chunks; a.fill = w.fill;
   a.prefix_slots = p->plan.slots;
   a.tails = (uint32_t)w.tails;
   a.slots = w.slots;
   a.ml = (float2*)p->workspace;
+  a.places = (int4*)((uint8_t*)p->workspace + w.places);
   a.acc = (float*)((uint8_t*)p->workspace + w.acc);
   const bool b16 = p->q_type == KVQ_PAGED_BF16;
   const int gs = p->cache.format == KVQ_PAGED_INT8 ? p->cache.group_size : 0;

@@ -170,7 +170,7 @@ def decode_attn_shared(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_table:
     with n = ``context_lens[b]`` (the new token included), out = softmax_t(sm_scale * inv_tau[h] * q . k_t) @ v_t over t < n,
     statistics and sums in fp32; token t < ``prefix.lens[g]`` lies in the pages of the group's first sequence, whatever
     b's own table says there.  Sequences that see nothing are zero.  fp16 / bf16 pages must have q's type; INT8 pages
-    serve both, with the values code * scale in fp16 (as ``get_kv`` gives them).  Hq / Hkv is at most 128, B at most 4096.
+    serve both (V's values code * scale are used in fp16).  Hq / Hkv is at most 128, B at most 4096.
     """
     if q.ndim != 3 or q.shape[2] != HEAD_DIM:
         raise ValueError(f"q must be [B, Hq, {HEAD_DIM}], got {tuple(q.shape)}")

@@ -5,7 +5,7 @@ What a call must not look at is poisoned: a sequence's own slots below its prefi
 of nobody hold NaN (INT8: NaN scales); table entries of the prefix of all but a group's first sequence name no page.
 
 Tolerances are those derived in test_gpu_paged (output, probabilities, scores, sums), over the values that the call
-works with: INT8 codes x scale rounded to fp16, so that their rounding adds nothing."""
+works with: K's codes x scale, V's code x scale rounded to fp16, so that their rounding adds nothing."""
 import math
 
 import pytest
@@ -46,7 +46,7 @@ class Groups(Pool):
 
     def values(self):
         k, v = super().values()
-        return (k.half().double(), v.half().double()) if self.int8 else (k, v)
+        return (k, v.half().double()) if self.int8 else (k, v)
 
 
 def call(pool, q, **kw):
