@@ -3,14 +3,16 @@
 //   p = softmax(x / T),  log p_t = (x_t - m) / T - log l,  H = log l - sum (x - m) / T e^((x - m) / T) / l,
 //   l = sum e^((x - m) / T)
 //
-// One pass over the logits: each thread keeps a running maximum m and the two sums in fp32.  What bounds it: HBM; few
-// rows are split over work-groups, whose parts a second launch joins.
+// One pass over the logits: each thread keeps a running maximum m and the two sums in fp32.  What bounds it: HBM, and the
+// vector units nearly as much (8 instructions a logit, one of them an exponential); few rows are split over
+// work-groups, whose parts a second launch joins.
 //
-// The likeliest: a wave keeps a list of candidates of its own in LDS, and what all but its `top` best are below.  A
-// vector is looked at only where its largest logit reaches that bar.  A candidate is one whole number, the
-// logit's order above the complement of the token's, so that no two are equal and the lower token wins among equal
-// logits; a list that is full is cut down to its best by counting, for each, how many are above it.  Sorted lists
-// (of waves, then of work-groups) are joined by taking the largest of their heads, `top` times.
+// The likeliest: the pass leaves the maximum of every 32 logits that a lane takes (of 64 and more in long rows) in LDS.  The
+// top-th largest of 64 groups' maxima is a bar that at least `top` logits reach; only the 32s that reach it are read
+// again, and what reaches it in them, hardly more than `top` logits, is put in order by counting, for each, how many are
+// above it.  A candidate is one whole number, the logit's order above the complement of the token's, so that no two
+// are equal and the lower token wins among equal logits.  Rows that have too many candidates (masks that leave
+// fewer than `top`, many equal logits) are gone through again with lists (pick).
 #include <type_traits>
 
 #include "kvq_logprobs.h"
@@ -23,7 +25,10 @@ constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kVec = 4;                         // 16-byte vectors of a thread a step
 constexpr int kTop = KVQ_LOGPROBS_MAX_TOP;
-constexpr int kList = 128;                      // candidates of a wave
+constexpr int kList = 128;                      // candidates of a wave's list
+constexpr int kSlots = 16;                      // maxima that a thread leaves
+constexpr int kBlocks = 128;                    // of them, those that are read again
+constexpr int kKeys = kWaves * kList;           // candidates of a work-group
 constexpr int kMaxParts = 64;                   // work-groups of a row
 constexpr float kLowest = -3.4028234664e38f;
 
@@ -85,7 +90,7 @@ __device__ __forceinline__ uint64_t read_lane(uint64_t x, int lane) {
 
 typedef __attribute__((address_space(3))) uint64_t lds_u64;
 
-// A wave's candidates: `count` of them in its list, of which the best `top` are kept.
+// A wave's candidates where there are many: `count` of them in its list, of which the best `top` are kept.
 struct List {
   lds_u64* key;    // [kList], this wave's
   uint64_t bar;    // no key at or below it is among the best
@@ -133,190 +138,280 @@ struct List {
   }
 };
 
-// The k-th largest of the lanes' values: as many values as that are at or above it.
-__device__ __forceinline__ float kth_of_lanes(float x, int k) {
-  const int lane = threadIdx.x & 63;
-  int above = 0;
-#pragma unroll 8
-  for (int i = 0; i < 64; ++i) {
-    const float y = row_lane(x, i);
-    above += y > x || (y == x && i < lane);
-  }
-  return row_lane(x, __builtin_ctzll(__ballot(above == k - 1)));
-}
-
-// The `top` largest keys of up to 64 sorted lists (lane p: list p of `have` keys); lane i < top has the i-th.
-__device__ __forceinline__ uint64_t best_of(const lds_u64* list, int have, int top) {
-  const int lane = threadIdx.x & 63;
-  int at = 0;
-  uint64_t head = have > 0 ? list[0] : 0, mine = 0;
-  for (int i = 0; i < top; ++i) {
-    uint64_t best = head;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-      const uint64_t other = __shfl_xor((unsigned long long)best, o, 64);
-      best = other > best ? other : best;
-    }
-    if (lane == i) mine = best;
-    if (head == best) head = ++at < have ? list[at] : 0;  // no two keys are equal, but for the 0 of an empty list
-  }
-  return mine;
-}
-
 template <class T>
 __device__ __forceinline__ float value_at(const uint8_t* p) {
   if constexpr (std::is_same<T, float>::value) return *(const float*)p;
   else return T::to_f(*(const uint16_t*)p);
 }
 
-// Writes a row's outputs from its sums and, in the lanes, its best keys.  One wave.
+// A logit's log p.
+struct LogP {
+  float m, inv, log_l;
+  bool none;
+  __device__ __forceinline__ LogP(const LpArgs& a, const Sums& f) : m(f.m), inv(a.inv), log_l(logf(f.l)), none(f.m == kNegInf) {}
+  __device__ __forceinline__ float operator()(float x) const { return none ? __builtin_nanf("") : fmaf(x - m, inv, -log_l); }
+};
+
+// Writes a row's log p of its token and its entropy.  One thread.
 template <class T>
-__device__ __forceinline__ void finish(const LpArgs& a, int64_t row, Sums f, uint64_t key) {
-  const int lane = threadIdx.x & 63;
-  const float log_l = logf(f.l), nan = __builtin_nanf("");
-  const bool none = f.m == kNegInf;
-  auto log_p = [&](float x) { return none ? nan : fmaf(x - f.m, a.inv, -log_l); };
-  if (lane == 0) {
-    a.entropy[row] = none ? nan : fmaxf(log_l - a.inv * (f.s / f.l), 0.f) + 0.f * f.l;
-    if (a.tokens) {
-      const int64_t t = a.tokens64 ? ((const int64_t*)a.tokens)[row] : ((const int32_t*)a.tokens)[row];
-      a.logprobs[row] = t >= 0 && t < a.vocab
-                            ? log_p(value_at<T>(a.logits + row * a.row_bytes + t * (std::is_same<T, float>::value ? 4 : 2))) : nan;
-    }
-  }
-  if (lane < a.top) {
-    a.top_tokens[row * a.top + lane] = (int64_t)(uint32_t)~(uint32_t)key;
-    a.top_logprobs[row * a.top + lane] = log_p(logit_of(key));
-  }
+__device__ __forceinline__ void finish(const LpArgs& a, int64_t row, const Sums& f) {
+  const LogP log_p(a, f);
+  const float nan = __builtin_nanf("");
+  a.entropy[row] = log_p.none ? nan : fmaxf(log_p.log_l - a.inv * (f.s / f.l), 0.f) + 0.f * f.l;
+  if (!a.tokens) return;
+  const int64_t t = a.tokens64 ? ((const int64_t*)a.tokens)[row] : ((const int32_t*)a.tokens)[row];
+  a.logprobs[row] = t >= 0 && t < a.vocab ? log_p(value_at<T>(a.logits + row * a.row_bytes + t * (std::is_same<T, float>::value ? 4 : 2))) : nan;
 }
 
+// Calls out(place, key) for the best `top` of n keys in LDS, place by place, by any thread.
+template <int THREADS, class F>
+__device__ __forceinline__ void best_of(const lds_u64* key, int n, int top, F out) {
+  for (int i = threadIdx.x; i < n; i += THREADS) {
+    const uint64_t mine = key[i];
+    int above = 0;
+    for (int j = 0; j < n; ++j) above += key[j] > mine;
+    if (above < top) out(above, mine);
+  }
+}
+__device__ __forceinline__ void put_top(const LpArgs& a, int64_t row, const LogP& log_p, int place, uint64_t key) {
+  a.top_tokens[row * a.top + place] = (int64_t)(uint32_t)~(uint32_t)key;
+  a.top_logprobs[row * a.top + place] = log_p(logit_of(key));
+}
+
+// A work-group's part of a row.
+template <class T>
+struct Part {
+  static constexpr int E = std::is_same<T, float>::value ? 4 : 8, S = 16 / E;  // logits of a vector, bytes of one
+  const uint8_t* x0;
+  const u32x4* v;   // the row's whole vectors, from its first aligned logit on: begin .. end - 1 of them are the part's
+  int head, begin, end;
+  int first, rest;  // logits before the first vector and behind the last, where they are this part's
+  __device__ __forceinline__ Part(const LpArgs& a, int64_t row, int part) {
+    x0 = a.logits + row * a.row_bytes;
+    head = min((int)(((0u - (uint32_t)(uintptr_t)x0) & 15u) / S), a.vocab);
+    const int vectors = (a.vocab - head) / E;
+    v = (const u32x4*)(x0 + head * S);
+    begin = (int)((int64_t)vectors * part / a.parts);
+    end = (int)((int64_t)vectors * (part + 1) / a.parts);
+    first = part == 0 ? head : 0;
+    rest = part == 0 ? a.vocab - head - vectors * E : 0;
+  }
+  // token i of the first + rest
+  __device__ __forceinline__ int edge(const LpArgs& a, int i) const { return i < first ? i : a.vocab - rest + i - first; }
+  static __device__ __forceinline__ float logit(const u32x4& w, int e) {
+    const uint32_t bits = w[e * 4 / E];
+    if constexpr (E == 4) return __builtin_bit_cast(float, bits);
+    else return T::to_f((uint16_t)(bits >> (e & 1 ? 16 : 0)));
+  }
+};
+
+// The part's best, by lists, whatever there is in it: a wave's `top` best at a time are what the next have to pass.
+// Leaves each wave's in its list, count[wave] of them.
+template <class T>
+__device__ __attribute__((noinline)) void pick(const LpArgs* a, const Part<T>* p, lds_u64* keys, int* count) {
+  constexpr int E = Part<T>::E;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  List list{keys + wave * kList, 0, kNegInf, 0, a->top};
+  for (int at = p->begin + wave * 64; at < p->end; at += kThreads) {
+    const int i = at + lane;
+    const bool there = i < p->end;
+    u32x4 w = {0, 0, 0, 0};
+    if (there) w = p->v[i];
+    for (int e = 0; e < E; ++e) {
+      // element e of a vector in registers, e not a constant
+      const uint32_t lo = E == 4 ? (e < 2 ? (e ? w[1] : w[0]) : e == 2 ? w[2] : w[3])
+                                 : (e < 4 ? (e < 2 ? w[0] : w[1]) : e < 6 ? w[2] : w[3]);
+      float x;
+      if constexpr (E == 4) x = __builtin_bit_cast(float, lo);
+      else x = T::to_f((uint16_t)(lo >> (e & 1 ? 16 : 0)));
+      if (__any(there && !(x < list.low))) list.offer(key_of(x, p->head + i * E + e), there);
+    }
+  }
+  if (wave == 0) {
+    const int n = p->first + p->rest, token = p->edge(*a, lane);
+    list.offer(lane < n ? key_of(value_at<T>(p->x0 + (int64_t)token * Part<T>::S), token) : 0, lane < n);
+  }
+  list.cut();
+  if (lane == 0) count[wave] = list.count;
+}
+
+// Work of a launch: a part of a row a work-group.
 template <class T, bool TOP>
 __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
-  constexpr int E = std::is_same<T, float>::value ? 4 : 8, S = 16 / E;  // logits of a vector, bytes of one
-  __shared__ uint64_t keys[TOP ? kWaves * kList : 1];
+  using P = Part<T>;
+  constexpr int E = P::E;
+  __shared__ float maxima[TOP ? kSlots : 1][kThreads];
+  __shared__ uint64_t keys[TOP ? kKeys : 1];
+  __shared__ uint32_t blocks[TOP ? kBlocks : 1];
   __shared__ Sums sums[kWaves];
-  __shared__ int counts[kWaves];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t parts = (uint32_t)a.parts;
-  const int64_t row = blockIdx.x / parts;
-  const int part = (int)(blockIdx.x % parts);
-  const uint8_t* const x0 = a.logits + row * a.row_bytes;
-  // the row's whole vectors, from its first aligned logit on, and this work-group's share of them
-  const int head = min((int)(((0u - (uint32_t)(uintptr_t)x0) & 15u) / S), a.vocab), vectors = (a.vocab - head) / E;
-  const u32x4* const v = (const u32x4*)(x0 + head * S);
-  const int begin = (int)((int64_t)vectors * part / a.parts), end = (int)((int64_t)vectors * (part + 1) / a.parts);
+  __shared__ float group[TOP ? kThreads : 1];
+  __shared__ int counts[kWaves], n_blocks, n_keys;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t row = blockIdx.x / (uint32_t)a.parts;
+  const int part = (int)(blockIdx.x % (uint32_t)a.parts);
+  const P p(a, row, part);
+  // a thread's steps, and how many of them a maximum is of
+  const int steps = (p.end - p.begin + kThreads * kVec - 1) / (kThreads * kVec), per = (steps + kSlots - 1) / kSlots;
+  if (TOP && tid == 0) n_blocks = n_keys = 0;
 
   Sums f{kNegInf, 0.f, 0.f};
-  List list{(lds_u64*)keys + (TOP ? wave * kList : 0), 0, kNegInf, 0, a.top};
+  float most = kNegInf, all = kNegInf;  // of the slot, of all
   auto step = [&](int at, bool whole) {
     u32x4 w[kVec];
 #pragma unroll
     for (int u = 0; u < kVec; ++u) {
       const int i = at + 64 * u + lane;
-      if (whole || i < end) w[u] = ld_stream<u32x4>(v + i);
+      if (whole || i < p.end) w[u] = ld_stream<u32x4>(p.v + i);
     }
-    float x[kVec][E], top[kVec];
+    float x[kVec][E], mx = kNegInf;
 #pragma unroll
     for (int u = 0; u < kVec; ++u) {
-      const bool there = whole || at + 64 * u + lane < end;
+      const bool there = whole || at + 64 * u + lane < p.end;
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const uint32_t bits = w[u][e * 4 / E];
-        if constexpr (E == 4) x[u][e] = __builtin_bit_cast(float, bits);
-        else x[u][e] = T::to_f((uint16_t)(bits >> (e & 1 ? 16 : 0)));
-        if (!there) x[u][e] = kNegInf;
+        x[u][e] = there ? P::logit(w[u], e) : kNegInf;
+        mx = fmaxf(mx, x[u][e]);
       }
-      top[u] = x[u][0];
-#pragma unroll
-      for (int e = 1; e < E; ++e) top[u] = fmaxf(top[u], x[u][e]);
     }
-    float mx = top[0];
-#pragma unroll
-    for (int u = 1; u < kVec; ++u) mx = fmaxf(mx, top[u]);
     if (mx > f.m) f.to(mx, a.c);
 #pragma unroll
     for (int u = 0; u < kVec; ++u)
 #pragma unroll
       for (int e = 0; e < E; ++e) f.add_logit(x[u][e], a.c);
-    if constexpr (TOP) {
-      const bool first = list.bar == 0;
-      if (first) list.low = fmaxf(list.low, kth_of_lanes(mx == mx ? mx : kNegInf, list.top));  // that many reach it
-#pragma unroll
-      for (int u = 0; u < kVec; ++u) {
-        if (!__any(!(top[u] < list.low))) continue;
-        const int i = at + 64 * u + lane;
-        const bool there = whole || i < end;
-#pragma unroll
-        for (int e = 0; e < E; ++e) list.offer(key_of(x[u][e], head + i * E + e), there && !(x[u][e] < list.low));
-      }
-      if (first) list.cut();
-    }
+    most = fmaxf(most, mx);
   };
-  int at = begin + wave * 64 * kVec;
-  for (; at + 64 * kVec <= end; at += kThreads * kVec) step(at, true);
-  if (at < end) step(at, false);
-  // the logits before the first vector and behind the last: fewer than 16
-  if (part == 0 && wave == 0) {
-    const int rest = a.vocab - head - vectors * E;
-    const bool there = lane < head + rest;
-    const int token = lane < head ? lane : a.vocab - rest + lane - head;
-    const float x = there ? value_at<T>(x0 + token * S) : kNegInf;
+  {
+    int at = p.begin + wave * 64 * kVec;
+    for (int i = 0, slot = 0; slot < kSlots && i < steps; ++slot) {
+      for (int j = 0; j < per && i < steps; ++j, ++i, at += kThreads * kVec) {
+        if (at + 64 * kVec <= p.end) step(at, true);
+        else if (at < p.end) step(at, false);
+      }
+      if constexpr (TOP) maxima[slot][tid] = most;
+      all = fmaxf(all, most);
+      most = kNegInf;
+    }
+  }
+  if (wave == 0 && p.first + p.rest > 0) {  // fewer than 16
+    const bool there = lane < p.first + p.rest;
+    const float x = there ? value_at<T>(p.x0 + (int64_t)p.edge(a, lane) * P::S) : kNegInf;
     if (x > f.m) f.to(x, a.c);
     f.add_logit(x, a.c);
-    if constexpr (TOP) list.offer(key_of(x, token), there);
   }
-
-  // the lanes' sums, then the waves'
   f.lanes(a.c);
-  if constexpr (TOP) list.cut();
-  if (lane == 0) {
-    sums[wave] = f;
-    counts[wave] = list.count;
-  }
+  if (lane == 0) sums[wave] = f;
+  if constexpr (TOP) group[tid] = all;
   __syncthreads();
-  if (wave) return;
+  if (!TOP && wave) return;
   f = sums[0];
   for (int w = 1; w < kWaves; ++w) f.add(sums[w], a.c);
-  uint64_t key = 0;
-  if constexpr (TOP) key = best_of((lds_u64*)keys + (lane < kWaves ? lane : 0) * kList, lane < kWaves ? counts[lane] : 0, a.top);
-  if (a.parts == 1) {
-    finish<T>(a, row, f, key);
-    return;
+  if (tid == 0) {
+    if (a.parts == 1) finish<T>(a, row, f);
+    else a.sums[row * a.parts + part] = float4v{f.m, f.l, f.s, 0.f};
   }
-  if (lane == 0) a.sums[row * a.parts + part] = float4v{f.m, f.l, f.s, 0.f};
-  if (TOP && lane < a.top) a.keys[(row * a.parts + part) * a.top + lane] = key;
+  if constexpr (TOP) {
+    // the bar: the top-th largest of 64 groups' maxima
+    float mine = group[lane];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) mine = fmaxf(mine, group[64 * w + lane]);
+    int above = 0;
+#pragma unroll 8
+    for (int i = 0; i < 64; ++i) {
+      const float y = row_lane(mine, i);
+      above += y > mine || (y == mine && i < lane);
+    }
+    const float bar = row_lane(mine, __builtin_ctzll(__ballot(above == a.top - 1)));
+    for (int slot = 0; slot * per < steps; ++slot)
+      if (maxima[slot][tid] >= bar) {
+        const int i = atomicAdd(&n_blocks, 1);
+        if (i < kBlocks) blocks[i] = (uint32_t)(slot << 16 | tid);
+      }
+    if (tid < p.first + p.rest) {
+      const int token = p.edge(a, tid);
+      const float x = value_at<T>(p.x0 + (int64_t)token * P::S);
+      keys[atomicAdd(&n_keys, 1)] = key_of(x, token);
+    }
+    __syncthreads();
+    const int nb = n_blocks;
+    bool many = nb > kBlocks || bar == kNegInf;
+    if (!many) {
+      for (int i = tid; i < nb * per * kVec; i += kThreads) {
+        const uint32_t b = blocks[i / (per * kVec)];
+        const int j = i % (per * kVec), it = (int)(b >> 16) * per + j / kVec, t = (int)(b & 0xFFFF);
+        const int at = p.begin + (it * kThreads + (t >> 6) * 64) * kVec + 64 * (j % kVec) + (t & 63);
+        if (it >= steps || at >= p.end) continue;
+        const u32x4 w = p.v[at];
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const float x = P::logit(w, e);
+          if (x >= bar) {
+            const int k = atomicAdd(&n_keys, 1);
+            if (k < kKeys) keys[k] = key_of(x, p.head + at * E + e);
+          }
+        }
+      }
+      __syncthreads();
+      many = n_keys > kKeys;
+    }
+    int n = n_keys;
+    if (many) {
+      const LpArgs args = a;
+      const P mine2 = p;
+      __syncthreads();
+      pick<T>(&args, &mine2, (lds_u64*)keys, counts);
+      __syncthreads();
+      // the lists one behind the other: each wave moves its own, which ends before the next one's begins
+      n = 0;
+      for (int w = 0; w < kWaves; ++w) {
+        const int c = counts[w];
+        const uint64_t k = tid < c ? keys[w * kList + tid] : 0;
+        __syncthreads();
+        if (tid < c) keys[n + tid] = k;
+        __syncthreads();
+        n += c;
+      }
+    }
+    if (a.parts == 1) {
+      const LogP log_p(a, f);
+      best_of<kThreads>((const lds_u64*)keys, n, a.top, [&](int place, uint64_t key) { put_top(a, row, log_p, place, key); });
+    } else {
+      uint64_t* const out = a.keys + (row * a.parts + part) * a.top;
+      for (int i = n + tid; i < a.top; i += kThreads) out[i] = 0;  // below all keys
+      best_of<kThreads>((const lds_u64*)keys, n, a.top, [&](int place, uint64_t key) { out[place] = key; });
+    }
+  }
 }
 
-// Joins the parts of a row: a wave.
+// Joins the parts of a row: a work-group.
 template <class T>
-__global__ __launch_bounds__(64) void logprobs_join_kernel(LpArgs a) {
+__global__ __launch_bounds__(kThreads) void logprobs_join_kernel(LpArgs a) {
   __shared__ uint64_t keys[kMaxParts * kTop];
-  const int lane = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63;
   const int64_t row = blockIdx.x;
+  const int n = a.parts * a.top;
+  for (int i = tid; i < n; i += kThreads) keys[i] = a.keys[row * n + i];
   Sums f{kNegInf, 0.f, 0.f};
   if (lane < a.parts) {
     const float4v x = a.sums[row * a.parts + lane];
     f = Sums{x[0], x[1], x[2]};
   }
   f.lanes(a.c);
-  uint64_t key = 0;
-  if (a.top) {
-    for (int i = lane; i < a.parts * a.top; i += 64) keys[i] = a.keys[row * a.parts * a.top + i];
-    __syncthreads();
-    // a part of fewer logits ends its list with zeros, which are below all keys
-    key = best_of((lds_u64*)keys + (lane < a.parts ? lane * a.top : 0), lane < a.parts ? a.top : 0, a.top);
-  }
-  finish<T>(a, row, f, key);
+  if (tid == 0) finish<T>(a, row, f);
+  if (!a.top) return;
+  __syncthreads();
+  const LogP log_p(a, f);
+  best_of<kThreads>((const lds_u64*)keys, n, a.top, [&](int place, uint64_t key) { put_top(a, row, log_p, place, key); });
 }
 
 // ---------------------------------------------------------------- host
 
-constexpr int kFill = 2048;  // work-groups that fill the GPU
+constexpr int kFill = 2048;   // work-groups that fill the GPU
+constexpr int kMost = 1024;   // rows from which on each has one
 
 // Work-groups of a row: as many as fill the GPU, none of less than a step.
 int parts_of(const kvq_token_logprobs_params& p) {
   const int64_t step = (int64_t)kThreads * kVec * (p.logits_type == KVQ_LOGITS_F32 ? 4 : 8);
-  int64_t parts = p.rows > 0 ? (kFill + p.rows - 1) / p.rows : 1;
+  int64_t parts = p.rows > 0 && p.rows < kMost ? (kFill + p.rows - 1) / p.rows : 1;
   const int64_t most = ((int64_t)p.vocab + step - 1) / step;
   if (parts > most) parts = most;
   if (parts > kMaxParts) parts = kMaxParts;
@@ -343,7 +438,7 @@ int launch(const LpArgs& a, hipStream_t st) {
   else hipLaunchKernelGGL((logprobs_kernel<T, false>), grid, dim3(kThreads), 0, st, a);
   int rc = launched();
   if (rc || a.parts == 1) return rc;
-  hipLaunchKernelGGL(logprobs_join_kernel<T>, dim3((unsigned)a.rows), dim3(64), 0, st, a);
+  hipLaunchKernelGGL(logprobs_join_kernel<T>, dim3((unsigned)a.rows), dim3(kThreads), 0, st, a);
   return launched();
 }
 
