@@ -163,12 +163,34 @@ __device__ __forceinline__ void finish(const LpArgs& a, int64_t row, const Sums&
   a.logprobs[row] = t >= 0 && t < a.vocab ? log_p(value_at<T>(a.logits + row * a.row_bytes + t * (std::is_same<T, float>::value ? 4 : 2))) : nan;
 }
 
-// Calls out(place, key) for the best `top` of n keys in LDS, place by place, by any thread.
-template <int THREADS, class F>
-__device__ __forceinline__ void best_of(const lds_u64* key, int n, int top, F out) {
-  for (int i = threadIdx.x; i < n; i += THREADS) {
+// Calls out(place, key) for the best `top` of n keys in LDS, place by place, by any thread of the work-group.  Many are
+// thinned out first, into `few` (room for n), by the top-th largest of 64 groups' largest: 380 keys, of 19 parts, counted as
+// they are take the join 13 us, so 4.
+template <class F>
+__device__ __forceinline__ void best_of(const lds_u64* key, int n, int top, lds_u64* few, int* count, F out) {
+  if (n > 2 * 64) {
+    const int lane = threadIdx.x & 63;
+    uint64_t mine = 0;
+    for (int i = lane; i < n; i += 64) mine = key[i] > mine ? key[i] : mine;
+    int above = 0;
+#pragma unroll 8
+    for (int i = 0; i < 64; ++i) {
+      const uint64_t y = read_lane(mine, i);
+      above += y > mine || (y == mine && i < lane);
+    }
+    const uint64_t bar = read_lane(mine, __builtin_ctzll(__ballot(above == top - 1)));
+    if (threadIdx.x == 0) *count = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kThreads)
+      if (key[i] >= bar) few[atomicAdd(count, 1)] = key[i];
+    __syncthreads();
+    key = few;
+    n = *count;
+  }
+  for (int i = threadIdx.x; i < n; i += kThreads) {
     const uint64_t mine = key[i];
     int above = 0;
+#pragma unroll 8
     for (int j = 0; j < n; ++j) above += key[j] > mine;
     if (above < top) out(above, mine);
   }
@@ -235,12 +257,14 @@ __device__ __attribute__((noinline)) void pick(const LpArgs* a, const Part<T>* p
   if (lane == 0) count[wave] = list.count;
 }
 
-// Work of a launch: a part of a row a work-group.
+static_assert(sizeof(float) * kSlots * kThreads >= sizeof(uint64_t) * kKeys, "the keys that are thinned out lie where the maxima were");
+
+// A part of a row a work-group.
 template <class T, bool TOP>
 __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
   using P = Part<T>;
   constexpr int E = P::E;
-  __shared__ float maxima[TOP ? kSlots : 1][kThreads];
+  __shared__ __attribute__((aligned(8))) float maxima[TOP ? kSlots : 1][kThreads];  // and room for kKeys keys
   __shared__ uint64_t keys[TOP ? kKeys : 1];
   __shared__ uint32_t blocks[TOP ? kBlocks : 1];
   __shared__ Sums sums[kWaves];
@@ -373,11 +397,11 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
     }
     if (a.parts == 1) {
       const LogP log_p(a, f);
-      best_of<kThreads>((const lds_u64*)keys, n, a.top, [&](int place, uint64_t key) { put_top(a, row, log_p, place, key); });
+      best_of((const lds_u64*)keys, n, a.top, (lds_u64*)&maxima[0][0], &n_blocks, [&](int place, uint64_t key) { put_top(a, row, log_p, place, key); });
     } else {
       uint64_t* const out = a.keys + (row * a.parts + part) * a.top;
       for (int i = n + tid; i < a.top; i += kThreads) out[i] = 0;  // below all keys
-      best_of<kThreads>((const lds_u64*)keys, n, a.top, [&](int place, uint64_t key) { out[place] = key; });
+      best_of((const lds_u64*)keys, n, a.top, (lds_u64*)&maxima[0][0], &n_blocks, [&](int place, uint64_t key) { out[place] = key; });
     }
   }
 }
@@ -385,7 +409,8 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
 // Joins the parts of a row: a work-group.
 template <class T>
 __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(LpArgs a) {
-  __shared__ uint64_t keys[kMaxParts * kTop];
+  __shared__ uint64_t keys[kMaxParts * kTop], few[kMaxParts * kTop];
+  __shared__ int count;
   const int tid = threadIdx.x, lane = tid & 63;
   const int64_t row = blockIdx.x;
   const int n = a.parts * a.top;
@@ -400,13 +425,16 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(LpArgs a) {
   if (!a.top) return;
   __syncthreads();
   const LogP log_p(a, f);
-  best_of<kThreads>((const lds_u64*)keys, n, a.top, [&](int place, uint64_t key) { put_top(a, row, log_p, place, key); });
+  best_of((const lds_u64*)keys, n, a.top, (lds_u64*)few, &count, [&](int place, uint64_t key) { put_top(a, row, log_p, place, key); });
 }
 
 // ---------------------------------------------------------------- host
 
 constexpr int kFill = 2048;   // work-groups that fill the GPU
 constexpr int kMost = 1024;   // rows from which on each has one
+// Rows of so few steps have one too: a launch and its workspace less.  One row of 32000 fp16 logits, called one by one, 14.8
+// us, split 18.3 (in a graph a split one is 2 us faster); of 5 and more steps both take as long.
+constexpr int kSolo = 4;
 
 // Work-groups of a row: as many as fill the GPU, none of less than a step.
 int parts_of(const kvq_token_logprobs_params& p) {
@@ -414,6 +442,7 @@ int parts_of(const kvq_token_logprobs_params& p) {
   int64_t parts = p.rows > 0 && p.rows < kMost ? (kFill + p.rows - 1) / p.rows : 1;
   const int64_t most = ((int64_t)p.vocab + step - 1) / step;
   if (parts > most) parts = most;
+  if (most <= kSolo) parts = 1;
   if (parts > kMaxParts) parts = kMaxParts;
   return (int)(parts < 1 ? 1 : parts);
 }

@@ -65,15 +65,20 @@ def token_logprobs(logits: Tensor, tokens: Optional[Tensor] = None, top: int = 0
             raise ValueError(f"tokens must be integers {tuple(shape)}, one for each row of logits, got {tokens.dtype} {tuple(tokens.shape)}")
         if tokens.dtype not in (torch.int32, torch.int64):
             tokens = tokens.to(torch.int64)
-        tokens = tokens.to(device).reshape(-1).contiguous()
+        if tokens.device != device:
+            tokens = tokens.to(device)
+        tokens = tokens.contiguous()
     _no_grad(logits)
-    x = logits.reshape(-1, vocab)
-    if vocab > 1 and x.stride(1) != 1:
+    x = logits if logits.ndim == 2 else logits.reshape(-1, vocab)
+    rows, (step, inner) = x.shape[0], x.stride()
+    if vocab > 1 and inner != 1:
         x = x.contiguous()
-    rows = x.shape[0]
-    logprobs = None if tokens is None else x.new_empty(shape, dtype=torch.float32)
-    entropy = x.new_empty(shape, dtype=torch.float32)
-    best = x.new_empty((*shape, top), dtype=torch.float32) if top else None
+        step = vocab
+    if tokens is None:
+        logprobs, entropy = None, x.new_empty(shape, dtype=torch.float32)
+    else:
+        logprobs, entropy = torch.empty_like(tokens, dtype=torch.float32), torch.empty_like(tokens, dtype=torch.float32)
+    best = entropy.new_empty((*shape, top)) if top else None
     ids = x.new_empty((*shape, top), dtype=torch.int64) if top else None
     out = TokenLogprobs(logprobs, entropy, best, ids)
     if rows == 0:
@@ -81,7 +86,7 @@ def token_logprobs(logits: Tensor, tokens: Optional[Tensor] = None, top: int = 0
     nbytes = _scratch(rows, vocab, top, _TYPES[x.dtype])
     scratch = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     _call(C.lib().kvq_token_logprobs, _LOGPROBS.pack(
-        x.data_ptr(), x.stride(0), 0 if tokens is None else tokens.data_ptr(), 0 if tokens is None else logprobs.data_ptr(),
+        x.data_ptr(), step, 0 if tokens is None else tokens.data_ptr(), 0 if tokens is None else logprobs.data_ptr(),
         entropy.data_ptr(), best.data_ptr() if top else 0, ids.data_ptr() if top else 0,
         0 if scratch is None else scratch.data_ptr(), nbytes, rows, vocab, top, _TYPES[x.dtype],
         tokens is not None and tokens.dtype == torch.int64, inverse, 0), device)

@@ -19,6 +19,7 @@ from typing import Optional, Sequence, Tuple, Union
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from . import _capi as C
 from .paged import _SM, _TYPES, HEAD_DIM, PAGE_SIZES, _cache_fields, _call, _i32, _no_grad, _packer, _rows16, _tau
@@ -60,6 +61,7 @@ class PagePools:
             self.written &= (self.num_pages < 2 or sp > 0) and (self.heads < 2 or sh > 0) and st > 0
             # the stride of a dimension of one is not used, whatever it is
             rows.append((t.data_ptr(), sp * item if self.num_pages > 1 else 0, sh * item if self.heads > 1 else 0, st * item, row, 0))
+        self._grad = any(t.requires_grad for t in self.tensors)
         self.layout = tuple((t.shape[3], t.dtype) for t in self.tensors)
         self._blocks = (C.PagePool * len(rows))(*rows)
         self._at = ctypes.addressof(self._blocks)
@@ -107,7 +109,8 @@ def copy_paged(pools: Union[PagePools, Sequence[Tensor]], src: Pages, dst: Pages
             raise ValueError("into must have the pools' device, heads, page size, row sizes and types")
     if not to.written:
         raise ValueError("pages that are written must have memory of their own, got a stride of 0")
-    _no_grad(*pools.tensors, *(() if to is pools else to.tensors))
+    if pools._grad or to._grad or forward_ad._current_level >= 0:
+        _no_grad(*pools.tensors, *to.tensors)
     device = pools.device
     if not isinstance(src, Tensor) and not isinstance(dst, Tensor):
         src, dst = list(src), list(dst)
