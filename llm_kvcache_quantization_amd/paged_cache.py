@@ -6,6 +6,8 @@ attention hook drives it through :class:`INT8CacheWrapperContainer` like any of 
 
 * pages: sequences of different lengths share one pool per layer, and memory follows what is held;
 * ``prefill_attn``: a prompt, or the next chunk of one, is appended and attended in one call;
+* ``fork``: sequences are repeated, reordered and ended, sharing the pages that they have in common; those that
+  continue one prompt attend its pages once for all of them (:func:`decode_attn_shared`); ``compact`` gives memory back;
 * a bound: ``window`` (sliding window, with ``sinks`` first tokens that stay visible; pages that
   nothing can see any more go back to the pool) or ``budget`` (eviction by accumulated attention
   weight, keeping ``sinks`` first and ``recent`` last tokens, once a sequence is ``slack`` tokens over).
@@ -16,17 +18,57 @@ src/cache/fp16_cache.py).
 from __future__ import annotations
 
 import math
-from typing import List, Optional, Sequence, Tuple
+from collections import Counter
+from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 from torch import Tensor
 
 from .cache import _EngineBase
 from .paged import HEAD_DIM, PAGE_SIZES, append_paged, decode_attn_paged, evict_paged, prefill_attn_window
+from .shared import PagePools, SharedPrefix, copy_paged, decode_attn_shared
+
+# Tokens x KV heads that sequences have to read less by sharing for that to be worth its second launch.  us a step in a graph, each
+# by itself / shared, 100 tokens of their own: 8 sequences of 28 / 4 heads over 2048 tokens (57 thousand) 11.4 / 11.4, 16 of 12 / 2 (61)
+# 11.2 / 12.2, 32 of 28 / 4 over 1024 (127) 14.9 / 13.8, 16 over 8192 (492) 32.6 / 18.1
+_MIN_SAVED = 1 << 16
+
+
+def _common(a: Sequence[int], b: Sequence[int]) -> int:
+    """Leading pages that two sequences have in common."""
+    lo, hi = 0, min(len(a), len(b))
+    while lo < hi:  # the first `lo` are alike, and more than `hi` are not
+        mid = (lo + hi + 1) // 2
+        if a[lo:mid] == b[lo:mid]:
+            lo = mid
+        else:
+            hi = mid - 1
+    return lo
+
+
+def shared_groups(rows: Sequence[List[int]]) -> Tuple[List[int], List[int]]:
+    """(sizes, pages) of groups of neighbouring sequences and the leading pages that each group's have in common: of the
+    groups that one least length of common pages gives, those that save the most pages."""
+    common = [_common(a, b) for a, b in zip(rows, rows[1:])]
+    best, groups = 0, ([1] * len(rows), [0] * len(rows))
+    for least in sorted(set(common) - {0}):
+        sizes, pages = [1], [0]
+        for n in common:
+            if n >= least:
+                pages[-1] = n if sizes[-1] == 1 else min(pages[-1], n)
+                sizes[-1] += 1
+            else:
+                sizes.append(1)
+                pages.append(0)
+        saved = sum((s - 1) * p for s, p in zip(sizes, pages))
+        if saved > best:
+            best, groups = saved, (sizes, pages)
+    return groups
 
 
 class PagedKVCache(_EngineBase):
-    """A paged cache of fp16, bf16 or INT8 pages (``dtype``; INT8 with fp16 scales per (token, ``group_size``)).
+    """A paged cache of fp16, bf16 or INT8 pages (``dtype``; INT8 with fp16 scales per (token, ``group_size``)).  ``fork``
+    repeats, reorders and ends its sequences.
 
     ``num_pages`` fixes the pool (``RuntimeError`` when it is used up); without it the pool grows by doubling.
     ``max_seq_len`` bounds the tokens that a sequence holds (those of pages given back no longer count).  Layers share the
@@ -80,10 +122,14 @@ class PagedKVCache(_EngineBase):
         self._weights: List[Optional[Tensor]] = [None] * n
         self._batch = self._heads = 0
         self._total = 0                                        # pages of a pool
+        self._handle: Optional[PagePools] = None               # the pools of all layers, for copies
         self._forget()
 
     def _forget(self) -> None:
         n = self.num_layers
+        self._refs: Dict[int, int] = {}                        # sequences that a page serves, where more than one
+        self._groups: Optional[tuple] = None                   # (sizes, shared tokens), as long as no page changes hands
+        self._prefixes: Dict[int, SharedPrefix] = {}           # the same as the attention takes it, by query heads
         self._held: List[List[int]] = [[] for _ in range(n)]   # tokens held of each sequence, per layer
         self._seen: List[List[int]] = [[] for _ in range(n)]   # tokens appended to each sequence, per layer
         self._rows: List[List[int]] = [[] for _ in range(self._batch)]  # pages of each sequence, -1: given back
@@ -129,6 +175,16 @@ class PagedKVCache(_EngineBase):
             t = self._lens[key] = torch.tensor(values, dtype=torch.int32, device=device)
         return t
 
+    def _drop_page(self, page: int) -> None:
+        """One sequence no longer needs a page."""
+        left = self._refs.get(page, 1) - 1
+        if left > 1:
+            self._refs[page] = left
+        elif left == 1:
+            del self._refs[page]
+        else:
+            self._free.append(page)
+
     def _give_back(self, counts: Optional[List[int]] = None) -> None:
         """Returns pages that no layer in use needs: behind the longest held length, or out of the window's sight, that of
         the next token where a sequence takes one (`counts`; None: all do), else of its last.  (A layer that begins later
@@ -145,7 +201,7 @@ class PagedKVCache(_EngineBase):
                 page = row.pop()
                 changed = True
                 if page >= 0:
-                    self._free.append(page)
+                    self._drop_page(page)
         if self.window is not None:
             keep = -(-self.sinks // ps)
             for b, (row, lo) in enumerate(zip(self._rows, least)):
@@ -153,7 +209,7 @@ class PagedKVCache(_EngineBase):
                 end = max(lo + (1 if counts is None or counts[b] else 0) - self.window, 0) // ps
                 for i in range(max(self._gone.get(b, 0), keep), end):
                     if row[i] >= 0:
-                        self._free.append(row[i])
+                        self._drop_page(row[i])
                         row[i] = -1
                         changed = True
                 if end > max(self._gone.get(b, 0), keep):
@@ -175,6 +231,35 @@ class PagedKVCache(_EngineBase):
             out += [(b, i) for i in range(len(row), -(-t // ps))]
         return out
 
+    def _copies(self, held: List[int], target: List[int]) -> List[Tuple[int, int]]:
+        """(sequence, place) of pages that tokens held .. target - 1 are written to, or that an eviction may write to, and that
+        serve other sequences too: all of these but one, whoever comes last, get a copy of their own."""
+        if not self._refs:
+            return []
+        ps, left, out = self.page_size, dict(self._refs), []
+        for b, (row, h, t) in enumerate(zip(self._rows, held, target)):
+            places = range(len(row)) if self.budget is not None else range(h // ps, min(len(row), -(-t // ps))) if t > h else ()
+            for i in places:
+                if left.get(row[i], 1) > 1:
+                    left[row[i]] -= 1
+                    out.append((b, i))
+        return out
+
+    def _copy(self, places: List[Tuple[int, int]], device) -> None:
+        """Copies pages of places that are about to be written, of all layers, and puts the copies there."""
+        new = self._free[len(self._free) - len(places) :]
+        most = [max(x) for x in zip(*[h for h in self._held if h])]  # slots that any layer holds
+        lens = [min(self.page_size, max(most[b] - i * self.page_size, 0)) for b, i in places]
+        if self._handle is None:
+            self._handle = PagePools([x for pool in self._pools if pool is not None for x in pool if x is not None])
+        t = torch.tensor([[self._rows[b][i] for b, i in places], new, lens], dtype=torch.int32, device=device)
+        copy_paged(self._handle, t[0], t[1], t[2])
+        del self._free[len(self._free) - len(places) :]
+        for (b, i), page in zip(places, new):
+            self._drop_page(self._rows[b][i])
+            self._rows[b][i] = page
+        self._table = self._groups = None
+
     def _reserve(self, layer_id: int, counts: List[int], device) -> None:
         """Pages for `counts` more tokens of each sequence."""
         held = self._held[layer_id] or [0] * self._batch
@@ -184,15 +269,17 @@ class PagedKVCache(_EngineBase):
             most = max((t - max(lost.get(b, 0) - keep, 0) * self.page_size for b, t in enumerate(target)), default=0)
             if most > self.max_seq_len:
                 raise ValueError(f"target_len {most} exceeds max_seq_len {self.max_seq_len} for layer {layer_id}")
-        need = self._needs(held, target)
-        if len(need) > len(self._free):
+        need, copies = self._needs(held, target), self._copies(held, target)
+        if len(need) + len(copies) > len(self._free):
             self._give_back(counts)  # short of pages: all that the new tokens do not see
-            need = self._needs(held, target)
-        short = len(need) - len(self._free)
+            need, copies = self._needs(held, target), self._copies(held, target)
+        short = len(need) + len(copies) - len(self._free)
         if short > 0:
             if self.num_pages is not None:
-                raise RuntimeError(f"out of pages: {len(need)} needed, {len(self._free)} of {self.num_pages} free")
+                raise RuntimeError(f"out of pages: {len(need) + len(copies)} needed, {len(self._free)} of {self.num_pages} free")
             self._grow(self._total + max(short, self._total))
+        if copies:
+            self._copy(copies, device)
         for b, i in need:
             row = self._rows[b]
             if i == len(row):
@@ -210,6 +297,7 @@ class PagedKVCache(_EngineBase):
                                        for x in pool)
         self._free = list(range(total - 1, self._total - 1, -1)) + self._free
         self._total = total
+        self._handle = None
 
     def _pool(self, layer_id: int, device) -> tuple:
         pool = self._pools[layer_id]
@@ -219,6 +307,7 @@ class PagedKVCache(_EngineBase):
             scales = [torch.empty((*shape, HEAD_DIM // self.group_size), dtype=torch.float16, device=device)
                       if self.dtype == torch.int8 else None for _ in range(2)]
             pool = self._pools[layer_id] = (*rows, *scales)
+            self._handle = None
         return pool
 
     def _block_table(self, device) -> Tensor:
@@ -341,6 +430,78 @@ class PagedKVCache(_EngineBase):
         kp, vp, ks, vs = self._pools[layer_id]
         return dense(kp, ks), dense(vp, vs)
 
+    # ---------------------------------------------------------------- sequences
+
+    def fork(self, parents: Sequence[int]) -> None:
+        """The batch becomes ``len(parents)`` sequences, the i-th of which goes on where sequence ``parents[i]`` stood: named
+        once it is kept, several times forked, not at all ended, in any order.
+
+        Sequences of one parent share its pages until they write to them: full pages stay shared, and of the last one
+        all but one get a copy when the next token comes.  With a ``budget`` they get copies of all pages then, since
+        an eviction moves tokens within them.  Attention over neighbours that share pages reads these once."""
+        parents = [int(p) for p in parents]
+        if not parents or any(not 0 <= p < self._batch for p in parents):
+            raise ValueError(f"parents must name at least one of the {self._batch} sequences held, got {parents}")
+        weights = [None if w is None else w[torch.tensor(parents, device=w.device)] for w in self._weights]
+        times = Counter(parents)
+        for p, row in enumerate(self._rows):
+            more = times.get(p, 0) - 1
+            for page in row if more else ():
+                if page >= 0:
+                    n = self._refs.pop(page, 1) + more
+                    if n > 1:
+                        self._refs[page] = n
+                    elif n == 0:
+                        self._free.append(page)
+        rows = [list(self._rows[p]) for p in parents]
+        self._rows, self._weights, self._batch = rows, weights, len(parents)
+        for lists in (self._held, self._seen):
+            for layer, counts in enumerate(lists):
+                if counts:
+                    lists[layer] = [counts[p] for p in parents]
+        for layer, counts in enumerate(self._seen):
+            self._layer_seq_lens[layer] = max(counts, default=0)
+        self._seq_len = max(self._layer_seq_lens)
+        self._gone, self._holes, *self._lost = ({i: d[p] for i, p in enumerate(parents) if p in d}
+                                                for d in (self._gone, self._holes, *self._lost))
+        self._table = self._groups = None
+        self._lens = {}
+
+    def compact(self) -> None:
+        """Moves what is held into pools of no more pages than that takes, and frees the others' memory.  A cache of a fixed
+        ``num_pages`` keeps its pools."""
+        used = list(dict.fromkeys(page for row in self._rows for page in row if page >= 0))
+        if self.num_pages is not None or len(used) == self._total:
+            return
+        if not used:
+            self._pools, self._free, self._total, self._handle = [None] * self.num_layers, [], 0, None
+            return
+        old = [x for pool in self._pools if pool is not None for x in pool if x is not None]
+        pools = [None if pool is None else tuple(None if x is None else x.new_empty((len(used), *x.shape[1:])) for x in pool)
+                 for pool in self._pools]
+        handle = PagePools([x for pool in pools if pool is not None for x in pool if x is not None])
+        copy_paged(old, used, range(len(used)), into=handle)
+        place = {page: i for i, page in enumerate(used)}
+        self._pools, self._handle, self._total, self._free = pools, handle, len(used), []
+        self._rows = [[place.get(page, -1) for page in row] for row in self._rows]
+        self._refs = {place[page]: n for page, n in self._refs.items()}
+        self._table = None
+
+    def _prefix(self, q_heads: int, device) -> Optional[SharedPrefix]:
+        """How the sequences share their first tokens, where that is worth an attention of its own."""
+        if not self._refs or self.window is not None or self.budget is not None:
+            return None
+        if self._groups is None:
+            full = [min(n) // self.page_size for n in zip(*[h for h in self._held if h])]  # pages that no layer writes any more
+            sizes, pages = shared_groups([row[:n] for row, n in zip(self._rows, full)])
+            self._groups, self._prefixes = (sizes, [n * self.page_size for n in pages]), {}
+        if sum((s - 1) * n for s, n in zip(*self._groups)) * self._heads < _MIN_SAVED:
+            return None
+        prefix = self._prefixes.get(q_heads)
+        if prefix is None:
+            prefix = self._prefixes[q_heads] = SharedPrefix(*self._groups, q_heads, self._heads, device)
+        return prefix
+
     # ---------------------------------------------------------------- attention
 
     def _attend_one(self, layer_id: int, q: Tensor, sm_scale: Optional[float], tau: Optional[Tensor],
@@ -348,6 +509,9 @@ class PagedKVCache(_EngineBase):
         kp, vp, ks, vs, table, lens = self._tensors(layer_id)
         if held is not None:
             lens = self._device_ints(held, q.device)
+        prefix = self._prefix(q.shape[1], q.device)
+        if prefix is not None:
+            return decode_attn_shared(q, kp, vp, table, lens, prefix, sm_scale, k_scale=ks, v_scale=vs, inv_tau=tau)
         return decode_attn_paged(q, kp, vp, table, lens, sm_scale, k_scale=ks, v_scale=vs, inv_tau=tau, window=self.window,
                                  sinks=self.sinks, weights=weights)
 
