@@ -42,7 +42,7 @@ from .patch import (  # noqa: F401
     apply_int8_fused_patch,
     remove_int8_fused_patch,
 )
-from .modes import create_kv_cache, generate_from_ids, load_calibration  # noqa: F401
+from .modes import create_kv_cache, generate_from_ids, load_calibration, sample_from_ids  # noqa: F401
 
 __all__ = [
     "DecodePlan",
@@ -82,5 +82,6 @@ __all__ = [
     "remove_int8_fused_patch",
     "create_kv_cache",
     "generate_from_ids",
+    "sample_from_ids",
     "load_calibration",
 ]

@@ -15,6 +15,9 @@
   decode, timed per step with a device synchronisation as the reference's CUDATimer does.
   The fused modes decode through the attention hook (:mod:`patch`); fp16 decodes through
   the model's own cache; the baseline modes hand the dequantized cache to the model.
+* :func:`sample_from_ids` -- several sampled continuations of each prompt over a paged cache: the prompt is
+  run once, its pages are shared (``PagedKVCache.fork``), sequences that have ended leave the batch, and every
+  token comes with its log probability.  No counterpart in the reference, which is greedy with one answer a prompt.
 
 The KIVI-family and mixed modes (``kivi_style``, ``int4_kivi_aligned``, ``int4_ours_asym*``,
 ``int4_mixed_kv``): the reference decodes them by dequantizing before attention (it forces
@@ -35,6 +38,8 @@ import torch
 
 from .cache import (FP16KVCache, INT4KVCache, INT8KVCache, KIVIStyleKVCache, MixedKVCache,
                     RoleAwareAllocatorKVCache, RoleAwareAsymKVCache, load_per_layer_bits_from_policy)
+from .paged_cache import PagedKVCache
+from .scoring import MAX_TOP, token_logprobs
 
 # src/engine/generate_loop.py:44-46
 _FUSED_KV_MODES = frozenset({"int8_fused", "int8_ours", "int4_fused", "int4_ours", "int4_ours_mixed"})
@@ -292,6 +297,25 @@ class GenerationBatchOutput:
     decode_attn_impl: str = "triton_fused"
     kv_cache_mem_mb: float = 0.0
     decode_stats: Optional[dict] = None
+    # with top_logprobs, of every generated token [B, T]: its log probability, the entropy it was chosen at, and the likeliest
+    # tokens with theirs [B, T, top_logprobs]
+    logprobs: Optional[torch.Tensor] = None
+    entropy: Optional[torch.Tensor] = None
+    top_logprobs: Optional[torch.Tensor] = None
+    top_tokens: Optional[torch.Tensor] = None
+
+
+@dataclass
+class SampleBatchOutput:
+    """What sample_from_ids returns.  Row b * num_samples + i is sample i of prompt b; behind a row's last token (its eos, if it
+    has one) generated_ids repeat the eos and the rest is 0."""
+    generated_ids: torch.Tensor               # [B * num_samples, T]
+    lengths: List[int]                        # tokens of each row, the eos among them
+    logprobs: torch.Tensor                    # [B * num_samples, T], at the temperature that drew them
+    entropy: torch.Tensor
+    top_logprobs: Optional[torch.Tensor] = None  # [B * num_samples, T, top_logprobs]
+    top_tokens: Optional[torch.Tensor] = None
+    kv_cache_mem_mb: float = 0.0
 
 
 def _past_layers(pkv):
@@ -400,16 +424,19 @@ def generate_from_ids(model, tokenizer, input_ids: torch.Tensor, attention_mask=
                       stop_on_eos: bool = True, quant_bits: Optional[int] = None, residual_length: int = 0,
                       check_numerics: bool = True, k_bits: Optional[int] = None, v_bits: Optional[int] = None,
                       policy_json: Optional[str] = None,
-                      project_root: Optional[str] = None) -> GenerationBatchOutput:
+                      project_root: Optional[str] = None, top_logprobs: Optional[int] = None) -> GenerationBatchOutput:
     """Greedy generation with explicit prefill + token-by-token decode
     (src/engine/generate_loop.py:393-1581, the modes of ``KV_MODES``).  Batches need
-    uniform lengths (an all-ones attention mask), as in the reference."""
+    uniform lengths (an all-ones attention mask), as in the reference.  ``top_logprobs`` (0 to 32; not in the reference): the
+    output carries the tokens' log probabilities and that many alternatives (outside the timed steps)."""
     from .patch import INT8CacheWrapperContainer, apply_int8_fused_patch, remove_int8_fused_patch
 
     check_kv_mode(kv_mode)
     if decode_attn_impl not in DECODE_ATTN_IMPLS:
         raise ValueError(f"decode_attn_impl={decode_attn_impl!r} not supported. Choose from "
                          f"{sorted(DECODE_ATTN_IMPLS)}.")
+    if top_logprobs is not None and not 0 <= top_logprobs <= MAX_TOP:
+        raise ValueError(f"top_logprobs must be None or 0 to {MAX_TOP}, got {top_logprobs}")
     if kv_mode == "int4_ours_asym_alloc" and policy_json is None:
         raise ValueError("kv_mode='int4_ours_asym_alloc' requires a non-empty policy_json")
     if not torch.cuda.is_available():
@@ -524,6 +551,7 @@ def generate_from_ids(model, tokenizer, input_ids: torch.Tensor, attention_mask=
                 h.remove()
             hooks = []
         steps = [nxt]
+        scores = [] if top_logprobs is None else [token_logprobs(out.logits[:, -1, :].detach(), nxt, top_logprobs)]
         times: List[float] = []
         eos = getattr(tokenizer, "eos_token_id", None) if tokenizer is not None else None
         if isinstance(eos, (list, tuple)):
@@ -557,6 +585,8 @@ def generate_from_ids(model, tokenizer, input_ids: torch.Tensor, attention_mask=
                     done = done | (nxt == eos)
             _sync()
             times.append((time.perf_counter() - t0) * 1e3)
+            if top_logprobs is not None:
+                scores.append(token_logprobs(out.logits[:, -1, :].detach(), nxt, top_logprobs))
             steps.append(nxt)
             cur = nxt.view(B, 1)
         gen = torch.stack(steps, dim=1) if steps else torch.empty(B, 0, dtype=torch.long, device=dev)
@@ -565,10 +595,103 @@ def generate_from_ids(model, tokenizer, input_ids: torch.Tensor, attention_mask=
         return GenerationBatchOutput(
             generated_ids=gen, ttft_ms=ttft_ms, tpot_ms=(sum(times) / len(times)) if times else 0.0,
             decode_times_ms=times, kv_mode=kv_mode, decode_attn_impl=decode_attn_impl,
-            kv_cache_mem_mb=mem, decode_stats=stats)
+            kv_cache_mem_mb=mem, decode_stats=stats,
+            **{name: torch.stack(x, dim=1) for name, x in _columns(scores).items()})
     finally:
         for h in hooks:
             h.remove()
         if patched:
             remove_int8_fused_patch(model)
         kv_cache.clear()
+
+
+def _columns(scores) -> dict:
+    """The steps' TokenLogprobs as lists by name; what they do not have is left out."""
+    if not scores:
+        return {}
+    return {name: [getattr(s, name) for s in scores] for name in scores[0]._fields if getattr(scores[0], name) is not None}
+
+
+def sample_from_ids(model, tokenizer, input_ids: torch.Tensor, num_samples: int = 1, max_new_tokens: int = 128,
+                    temperature: float = 1.0, seed: int = 1234, top_logprobs: int = 0,
+                    kv_dtype: Optional[torch.dtype] = None, group_size: int = 32, page_size: int = 64,
+                    num_pages: Optional[int] = None, inv_tau: Optional[torch.Tensor] = None,
+                    stop_on_eos: bool = True) -> SampleBatchOutput:
+    """``num_samples`` continuations of each of the prompts input_ids [B, S] (of one length), drawn at ``temperature`` (0: the
+    likeliest token, in all samples alike), over a :class:`PagedKVCache` of ``kv_dtype`` pages (default: the model's type; torch.int8 with
+    scales per ``group_size``).  The prompts run once; their samples share the pages and attend them together.  A sample
+    ends with its eos and leaves the batch."""
+    from .patch import INT8CacheWrapperContainer, apply_int8_fused_patch, remove_int8_fused_patch
+
+    if num_samples < 1 or max_new_tokens < 1:
+        raise ValueError(f"num_samples and max_new_tokens must be positive, got {num_samples} and {max_new_tokens}")
+    if not 0 <= temperature < float("inf"):
+        raise ValueError(f"temperature must be >= 0 and finite, got {temperature}")
+    if not 0 <= top_logprobs <= MAX_TOP:
+        raise ValueError(f"top_logprobs must be 0 to {MAX_TOP}, got {top_logprobs}")
+    if not isinstance(input_ids, torch.Tensor):
+        raise TypeError(f"input_ids must be a torch.Tensor, got {type(input_ids)}")
+    if input_ids.ndim != 2 or 0 in input_ids.shape:
+        raise ValueError(f"input_ids must be non-empty [B, S], got {tuple(input_ids.shape)}")
+    if not torch.cuda.is_available():
+        raise RuntimeError("CUDA is required for generation. Please run on a GPU-enabled server.")
+    dev = model.device
+    input_ids = input_ids.to(device=dev, dtype=torch.long)
+    batch, prompt = input_ids.shape
+    longest = getattr(model.config, "max_position_embeddings", None)
+    if longest is not None and prompt + max_new_tokens > int(longest):
+        raise ValueError(f"prompt_len + max_new_tokens = {prompt + max_new_tokens} exceeds the model's "
+                         f"max_position_embeddings={longest}")
+    eos = getattr(tokenizer, "eos_token_id", None) if tokenizer is not None and stop_on_eos else None
+    if isinstance(eos, (list, tuple)):
+        eos = eos[0] if eos else None
+    layers = int(getattr(model.config, "num_hidden_layers", 28))
+    cache = PagedKVCache(layers, device=str(dev), dtype=model.dtype if kv_dtype is None else kv_dtype, page_size=page_size,
+                         num_pages=num_pages, group_size=group_size, max_seq_len=prompt + max_new_tokens, inv_tau=inv_tau)
+    past = INT8CacheWrapperContainer(cache, layers)
+    rows = batch * num_samples
+    ids = torch.full((rows, max_new_tokens), 0 if eos is None else int(eos), dtype=torch.long, device=dev)
+    kept = {"logprobs": ids.new_zeros(ids.shape, dtype=torch.float32), "entropy": ids.new_zeros(ids.shape, dtype=torch.float32)}
+    if top_logprobs:
+        kept["top_logprobs"] = ids.new_zeros((*ids.shape, top_logprobs), dtype=torch.float32)
+        kept["top_tokens"] = ids.new_zeros((*ids.shape, top_logprobs))
+    lengths = [max_new_tokens] * rows
+    generator = torch.Generator(device=dev).manual_seed(seed)
+    apply_int8_fused_patch(model)
+    try:
+        with torch.no_grad():
+            logits = model(input_ids=input_ids, past_key_values=past, use_cache=True).logits[:, -1]
+            if num_samples > 1:
+                logits = logits.repeat_interleave(num_samples, dim=0)
+                cache.fork([b for b in range(batch) for _ in range(num_samples)])
+            alive, where = list(range(rows)), slice(None)  # rows of the batch, and the same as an index
+            for t in range(max_new_tokens):
+                if temperature > 0:
+                    p = torch.softmax(logits.float() / temperature, dim=-1)
+                    token = torch.multinomial(p, 1, generator=generator).squeeze(1)
+                else:
+                    token = logits.argmax(dim=-1)
+                ids[where, t] = token
+                scores = token_logprobs(logits, token, top_logprobs, temperature=temperature if temperature > 0 else 1.0)
+                for name, x in kept.items():
+                    x[where, t] = getattr(scores, name)
+                if t + 1 == max_new_tokens:
+                    break
+                if eos is not None:
+                    going = [i for i, over in enumerate((token == eos).tolist()) if not over]
+                    if len(going) < len(alive):
+                        for i in set(range(len(alive))) - set(going):
+                            lengths[alive[i]] = t + 1
+                        if not going:
+                            break
+                        cache.fork(going)
+                        alive = [alive[i] for i in going]
+                        token = token[torch.tensor(going, device=dev)]
+                        where = torch.tensor(alive, device=dev)
+                logits = model(input_ids=token.view(-1, 1), past_key_values=past, use_cache=True).logits[:, -1]
+        used = max(lengths)
+        return SampleBatchOutput(ids[:, :used], lengths, kv_cache_mem_mb=cache.get_memory_mb(),
+                                 **{name: x[:, :used] for name, x in kept.items()})
+    finally:
+        remove_int8_fused_patch(model)
+        cache.release()
