@@ -298,10 +298,14 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
       }
     }
     if (mx > f.m) f.to(mx, a.c);
+    // a step's sums by themselves, a vector's apart: short chains, in time and in rounding
+    Sums g[2] = {{f.m, 0.f, 0.f}, {f.m, 0.f, 0.f}};
 #pragma unroll
     for (int u = 0; u < kVec; ++u)
 #pragma unroll
-      for (int e = 0; e < E; ++e) f.add_logit(x[u][e], a.c);
+      for (int e = 0; e < E; ++e) g[u & 1].add_logit(x[u][e], a.c);
+    f.l += g[0].l + g[1].l;
+    f.s += g[0].s + g[1].s;
     most = fmaxf(most, mx);
   };
   {
