@@ -26,7 +26,7 @@ from torch import Tensor
 
 from .cache import _EngineBase
 from .paged import HEAD_DIM, PAGE_SIZES, append_paged, decode_attn_paged, evict_paged, prefill_attn_window
-from .shared import PagePools, SharedPrefix, copy_paged, decode_attn_shared
+from .shared import MAX_ROWS, PagePools, SharedPrefix, copy_paged, decode_attn_shared
 
 # Tokens x KV heads that sequences have to read less by sharing for that to be worth its second launch.  us a step in a graph, each
 # by itself / shared, 100 tokens of their own: 8 sequences of 28 / 4 heads over 2048 tokens (57 thousand) 11.4 / 11.4, 16 of 12 / 2 (61)
@@ -438,7 +438,8 @@ class PagedKVCache(_EngineBase):
 
         Sequences of one parent share its pages until they write to them: full pages stay shared, and of the last one
         all but one get a copy when the next token comes.  With a ``budget`` they get copies of all pages then, since
-        an eviction moves tokens within them.  Attention over neighbours that share pages reads these once."""
+        an eviction moves tokens within them.  Attention over neighbours that share pages reads these once.
+        (``clear`` keeps the last fork's batch size, ``release`` none.)"""
         parents = [int(p) for p in parents]
         if not parents or any(not 0 <= p < self._batch for p in parents):
             raise ValueError(f"parents must name at least one of the {self._batch} sequences held, got {parents}")
@@ -489,7 +490,7 @@ class PagedKVCache(_EngineBase):
 
     def _prefix(self, q_heads: int, device) -> Optional[SharedPrefix]:
         """How the sequences share their first tokens, where that is worth an attention of its own."""
-        if not self._refs or self.window is not None or self.budget is not None:
+        if not self._refs or self.window is not None or self.budget is not None or self._batch > MAX_ROWS:
             return None
         if self._groups is None:
             full = [min(n) // self.page_size for n in zip(*[h for h in self._held if h])]  # pages that no layer writes any more

@@ -24,6 +24,8 @@ from torch.autograd import forward_ad
 from . import _capi as C
 from .paged import _SM, _TYPES, HEAD_DIM, PAGE_SIZES, _cache_fields, _call, _i32, _no_grad, _packer, _rows16, _tau
 
+MAX_ROWS = 4096  # of a call of decode_attn_shared
+
 _COPY, _SHARED = _packer(C.CopyPagesParams), _packer(C.SharedDecodeParams)
 
 
@@ -173,7 +175,7 @@ def decode_attn_shared(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_table:
     with n = ``context_lens[b]`` (the new token included), out = softmax_t(sm_scale * inv_tau[h] * q . k_t) @ v_t over t < n,
     statistics and sums in fp32; token t < ``prefix.lens[g]`` lies in the pages of the group's first sequence, whatever
     b's own table says there.  Sequences that see nothing are zero.  fp16 / bf16 pages must have q's type; INT8 pages
-    serve both (V's values code * scale are used in fp16).  Hq / Hkv is at most 128, B at most 4096.
+    serve both (V's values code * scale are used in fp16).  Hq / Hkv is at most 128, B at most 4096, and a page stride below 2^32 bytes.
     """
     if q.ndim != 3 or q.shape[2] != HEAD_DIM:
         raise ValueError(f"q must be [B, Hq, {HEAD_DIM}], got {tuple(q.shape)}")

@@ -258,6 +258,17 @@ def test_attention_reads_a_shared_prefix_once(calls, monkeypatch):
     assert calls[-1][0] == "decode_attn_paged"  # 64 tokens of one head are too few
 
 
+@pytest.mark.parametrize("rows,name", [(4096, "decode_attn_shared"), (4097, "decode_attn_paged")])
+def test_more_rows_than_the_shared_attention_takes(calls, rows, name):
+    c = make(layers=1)
+    k = tensor(1, 1, 32, 128)
+    c.append(0, k, k)
+    c.fork([0] * rows)
+    k = tensor(rows, 1, 1, 128)
+    c.append_decode_attn(0, k[:, :, 0], k, k)
+    assert calls[-1][0] == name and c.get_seq_lens(0) == [33] * rows
+
+
 def test_refusals(calls):
     c = make()
     with pytest.raises(ValueError):
