@@ -625,8 +625,8 @@ def sample_from_ids(model, tokenizer, input_ids: torch.Tensor, num_samples: int 
 
     if num_samples < 1 or max_new_tokens < 1:
         raise ValueError(f"num_samples and max_new_tokens must be positive, got {num_samples} and {max_new_tokens}")
-    if not 0 <= temperature < float("inf"):
-        raise ValueError(f"temperature must be >= 0 and finite, got {temperature}")
+    if not (temperature == 0 or 1e-30 < temperature < 1e30):  # what token_logprobs takes
+        raise ValueError(f"temperature must be 0 or positive and finite, got {temperature}")
     if not 0 <= top_logprobs <= MAX_TOP:
         raise ValueError(f"top_logprobs must be 0 to {MAX_TOP}, got {top_logprobs}")
     if not isinstance(input_ids, torch.Tensor):
@@ -667,8 +667,10 @@ def sample_from_ids(model, tokenizer, input_ids: torch.Tensor, num_samples: int 
             alive, where = list(range(rows)), slice(None)  # rows of the batch, and the same as an index
             for t in range(max_new_tokens):
                 if temperature > 0:
+                    # the first of independent exponential arrivals at rates p; of logits that are NaN any token, where
+                    # multinomial's check would end the process
                     p = torch.softmax(logits.float() / temperature, dim=-1)
-                    token = torch.multinomial(p, 1, generator=generator).squeeze(1)
+                    token = (p / torch.empty_like(p).exponential_(generator=generator)).argmax(dim=-1)
                 else:
                     token = logits.argmax(dim=-1)
                 ids[where, t] = token

@@ -203,6 +203,39 @@ def test_samples_end_and_leave(monkeypatch):
     assert K.sample_from_ids(m, Tok(eos), ids, num_samples=6, max_new_tokens=12, seed=1, stop_on_eos=False).lengths == [12] * 6
 
 
+def test_samples_of_a_model_without_numbers():
+    """Logits that are NaN draw some token each, whose log probability is NaN."""
+    K = _k()
+    m = _tiny_lm(F16)
+    with torch.no_grad():
+        m.lm_head.weight.fill_(math.nan)
+    ids = torch.randint(0, 211, (1, 20), generator=torch.Generator().manual_seed(2)).to(DEV)
+    out = K.sample_from_ids(m, None, ids, num_samples=3, max_new_tokens=4)
+    assert ((out.generated_ids >= 0) & (out.generated_ids < 211)).all() and out.logprobs.isnan().all()
+
+
+@pytest.mark.parametrize("temperature", [1e-29, 0.05, 1.0, 1e29])
+def test_draws_follow_the_temperature(temperature):
+    """4096 samples of one token: cold ones are the likeliest, others as often as their probability says, within 6
+    deviations and 36 (Bernstein: one of 211 tokens beyond that by chance, below 1e-5)."""
+    K = _k()
+    m = _tiny_lm(F16)
+    with torch.no_grad():
+        m.lm_head.weight.div_(20.0)
+    ids = torch.randint(0, 211, (1, 20), generator=torch.Generator().manual_seed(2)).to(DEV)
+    n = 4096
+    out = K.sample_from_ids(m, None, ids, num_samples=n, max_new_tokens=1, temperature=temperature)
+    with torch.no_grad():
+        logits = m(input_ids=ids).logits[0, -1].double()
+    off = 2.0 ** -10 * 16  # by the attention's roundings (above), so that logits differ by twice that more or less
+    if temperature < 0.01:
+        assert (logits[out.generated_ids] >= logits.max() - 2 * off).all()
+        return
+    p = torch.softmax(logits / temperature, -1)
+    seen = torch.bincount(out.generated_ids[:, 0], minlength=211).double()
+    assert ((seen - n * p).abs() <= 6 * (n * p * (1 - p)).sqrt() + 36 + n * p * math.expm1(2 * off / temperature)).all()
+
+
 def test_greedy_samples_are_the_models_tokens():
     K = _k()
     m = _tiny_lm(F16)
@@ -225,6 +258,9 @@ def test_refusals():
                dict(top_logprobs=-1), dict(max_new_tokens=2000), dict(kv_dtype=torch.float32)):
         with pytest.raises(ValueError):
             K.sample_from_ids(m, None, ids, **kw)
+    for t in (1e-31, 1e-320, 1e31, math.nan):
+        with pytest.raises(ValueError):
+            K.sample_from_ids(m, None, ids, temperature=t)
     with pytest.raises(TypeError):
         K.sample_from_ids(m, None, [[1, 2]])
     with pytest.raises(ValueError):
