@@ -4,8 +4,10 @@
 //   l = sum e^((x - m) / T)
 //
 // One pass over the logits: each thread keeps a running maximum m and the two sums in fp32.  What bounds it: HBM, and the
-// vector units nearly as much (8 instructions a logit, one of them an exponential); few rows are split over
-// work-groups, whose parts a second launch joins.
+// vector units nearly as much (7 instructions a logit, one of them an exponential): 2047 rows of 152064 bf16 logits
+// 105 us, 5.9 TB/s (12 us more with one instruction a logit more, and the likeliest by counting).  Few rows are split over
+// work-groups, whose parts a second launch joins: 32 rows of 151936 with 20 of the likeliest 10 and 4.5 us, a chain of
+// latencies (one row of 32000, in one launch, 8).
 //
 // The likeliest: the pass leaves the maximum of every 32 logits that a lane takes (of 64 and more in long rows) in LDS.  The
 // top-th largest of 64 groups' maxima is a bar that at least `top` logits reach; only the 32s that reach it are read
@@ -63,10 +65,12 @@ struct Sums {
     l += o.l;
     s += o.s;
   }
-  __device__ __forceinline__ void add_logit(float x, float c) {  // at or below the maximum
+  // A logit at or below the maximum.  -Inf x 0 is no 0: where there may be such logits they are CLAMPed.
+  template <bool CLAMP>
+  __device__ __forceinline__ void add_logit(float x, float c) {
     const float d = x - shift_of(m), p = fast_exp2(d * c);
     l += p;
-    s = fmaf(fmaxf(d, kLowest), p, s);  // -Inf x 0 would be no 0
+    s = fmaf(CLAMP ? fmaxf(d, kLowest) : d, p, s);
   }
   __device__ __forceinline__ void lanes(float c) {
 #pragma unroll
@@ -86,6 +90,17 @@ __device__ __forceinline__ float logit_of(uint64_t key) {
 
 __device__ __forceinline__ uint64_t read_lane(uint64_t x, int lane) {
   return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), lane) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)x, lane);
+}
+
+// The k-th largest of a wave's 64 numbers, bit by bit: counting those above each takes a work-group 1 us more.
+__device__ __forceinline__ uint32_t kth_largest(uint32_t x, int k) {
+  uint32_t found = 0;
+#pragma unroll
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t t = found | 1u << bit;
+    if (__popcll(__ballot(x >= t)) >= k) found = t;
+  }
+  return found;
 }
 
 typedef __attribute__((address_space(3))) uint64_t lds_u64;
@@ -164,21 +179,15 @@ __device__ __forceinline__ void finish(const LpArgs& a, int64_t row, const Sums&
 }
 
 // Calls out(place, key) for the best `top` of n keys in LDS, place by place, by any thread of the work-group.  Many are
-// thinned out first, into `few` (room for n), by the top-th largest of 64 groups' largest: 380 keys, of 19 parts, counted as
-// they are take the join 13 us, so 4.
+// thinned out first, into `few` (room for n), by the logit of the top-th largest of 64 groups' largest: 380 keys, of 19
+// parts, counted as they are take the join 13 us, so 4.5; from 32, 64 or 128 keys on takes as long.
 template <class F>
 __device__ __forceinline__ void best_of(const lds_u64* key, int n, int top, lds_u64* few, int* count, F out) {
   if (n > 2 * 64) {
     const int lane = threadIdx.x & 63;
     uint64_t mine = 0;
     for (int i = lane; i < n; i += 64) mine = key[i] > mine ? key[i] : mine;
-    int above = 0;
-#pragma unroll 8
-    for (int i = 0; i < 64; ++i) {
-      const uint64_t y = read_lane(mine, i);
-      above += y > mine || (y == mine && i < lane);
-    }
-    const uint64_t bar = read_lane(mine, __builtin_ctzll(__ballot(above == top - 1)));
+    const uint64_t bar = (uint64_t)kth_largest((uint32_t)(mine >> 32), top) << 32;
     if (threadIdx.x == 0) *count = 0;
     __syncthreads();
     for (int i = threadIdx.x; i < n; i += kThreads)
@@ -299,13 +308,20 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
     }
     if (mx > f.m) f.to(mx, a.c);
     // a step's sums by themselves, a vector's apart: short chains, in time and in rounding
-    Sums g[2] = {{f.m, 0.f, 0.f}, {f.m, 0.f, 0.f}};
+    auto sum = [&](auto clamp) {
+      Sums g[2] = {{f.m, 0.f, 0.f}, {f.m, 0.f, 0.f}};
 #pragma unroll
-    for (int u = 0; u < kVec; ++u)
+      for (int u = 0; u < kVec; ++u)
 #pragma unroll
-      for (int e = 0; e < E; ++e) g[u & 1].add_logit(x[u][e], a.c);
-    f.l += g[0].l + g[1].l;
-    f.s += g[0].s + g[1].s;
+        for (int e = 0; e < E; ++e) g[u & 1].template add_logit<decltype(clamp)::value>(x[u][e], a.c);
+      return Sums{f.m, g[0].l + g[1].l, g[0].s + g[1].s};
+    };
+    // again where a logit was -Inf (or none was a number): the clamp costs one of eight instructions, 115 us for 109 at
+    // 2047 rows of 152064
+    Sums g = whole ? sum(std::false_type{}) : sum(std::true_type{});
+    if (whole && g.s != g.s) g = sum(std::true_type{});
+    f.l += g.l;
+    f.s += g.s;
     most = fmaxf(most, mx);
   };
   {
@@ -324,7 +340,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
     const bool there = lane < p.first + p.rest;
     const float x = there ? value_at<T>(p.x0 + (int64_t)p.edge(a, lane) * P::S) : kNegInf;
     if (x > f.m) f.to(x, a.c);
-    f.add_logit(x, a.c);
+    f.add_logit<true>(x, a.c);
   }
   f.lanes(a.c);
   if (lane == 0) sums[wave] = f;
@@ -342,13 +358,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
     float mine = group[lane];
 #pragma unroll
     for (int w = 1; w < kWaves; ++w) mine = fmaxf(mine, group[64 * w + lane]);
-    int above = 0;
-#pragma unroll 8
-    for (int i = 0; i < 64; ++i) {
-      const float y = row_lane(mine, i);
-      above += y > mine || (y == mine && i < lane);
-    }
-    const float bar = row_lane(mine, __builtin_ctzll(__ballot(above == a.top - 1)));
+    const float bar = logit_of((uint64_t)kth_largest(order_of(mine), a.top) << 32);
     for (int slot = 0; slot * per < steps; ++slot)
       if (maxima[slot][tid] >= bar) {
         const int i = atomicAdd(&n_blocks, 1);
