@@ -289,6 +289,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
 
   Sums f{kNegInf, 0.f, 0.f};
   float most = kNegInf, all = kNegInf;  // of the slot, of all
+  bool clamp = false;
   auto step = [&](int at, bool whole) {
     u32x4 w[kVec];
 #pragma unroll
@@ -316,10 +317,14 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LpArgs a) {
         for (int e = 0; e < E; ++e) g[u & 1].template add_logit<decltype(clamp)::value>(x[u][e], a.c);
       return Sums{f.m, g[0].l + g[1].l, g[0].s + g[1].s};
     };
-    // again where a logit was -Inf (or none was a number): the clamp costs one of eight instructions, 115 us for 109 at
-    // 2047 rows of 152064
-    Sums g = whole ? sum(std::false_type{}) : sum(std::true_type{});
-    if (whole && g.s != g.s) g = sum(std::true_type{});
+    // The clamp is one of eight instructions, 115 us for 109 at 2047 rows of 152064: a wave takes it from the first step on
+    // that has a -Inf (or no number).
+    Sums g;
+    if (whole && !clamp) {
+      g = sum(std::false_type{});
+      clamp = __any(g.s != g.s);
+    }
+    if (!whole || clamp) g = sum(std::true_type{});
     f.l += g.l;
     f.s += g.s;
     most = fmaxf(most, mx);
