@@ -449,8 +449,11 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(LpArgs a) {
 
 // ---------------------------------------------------------------- host
 
-constexpr int kFill = 2048;   // work-groups that fill the GPU
-constexpr int kMost = 1024;   // rows from which on each has one
+// Work-groups that fill the GPU, and rows from which on each has one.  Rows of 151936 bf16 logits with 5 of the likeliest, us in a
+// graph: 128 over 512, 1024 and 2048 work-groups 17.3, 18.0, 22.8; 256 24.4, 23.6, 27.2, one each 29.4; 400 34.8 over 2048, one
+// each 32.6; 768 51 and 44.
+constexpr int kFill = 512;
+constexpr int kMost = 384;
 // Rows of so few steps have one too: a launch and its workspace less.  One row of 32000 fp16 logits, called one by one, 14.8
 // us, split 18.3 (in a graph a split one is 2 us faster); of 5 and more steps both take as long.
 constexpr int kSolo = 4;
