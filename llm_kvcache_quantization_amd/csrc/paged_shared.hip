@@ -12,6 +12,13 @@
 // 64 tokens, in LDS, two buffers, as the prompts' attention does it.  A wave has 32 columns.  Up to 64 columns
 // two waves share them, each with half of a tile's tokens, and join at the end.
 //
+// What bounds it: with few tokens and columns a chain of latencies (plan, table, load, the tile's products and
+// exponentials one after another: 1.1 + 0.7 + 0.6 + 2.3 us before the first tile, 1.5 a tile of 128 columns), else HBM
+// with 16-bit pages (four prompts of up to 16384 tokens with 8 rows of 28 / 4 heads each, 94 MB: 22.8 us; 6.6 TB/s while the
+// tiles run, 4.1 with start and end), and with INT8 pages the vector and matrix units in turn (39% and 14% of busy cycles; one
+// prompt of 32768, 32 rows of 40 / 8 heads: 80 us, 270 TFLOP/s), two waves a SIMD being all that the registers allow.
+// The join: 3.3 to 6 us.
+//
 // Tokens that nobody sees (outside the run's range, pages that are not there) are loaded from a row of zeros, so
 // that a masked NaN reaches nobody; all columns of a work-group see the same tokens.  A row that is shorter than its
 // group's prefix takes no part in it: its tail begins at its first token, in the pages of the group's first row.
@@ -69,7 +76,8 @@ struct ShArgs {
   float* acc;            // [kv_heads][slots][128]
 };
 
-constexpr int kTailTiles = 3;  // least tiles of a tail's work-group
+// Least tiles of a tail's work-group: 16 rows with 700 tokens behind 8191 shared ones 18.8 us, with one tile 19.0, with six 21.7.
+constexpr int kTailTiles = 3;
 
 // The tiles of a row's own tokens lo .. hi - 1.
 struct Tail {
@@ -713,11 +721,16 @@ __global__ __launch_bounds__(kThreads) void shared_join_kernel(ShArgs a) {
 
 // ---------------------------------------------------------------- host
 
-constexpr int kTarget = 512;        // work-groups that fill the GPU: two a CU
-constexpr int kPrefixTarget = 384;  // those of them for the prefixes, and where that leaves each more than kLong tiles
+// Work-groups that fill the GPU, two a CU, and those of them for the prefixes; more of them where each has more than kLong
+// tiles, so that the tails matter less.  us in a graph: four prompts of up to 16384 with 8 rows each over 256, 384 and 512 28.9, 27.5,
+// 33.3 (then the tails have to wait); one of 32768 with 32 rows, INT8, over 384, 448 and 512 92.0, 84.1, 86.8.
+constexpr int kTarget = 512;
+constexpr int kPrefixTarget = 384;
 constexpr int kLongTarget = 448;
 constexpr int kLong = 12;
-constexpr int kMinTiles = 3;        // least tiles of a prefix's work-group
+// Least tiles of a prefix's work-group, between a long run and many parts to join: 16 rows over 8191 tokens with 1, 3 and 6
+// 21.3, 18.7, 22.3; two rows over 517 10.1, 10.1, 11.0.
+constexpr int kMinTiles = 3;
 constexpr int kMaxSplits = 256;
 
 int plan(const int32_t* sizes, const int32_t* lens, int32_t groups, int32_t q_heads, int32_t kv_heads, kvq_shared_plan_info* info,

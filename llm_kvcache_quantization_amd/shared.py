@@ -32,7 +32,8 @@ _COPY, _SHARED = _packer(C.CopyPagesParams), _packer(C.SharedDecodeParams)
 class PagePools:
     """Tensors of pages that are copied together: [num_pages, heads, page_size, X] alike but for X and type, such as
     K, V and their scales of every layer.  Rows (X elements, 2 to 1024 bytes, a power of two) are contiguous, and one behind
-    the other where they have less than 16 bytes; pages and heads begin at multiples of 16 bytes.  Holds the tensors."""
+    the other where they have less than 16 bytes; pages and heads begin at multiples of 16 bytes.  Holds the tensors; layout, and whether they require a
+    gradient, are looked at here, once."""
 
     def __init__(self, tensors: Sequence[Tensor]):
         self.tensors = tuple(tensors)
