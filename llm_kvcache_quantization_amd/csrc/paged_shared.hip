@@ -209,16 +209,18 @@ struct Direct {
   }
 };
 
-// A tile of INT8 pages as it is, straight into LDS: K's codes [64][128]; V's with the scales [64][G] of both sides.
+// A tile of INT8 pages as it is, straight into LDS: K's codes [64][128]; V's with the scales of both sides.
 typedef u32x4 KCodes[kBN * 8];
 template <int G>
 struct VCodes {
   u32x4 v[kBN * 8];
+  // dwords as they lie in the pages, [pair of groups][token]; of one group, [pair of tokens]
   uint32_t ks[G == 1 ? 64 : kBN * G / 2], vs[G == 1 ? 64 : kBN * G / 2];  // at least a wave's load
 };
 
 // A thread's places in a tile of INT8 pages.  A wave instruction loads eight rows of 8 pieces of 16 codes, and a dword of
-// scales a lane (half a token's, one or two tokens'); waves 0 and 1 take K's scales, 2 and 3 V's, twice where one has all.
+// scales a lane (a pair of a token's, or two tokens'); waves 0 and 1 take K's scales, 2 and 3 V's, a pair of groups each or
+// the same twice.
 template <int GS>
 struct Coded {
   static constexpr int G = 128 / GS;
@@ -231,8 +233,7 @@ struct Coded {
     const uint32_t piece = tid & 7;
     k_off = (uint32_t)(row & 15) * (uint32_t)c.kst + piece * 16;
     v_off = (uint32_t)(row & 15) * (uint32_t)c.vst + piece * 16;
-    const int i = (G == 4 ? tid & 64 : 0) + lane;
-    s_row = min(i * 2 / G, kBN - 1);
+    s_row = G == 1 ? min(2 * lane, kBN - 1) : lane;
     k_at = (uint32_t)row * 256 + ((2 * piece) ^ (uint32_t)(row & 15)) * 16;
     v_at = (uint32_t)row * 256 + ((2 * piece) ^ (uint32_t)((row & 3) << 2)) * 16;
   }
@@ -266,7 +267,7 @@ struct Coded {
     const uint8_t* const x = v ? s.vs : s.ks;
     const uint32_t page_stride = (uint32_t)(v ? c.vssp : c.kssp);
     uint32_t* const lds = (v ? to.vs : to.ks) + (G == 4 ? 64 * (wave & 1) : 0);
-    const uint32_t in_token = G == 4 ? 4 * (threadIdx.x & 1) : 0;
+    const uint32_t in_token = G == 4 ? 4 * (wave & 1) : 0;
     if (ok == 15 && c.lg >= 6) {  // a tile of one page
       const uint32_t at = (uint32_t)((key0 & c.page_mask) + s_row) * (2 * G) / 4 * 4 + in_token;
       __builtin_amdgcn_global_load_lds((gptr)(x + (uint64_t)(uint32_t)p[0] * page_stride + at), (__attribute__((address_space(3))) void*)lds, 4, 0, 0);
@@ -305,7 +306,8 @@ struct Coded {
     const bool all = s.whole(key0, ok);
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      uint32_t scale = ((const uint16_t*)from.vs)[(row + 32 * e) * G + (threadIdx.x & 7) * 16 / GS];
+      const int g = (threadIdx.x & 7) * 16 / GS, at_row = row + 32 * e;
+      uint32_t scale = ((const uint16_t*)from.vs)[G == 1 ? at_row : g / 2 * 128 + at_row * 2 + g % 2];
       if (!all) {
         const int at = row + 32 * e, key = key0 + at;
         if (!((ok >> (at >> 4) & 1) && key >= s.lo && key < s.hi)) scale = 0;
@@ -342,7 +344,7 @@ struct Shared : AttnTile<M> {
   // Scores of codes: of each group by itself, times the tokens' scales.  Two groups at a time, whose scales are read for them:
   // all four have no room.
   static __device__ __forceinline__ float16v code_scores(const u32x4 (&kf)[8], const u32x4 (&q)[8], const uint32_t* scales, int u) {
-    const uint16_t* const first = (const uint16_t*)scales + (32 * u + 4 * ((threadIdx.x & 63) >> 5)) * G;
+    const int first = 32 * u + 4 * ((threadIdx.x & 63) >> 5);
     float16v sc;
 #pragma unroll
     for (int j = 0; j < 16; ++j) sc[j] = 0.f;
@@ -350,12 +352,17 @@ struct Shared : AttnTile<M> {
 #pragma unroll
     for (int g0 = 0; g0 < G; g0 += N) {
       if (g0) __builtin_amdgcn_sched_barrier(0);
-      uint32_t w[16];  // token j's, of groups g0 and g0 + 1
+      uint32_t w[16];  // token j's, of groups g0 and g0 + 1; of one group, a pair of tokens' in every second
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const uint16_t* const x = first + (8 * (j >> 2) + (j & 3)) * G + g0;
-        if constexpr (G == 1) w[j] = *x;
-        else w[j] = *(const uint32_t*)x;
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (G == 1) {
+          const u32x2 x = *(const u32x2*)((const uint16_t*)scales + first + 8 * i);
+          w[4 * i] = x[0]; w[4 * i + 2] = x[1];
+        } else {
+          const u32x4 x = *(const u32x4*)(scales + g0 / 2 * 64 + first + 8 * i);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) w[4 * i + r] = x[r];
+        }
       }
 #pragma unroll
       for (int g = g0; g < g0 + N; ++g) {
@@ -365,7 +372,7 @@ struct Shared : AttnTile<M> {
 #pragma unroll
         for (int kk = 8 * g / G; kk < 8 * (g + 1) / G; ++kk) d = M::mfma32(kf[kk], q[kk], d);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) sc[j] = fmaf(d[j], half_of(w[j], g - g0), sc[j]);
+        for (int j = 0; j < 16; ++j) sc[j] = fmaf(d[j], G == 1 ? half_of(w[j & ~1], j & 1) : half_of(w[j], g - g0), sc[j]);
       }
     }
     return sc;
