@@ -730,7 +730,8 @@ __global__ __launch_bounds__(kThreads) void shared_join_kernel(ShArgs a) {
 
 // Work-groups that fill the GPU, two a CU, and those of them for the prefixes; more of them where each has more than kLong
 // tiles, so that the tails matter less.  us in a graph: four prompts of up to 16384 with 8 rows each over 256, 384 and 512 28.9, 27.5,
-// 33.3 (then the tails have to wait); one of 32768 with 32 rows, INT8, over 384, 448 and 512 92.0, 84.1, 86.8.
+// 33.3 (then the tails have to wait); one of 32768 with 32 rows, INT8, over 416, 448 and 480 with up to 509 tokens of their own
+// 74.7, 80.3, 81.3, with one 77.0, 73.5, 73.5.
 constexpr int kTarget = 512;
 constexpr int kPrefixTarget = 384;
 constexpr int kLongTarget = 448;
@@ -769,8 +770,10 @@ int plan(const int32_t* sizes, const int32_t* lens, int32_t groups, int32_t q_he
     if (splits > kMaxSplits) splits = kMaxSplits;
     for (int i = 0; i < sizes[g]; ++i)
       put(row + i, {(int32_t)row, lens[g], (int32_t)slots, (int32_t)splits, (int32_t)per, (int32_t)cols, 0, 0});
-    for (int64_t s = 0; s < splits; ++s)
-      for (int64_t c0 = 0; c0 < cols; c0 += per) {
+    // The runs of a block of columns one behind the other: the two work-groups of a CU are then of different blocks where
+    // these differ in columns (160 in 96 and 64, INT8, 32768 tokens: 73.5 us, alternating 81.4).
+    for (int64_t c0 = 0; c0 < cols; c0 += per)
+      for (int64_t s = 0; s < splits; ++s) {
         const int64_t width = cols - c0 < per ? cols - c0 : per;
         put(rows + units, {(int32_t)row, (int32_t)c0, (int32_t)width, (int32_t)(tiles * s / splits), (int32_t)(tiles * (s + 1) / splits),
                            lens[g], (int32_t)(slots + c0 * splits + s * width), 0});
