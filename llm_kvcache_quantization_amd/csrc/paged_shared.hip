@@ -820,10 +820,10 @@ Launch launch_of(const kvq_shared_decode_params& p) {
   const int64_t most = (tiles + kTailTiles - 1) / kTailTiles;  // of a row
   int64_t groups;  // work-groups of tails, a KV head
   if (B <= 64) {
-    int64_t fill = kTarget / H - p.plan.units;  // what the prefixes leave
-    if (fill < (kTarget - kPrefixTarget) / H) fill = (kTarget - kPrefixTarget) / H;
-    // Long tails in many pieces end together: 32 rows with up to 4000 tokens of their own behind 32768 shared INT8 ones 150 us with
-    // B, 129 with 2 B, 123 with 4 B; with up to 1500 104, 92, 97; short ones have no more pieces than tiles allow.
+    int64_t fill = 2 * kTarget / H;
+    // Long tails in many pieces end together: 32 rows of 40 / 8 heads with up to 4000 tokens of their own behind 32768 shared INT8
+    // ones over B, 2 B and 4 B 150, 129 and 123 us; 4 rows with 16000 over 4 B 141, so 79.  Short ones have no more pieces than
+    // kTailTiles allows.
     if (fill < 4 * B) fill = 4 * B;
     w.fill = (int)fill;
     groups = fill + B < B * most ? fill + B : B * most;

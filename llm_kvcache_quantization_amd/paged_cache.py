@@ -33,6 +33,12 @@ from .shared import MAX_ROWS, PagePools, SharedPrefix, copy_paged, decode_attn_s
 # 11.2 / 12.2, 32 of 28 / 4 over 1024 (127) 14.9 / 13.8, 16 over 8192 (492) 32.6 / 18.1
 _MIN_SAVED = 1 << 16
 
+# Tokens that the decode of each by itself has to read for one of the shared attention, whose tiles of a row's own tokens are
+# dearer, INT8 ones more.  The same, us: 16 sequences of 28 / 4 heads over 4096 tokens with 4000 and 16000 of their own (1.9, 1.2
+# times as many) 38 / 36, 97 / 107; INT8 (1.9) 29 / 45; over 32768 with 16000 (2.7) 129 / 125, with 4000 (7) 93 / 60; 64 of 40 / 8
+# over 4096 with 4000 (2.0) 182 / 204, over 32768 with 16000 (2.9) 950 / 701
+_DEARER = {torch.float16: 1.4, torch.bfloat16: 1.4, torch.int8: 2.6}
+
 
 def _common(a: Sequence[int], b: Sequence[int]) -> int:
     """Leading pages that two sequences have in common."""
@@ -488,7 +494,7 @@ class PagedKVCache(_EngineBase):
         self._refs = {place[page]: n for page, n in self._refs.items()}
         self._table = None
 
-    def _prefix(self, q_heads: int, device) -> Optional[SharedPrefix]:
+    def _prefix(self, layer_id: int, q_heads: int, device) -> Optional[SharedPrefix]:
         """How the sequences share their first tokens, where that is worth an attention of its own."""
         if not self._refs or self.window is not None or self.budget is not None or self._batch > MAX_ROWS:
             return None
@@ -496,7 +502,8 @@ class PagedKVCache(_EngineBase):
             full = [min(n) // self.page_size for n in zip(*[h for h in self._held if h])]  # pages that no layer writes any more
             sizes, pages = shared_groups([row[:n] for row, n in zip(self._rows, full)])
             self._groups, self._prefixes = (sizes, [n * self.page_size for n in pages]), {}
-        if sum((s - 1) * n for s, n in zip(*self._groups)) * self._heads < _MIN_SAVED:
+        saved, tokens = sum((s - 1) * n for s, n in zip(*self._groups)), sum(self._held[layer_id])
+        if saved * self._heads < _MIN_SAVED or tokens < _DEARER[self.dtype] * (tokens - saved):
             return None
         prefix = self._prefixes.get(q_heads)
         if prefix is None:
@@ -510,7 +517,7 @@ class PagedKVCache(_EngineBase):
         kp, vp, ks, vs, table, lens = self._tensors(layer_id)
         if held is not None:
             lens = self._device_ints(held, q.device)
-        prefix = self._prefix(q.shape[1], q.device)
+        prefix = self._prefix(layer_id, q.shape[1], q.device)
         if prefix is not None:
             return decode_attn_shared(q, kp, vp, table, lens, prefix, sm_scale, k_scale=ks, v_scale=vs, inv_tau=tau)
         return decode_attn_paged(q, kp, vp, table, lens, sm_scale, k_scale=ks, v_scale=vs, inv_tau=tau, window=self.window,

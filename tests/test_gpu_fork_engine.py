@@ -34,6 +34,7 @@ def test_forked_steps(dtype, pages, page, monkeypatch):
 
     print(f"[fork] {dtype} {pages} page {page}", flush=True)
     monkeypatch.setattr(M, "_MIN_SAVED", 1)
+    monkeypatch.setattr(M, "_DEARER", dict.fromkeys(M._DEARER, 1.0))
     shared = []
     real = M.decode_attn_shared
     monkeypatch.setattr(M, "decode_attn_shared", lambda *a, **kw: (shared.append(a[5]), real(*a, **kw))[1])
@@ -151,6 +152,7 @@ def test_samples_have_their_log_probabilities(dtype, kv, monkeypatch):
     import llm_kvcache_quantization_amd.paged_cache as M
 
     monkeypatch.setattr(M, "_MIN_SAVED", 1)
+    monkeypatch.setattr(M, "_DEARER", dict.fromkeys(M._DEARER, 1.0))
     used = []
     real = M.decode_attn_shared
     monkeypatch.setattr(M, "decode_attn_shared", lambda *a, **kw: (used.append(a[5]), real(*a, **kw))[1])

@@ -258,6 +258,26 @@ def test_attention_reads_a_shared_prefix_once(calls, monkeypatch):
     assert calls[-1][0] == "decode_attn_paged"  # 64 tokens of one head are too few
 
 
+@pytest.mark.parametrize("dtype,last", [(torch.float16, 104), (torch.bfloat16, 104), (torch.int8, 14)])
+def test_long_tails_are_read_by_themselves(calls, monkeypatch, dtype, last):
+    """Four sequences share 64 tokens: each by itself reads 4 (64 + n), the shared attention 64 + 4 n; `last` is the greatest n
+    at which the former is 1.4 times as much, or 2.6 times for INT8 pages."""
+    monkeypatch.setattr(M, "_MIN_SAVED", 1)
+    times = {torch.int8: 2.6}.get(dtype, 1.4)
+    assert 4 * (64 + last) >= times * (64 + 4 * last) and 4 * (65 + last) < times * (68 + 4 * last)
+    c = make(layers=1, dtype=dtype)
+    kv = torch.bfloat16 if dtype == torch.bfloat16 else torch.float16
+    k = tensor(1, 1, 64, 128).to(kv)
+    c.append(0, k, k)
+    c.fork([0] * 4)
+    k = tensor(4, 1, last - 1, 128).to(kv)
+    c.append(0, k, k)
+    k = tensor(4, 1, 1, 128).to(kv)
+    for name in ("decode_attn_shared", "decode_attn_paged"):
+        c.append_decode_attn(0, k[:, :, 0], k, k)
+        assert calls[-1][0] == name
+
+
 @pytest.mark.parametrize("rows,name", [(4096, "decode_attn_shared"), (4097, "decode_attn_paged")])
 def test_more_rows_than_the_shared_attention_takes(calls, rows, name):
     c = make(layers=1)
