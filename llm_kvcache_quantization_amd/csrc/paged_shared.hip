@@ -16,7 +16,8 @@
 // exponentials one after another: 1.1 + 0.7 + 0.6 + 2.3 us before the first tile, 1.5 a tile of 128 columns), else HBM
 // with 16-bit pages (four prompts of up to 16384 tokens with 8 rows of 28 / 4 heads each, 94 MB: 22.8 us; 6.6 TB/s while the
 // tiles run, 4.1 with start and end), and with INT8 pages the vector and matrix units in turn (39% and 14% of busy cycles; one
-// prompt of 32768, 32 rows of 40 / 8 heads: 80 us, 270 TFLOP/s), two waves a SIMD being all that the registers allow.
+// prompt of 32768, 32 rows of 40 / 8 heads with up to 509 tokens of their own: 78 us, 274 TFLOP/s; with one 70), two waves a SIMD
+// being all that the registers allow.
 // The join: 3.3 to 6 us.
 //
 // Tokens that nobody sees (outside the run's range, pages that are not there) are loaded from a row of zeros, so
