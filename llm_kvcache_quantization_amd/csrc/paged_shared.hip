@@ -16,8 +16,8 @@
 // exponentials one after another: 1.1 + 0.7 + 0.6 + 2.3 us before the first tile, 1.5 a tile of 128 columns), else HBM
 // with 16-bit pages (four prompts of up to 16384 tokens with 8 rows of 28 / 4 heads each, 94 MB: 22.8 us; 6.6 TB/s while the
 // tiles run, 4.1 with start and end), and with INT8 pages the vector and matrix units in turn (39% and 14% of busy cycles; one
-// prompt of 32768, 32 rows of 40 / 8 heads with up to 509 tokens of their own: 78 us, 274 TFLOP/s; with one 70), two waves a SIMD
-// being all that the registers allow.
+// prompt of 32768, 32 rows of 40 / 8 heads with up to 509 tokens of their own: 78 us, 274 TFLOP/s), two waves a SIMD being all
+// that the registers allow.
 // The join: 3.3 to 6 us.
 //
 // Tokens that nobody sees (outside the run's range, pages that are not there) are loaded from a row of zeros, so
@@ -92,8 +92,11 @@ struct Tail {
     first = lo / kBN;
     count = hi > lo ? (hi + kBN - 1) / kBN - first : 0;
   }
-  // of `chunks` even runs of tiles, the i-th's first
-  __device__ __forceinline__ int begin(int i, int chunks) const { return first + (int)((uint32_t)count * (uint32_t)i / (uint32_t)chunks); }
+  // of `chunks` even runs of tiles, the i-th's first: first + count i / chunks, whose product may pass 32 bits
+  __device__ __forceinline__ int begin(int i, int chunks) const {
+    const uint32_t n = (uint32_t)chunks, whole = (uint32_t)count / n, rest = (uint32_t)count % n;
+    return first + (int)(whole * (uint32_t)i + rest * (uint32_t)i / n);
+  }
 };
 
 // Which row a tail's work-group is of, and which of its chunks; and, of each row, what the join needs: {first

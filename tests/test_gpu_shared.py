@@ -130,6 +130,26 @@ def test_long_tails():
     run([2], [64], [30000, 64], 5, 1, 128, BF16, 32)
 
 
+@pytest.mark.parametrize("shared", [0, 1 << 29])
+def test_longest_rows(shared):
+    """2^30 tokens, all in one page: the products of tiles and work-groups pass 32 bits.  Every token of the page stands as
+    often, so that the attention is the page's."""
+    g = torch.Generator().manual_seed(4)
+    k, v = (torch.randn(1, 1, 256, D, generator=g).to(F16) for _ in range(2))
+    q = torch.randn(1, 4, D, generator=g).to(F16)
+    K = _k()
+    table = torch.zeros(1, 1 << 22, dtype=torch.int32, device=DEV)
+    out = K.decode_attn_shared(q.to(DEV), k.to(DEV), v.to(DEV), table, torch.tensor([1 << 30], dtype=torch.int32, device=DEV),
+                               K.SharedPrefix([1], [shared], 4, 1, DEV), SM)
+    torch.cuda.synchronize()
+    p = torch.softmax(q[0].double() @ k[0, 0].double().T * SM, -1)
+    ref, size = p @ v[0, 0].double(), p @ v[0, 0].double().abs()
+    # Sums of up to 2^29 / 256 tokens a work-group in fp32, 16 a step, and of all of them: 2^17 steps and 2^11 parts of 2^-24 each,
+    # in numerator and denominator; fp16's P (2^-11), scores (2^-21 of |q| |k| sm, below 2^4) and output (2^-11)
+    tol = size * (2 * (2.0 ** 17 + 2.0 ** 11) * 2.0 ** -24 + 2.0 ** -11 + 2 * 2.0 ** -17) + ref.abs() * 2.0 ** -11
+    assert ((out[0].cpu().double() - ref).abs() <= tol).all()
+
+
 def test_strides_and_temperatures():
     run([3], [130], [140, 150, 131], 12, 2, 64, F16, tau=True)
     run([3], [130], [140, 150, 131], 12, 2, 64, BF16, 32, tau=True)
