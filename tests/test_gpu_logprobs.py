@@ -162,6 +162,35 @@ def test_masks(dtype):
     check(wide, torch.tensor([12345, 8, 160000]), 5)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_masks_begin_and_end_anywhere(dtype):
+    """Long rows, several steps a thread and several work-groups a row, whose masked runs lie anywhere."""
+    v = 70001
+    x, t = draw(8, v, dtype, 5)
+    runs = [(0, 1), (v - 1, v), (0, 20000), (20000, 45000), (45000, v), (1, v), (33333, 33334), (8, v - 8)]
+    for row, (a, b) in enumerate(runs):
+        x[row, a:b] = -math.inf
+    t[:] = torch.tensor([0, 0, 30000, 30000, 0, 0, 33333, 3])
+    check(x, t, 9)
+    check(x.repeat(60, 1)[:, :9001].contiguous(), t.repeat(60).clamp(max=9000), 2)  # a work-group a row
+
+
+@pytest.mark.parametrize("rows", [383, 384])
+def test_rows_of_one_and_several_work_groups(rows):
+    x, t = draw(rows, 20011, torch.bfloat16, rows)
+    check(x, t, 3)
+
+
+def test_rows_past_32_bits():
+    """Rows whose begins lie more than 2^32 bytes apart."""
+    v, step = 5003, (1 << 31) + 8
+    x, t = draw(3, v, torch.bfloat16, 6)
+    room = torch.empty(2 * step + v, dtype=torch.bfloat16, device=DEV)
+    rows = room.as_strided((3, v), (step, 1))
+    rows.copy_(x)
+    check(x, t, 4, out=_k().token_logprobs(rows, t.to(DEV), 4))
+
+
 def test_confident_rows_keep_their_small_logarithms():
     """log p of a token that has nearly all of the probability is the others' sum, not a difference of large numbers."""
     x = torch.full((2, 40000), -10.0)
