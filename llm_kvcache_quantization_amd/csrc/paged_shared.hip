@@ -35,7 +35,6 @@ constexpr int kThreads = 256;
 constexpr int kCols = 128;      // columns a work-group
 constexpr int kMaxRows = 4096;  // rows of a call
 constexpr int kMaxRep = 128;    // query heads of a KV head
-constexpr int kMaxChunks = 64;  // work-groups of a tail, where there are more rows than lanes
 
 // A prefix's work-group: columns col0 .. of the group whose first row is row0, tiles t0 .. t1 of its first len tokens; its
 // parts are slot .. slot + cols - 1 of a KV head's.
@@ -67,7 +66,8 @@ struct ShArgs {
   int32_t q_heads, rep;
   const Unit* units;
   const RowPlan* rows;
-  int32_t chunks;        // of a tail, at most, where there are more than 64 rows, else 0
+  int2* map;             // {row, chunk} of the tails' work-groups, -1 for none, where there are more than 64 rows
+  int32_t groups;        // work-groups of the tails of a KV head
   int32_t fill;          // work-groups that the tails of a KV head are shared out over (and one more a row, at most)
   int32_t prefix_slots;  // parts of the prefixes of a KV head; then those of the tails, [work-group][head]
   uint32_t tails;        // work-groups of tails, the launch's last
@@ -100,22 +100,18 @@ struct Tail {
 };
 
 // Which row a tail's work-group is of, and which of its chunks; and, of each row, what the join needs: {first
-// work-group, work-groups, whether it shares}.  Up to 64 rows are in a wave's lanes: the tiles of all are shared out
-// evenly, whatever their lengths.  More have as many chunks each.
+// work-group, work-groups, whether it shares}.  The tiles of all rows are shared out evenly, whatever their lengths.  Up to 64
+// rows are in a wave's lanes, and each work-group finds its own; those of more rows find it in a launch before this.
 struct Tails {
   int row, chunk, chunks;
   __device__ __forceinline__ Tails(const ShArgs& a, int at, bool write) {
     const int B = a.c.batch;
     row = -1;
-    if (a.chunks) {
-      if (at < B * a.chunks) {
-        const int b = at / a.chunks;
-        chunk = at % a.chunks;
-        const Tail t(a, plan_of_row(a.rows, b).len, ((const_i32)a.lens)[b]);
-        chunks = min(a.chunks, (t.count + kTailTiles - 1) / kTailTiles);
-        if (write && chunk == 0 && threadIdx.x == 0) a.places[b] = {b * a.chunks, chunks, t.shares, 0};
-        if (chunk < chunks) row = b;
-      }
+    if (a.map) {
+      const const_i32 m = (const_i32)(a.map + at);
+      row = m[0];
+      chunk = m[1];
+      if (row >= 0) chunks = ((const_i32)(a.places + row))[1];
       return;
     }
     const int lane = threadIdx.x & 63;
@@ -137,6 +133,39 @@ struct Tails {
     chunks = __builtin_amdgcn_readlane(mine, row);
   }
 };
+
+// Tails of more than 64 rows: a work-group, a run of rows a thread.
+__global__ __launch_bounds__(kThreads) void shared_places_kernel(ShArgs a) {
+  __shared__ unsigned long long total;
+  __shared__ int sums[kThreads / 64];
+  const int B = a.c.batch, tid = threadIdx.x, per_thread = (B + kThreads - 1) / kThreads;
+  const int b0 = min(tid * per_thread, B), b1 = min(b0 + per_thread, B);
+  if (tid == 0) total = 0;
+  __syncthreads();
+  unsigned long long count = 0;
+  for (int b = b0; b < b1; ++b) count += (unsigned long long)Tail(a, a.rows[b].len, a.lens[b]).count;
+  atomicAdd(&total, count);
+  __syncthreads();
+  const int per = max((int)((total + (unsigned)a.fill - 1) / (unsigned)a.fill), kTailTiles);
+  int mine = 0;
+  for (int b = b0; b < b1; ++b) mine += (Tail(a, a.rows[b].len, a.lens[b]).count + per - 1) / per;
+  const int upto = scan64(mine);
+  if ((tid & 63) == 63) sums[tid >> 6] = upto;
+  __syncthreads();
+  int at = upto - mine, all = 0;
+  for (int w = 0; w < kThreads / 64; ++w) {
+    if (w < tid >> 6) at += sums[w];
+    all += sums[w];
+  }
+  for (int b = b0; b < b1; ++b) {
+    const Tail t(a, a.rows[b].len, a.lens[b]);
+    const int n = (t.count + per - 1) / per;
+    a.places[b] = {at, n, t.shares, 0};
+    for (int i = 0; i < n; ++i) a.map[at + i] = {b, i};
+    at += n;
+  }
+  for (int i = all + tid; i < a.groups; i += kThreads) a.map[i] = {-1, 0};
+}
 
 __device__ const u32x4 zero_row[16] = {};
 
@@ -812,8 +841,8 @@ int check(const kvq_shared_decode_params* p, PagedCache& c) {
 }
 
 struct Launch {
-  int chunks, fill;
-  int64_t slots, places, acc, bytes;
+  int fill;
+  int64_t groups, slots, places, map, acc, bytes;
   int64_t tails, grid;
 };
 
@@ -822,37 +851,34 @@ Launch launch_of(const kvq_shared_decode_params& p) {
   const int64_t B = p.cache.batch, H = p.cache.kv_heads, rep = p.q_heads / H;
   const int64_t tiles = ((int64_t)p.cache.max_pages * p.cache.page_size + kBN - 1) / kBN;
   const int64_t most = (tiles + kTailTiles - 1) / kTailTiles;  // of a row
-  int64_t groups;  // work-groups of tails, a KV head
-  if (B <= 64) {
-    int64_t fill = 2 * kTarget / H;
-    // Long tails in many pieces end together: 32 rows of 40 / 8 heads with up to 4000 tokens of their own behind 32768 shared INT8
-    // ones over B, 2 B and 4 B 150, 129 and 123 us; 4 rows with 16000 over 4 B 141, so 79.  Short ones have no more pieces than
-    // kTailTiles allows.
-    if (fill < 4 * B) fill = 4 * B;
-    w.fill = (int)fill;
-    groups = fill + B < B * most ? fill + B : B * most;
-    if (groups < 1) groups = 1;  // who writes the places
-  } else {
-    int64_t chunks = kTarget / (B * H);
-    if (chunks > kMaxChunks) chunks = kMaxChunks;
-    if (chunks > most) chunks = most;
-    w.chunks = (int)(chunks < 1 ? 1 : chunks);
-    groups = B * w.chunks;
-  }
-  w.slots = p.plan.slots + groups * rep;
+  // Long tails in many pieces end together: 32 rows of 40 / 8 heads with up to 4000 tokens of their own behind 32768 shared INT8
+  // ones over B, 2 B and 4 B 150, 129 and 123 us; 4 rows with 16000 over 4 B 141, so 79.  Short ones have no more pieces than
+  // kTailTiles allows; work-groups that find none are dear where there are many rows.
+  int64_t fill = 2 * kTarget / H, rows = B <= 64 ? 4 * B : B;
+  if (fill < rows) fill = rows;
+  w.fill = (int)fill;
+  // what Tails, or the launch before it, makes of that: a piece of each row at the least
+  w.groups = fill + B < B * most ? fill + B : B * most;
+  if (w.groups < 1) w.groups = 1;  // who writes the places
+  w.slots = p.plan.slots + w.groups * rep;
   w.places = (8 * H * w.slots + 63) / 64 * 64;
-  w.acc = w.places + (16 * B + 63) / 64 * 64;
+  w.map = w.places + (16 * B + 63) / 64 * 64;
+  w.acc = w.map + (B > 64 ? (8 * w.groups + 63) / 64 * 64 : 0);
   w.bytes = w.acc + 512 * H * w.slots;
-  w.tails = H * groups;
+  w.tails = H * w.groups;
   w.grid = w.tails + H * p.plan.units;
   return w;
 }
 
 template <class T, bool I8, int GS>
 int launch(const ShArgs& a, const Launch& w, hipStream_t st) {
+  int rc = KVQ_OK;
+  if (a.map) {
+    hipLaunchKernelGGL(shared_places_kernel, dim3(1), dim3(kThreads), 0, st, a);
+    if ((rc = launched())) return rc;
+  }
   hipLaunchKernelGGL((shared_decode_kernel<T, I8, GS>), dim3((unsigned)w.grid), dim3(kThreads), 0, st, a);
-  const int rc = launched();
-  if (rc) return rc;
+  if ((rc = launched())) return rc;
   hipLaunchKernelGGL(shared_join_kernel<T>, dim3((unsigned)a.q_heads, (unsigned)a.c.batch), dim3(kThreads), 0, st, a);
   return launched();
 }
@@ -879,12 +905,13 @@ int decode(const kvq_shared_decode_params* p, hipStream_t st) {
   a.q_heads = p->q_heads; a.rep = p->q_heads / a.c.kv_heads;
   a.rows = (const RowPlan*)p->plan_words;
   a.units = (const Unit*)(p->plan_words + 8 * (int64_t)p->plan.rows);
-  a.chunks = w.chunks; a.fill = w.fill;
+  a.fill = w.fill; a.groups = (int32_t)w.groups;
   a.prefix_slots = p->plan.slots;
   a.tails = (uint32_t)w.tails;
   a.slots = w.slots;
   a.ml = (float2*)p->workspace;
   a.places = (int4*)((uint8_t*)p->workspace + w.places);
+  if (a.c.batch > 64) a.map = (int2*)((uint8_t*)p->workspace + w.map);
   a.acc = (float*)((uint8_t*)p->workspace + w.acc);
   const bool b16 = p->q_type == KVQ_PAGED_BF16;
   const int gs = p->cache.format == KVQ_PAGED_INT8 ? p->cache.group_size : 0;

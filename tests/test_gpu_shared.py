@@ -125,6 +125,15 @@ def test_most_rows():
         check(out[b], ref, tol, ("row", b))
 
 
+@pytest.mark.parametrize("dtype,int8", [(F16, 0), (BF16, 64)])
+def test_ragged_tails_of_many_rows(dtype, int8):
+    """More than 64 rows: one of them long, some with nothing of their own, some shorter than their prefix or empty."""
+    lens = [64 + 7 * (i % 5) for i in range(90)]
+    lens[3], lens[20], lens[21], lens[50], lens[51] = 4000, 0, 13, 64, 1
+    run([60, 1, 29], [64, 0, 48], lens, 4, 2, 16, dtype, int8)
+    run([257], [128], [128 + (3000 if i in (0, 255, 256) else i % 3) for i in range(257)], 2, 1, 32, dtype, int8)
+
+
 def test_long_tails():
     run([2, 1], [100, 20], [9000, 100, 5000], 12, 2, 16, F16)
     run([2], [64], [30000, 64], 5, 1, 128, BF16, 32)
