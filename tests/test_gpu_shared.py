@@ -270,6 +270,25 @@ def test_same_bits_again_and_in_a_graph(dtype, int8):
         assert torch.equal(got, want), i
 
 
+def test_many_rows_in_a_graph():
+    """More than 64 rows, whose tails a launch of their own shares out: replays follow the lengths of the moment."""
+    K = _k()
+    pool = Groups([70], [128], [129 + 11 * i for i in range(70)], 2, 16, F16).cuda()
+    q = torch.randn(70, 4, D, device=DEV).half()
+    lens = torch.tensor(pool.lens, dtype=torch.int32, device=DEV)
+    prefix = K.SharedPrefix(pool.sizes, pool.shared, 4, 2, DEV)
+    K.decode_attn_shared(q, *pool.args(), lens, prefix, SM)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = K.decode_attn_shared(q, *pool.args(), lens, prefix, SM)
+    for i in range(4):
+        lens.copy_((torch.tensor(pool.lens, device=DEV) - 37 * i).clamp(min=128 if i < 3 else 0))
+        want = K.decode_attn_shared(q, *pool.args(), lens, prefix, SM)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want), i
+
+
 def test_another_stream():
     K = _k()
     pool = Groups([3], [640], [700, 640, 900], 2, 16, F16).cuda()
