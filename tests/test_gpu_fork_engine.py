@@ -34,6 +34,7 @@ def test_forked_steps(dtype, pages, page, monkeypatch):
 
     print(f"[fork] {dtype} {pages} page {page}", flush=True)
     monkeypatch.setattr(M, "_MIN_SAVED", 1)
+    monkeypatch.setattr(M, "_PATCHED", 1)
     monkeypatch.setattr(M, "_DEARER", dict.fromkeys(M._DEARER, 1.0))
     shared = []
     real = M.decode_attn_shared
@@ -152,6 +153,7 @@ def test_samples_have_their_log_probabilities(dtype, kv, monkeypatch):
     import llm_kvcache_quantization_amd.paged_cache as M
 
     monkeypatch.setattr(M, "_MIN_SAVED", 1)
+    monkeypatch.setattr(M, "_PATCHED", 1)
     monkeypatch.setattr(M, "_DEARER", dict.fromkeys(M._DEARER, 1.0))
     used = []
     real = M.decode_attn_shared

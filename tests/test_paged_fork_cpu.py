@@ -149,9 +149,10 @@ def test_ending_and_reordering(calls):
     m.check()
 
 
-@pytest.mark.parametrize("seed", range(12))
-def test_any_run_of_calls(calls, seed):
-    """Random appends, steps, forks (beams: some twice, some ended) and compactions."""
+@pytest.mark.parametrize("seed", range(24))
+def test_any_run_of_calls(calls, monkeypatch, seed):
+    """Random appends, steps, forks (beams: some twice, some ended) and compactions; tables laid out or changed."""
+    monkeypatch.setattr(M, "_PATCHED", 1 if seed % 2 else 1 << 30)
     rng = random.Random(seed)
     c = make()
     m = Model(c)
