@@ -267,12 +267,14 @@ class PagedKVCache(_EngineBase):
             self._handle = PagePools([x for pool in self._pools if pool is not None for x in pool if x is not None])
         t = torch.tensor([[self._rows[b][i] for b, i in places], new, lens, *zip(*places)], dtype=torch.int32, device=device)
         copy_paged(self._handle, t[0], t[1], t[2])
+        table = self._table
+        if table is not None:  # another tensor: calls on other streams may still read the one that was
+            table = table.index_put((t[3], t[4]), t[1]) if table.numel() >= _PATCHED else None
         del self._free[len(self._free) - len(places) :]
         for (b, i), page in zip(places, new):
             self._drop_page(self._rows[b][i])
             self._rows[b][i] = page
-        if self._table is not None:  # another tensor: calls on other streams may still read the one that was
-            self._table = self._table.index_put((t[3], t[4]), t[1]) if self._table.numel() >= _PATCHED else None
+        self._table = table
         self._groups = None
 
     def _reserve(self, layer_id: int, counts: List[int], device) -> None:
