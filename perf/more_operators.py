@@ -136,10 +136,11 @@ def prepare(case, seed):
         # a model's logits: a wide bulk and a few tokens that stand out
         x = randn(n, v, dtype=torch.float32).mul_(2.0)
         likely = torch.randint(v, (n, 24), generator=g, device=DEV)
-        x.scatter_add_(1, likely, torch.rand(n, 24, generator=g, device=DEV) * 12)
+        # (one that is drawn twice has the larger, whichever a GPU writes first)
+        x.scatter_reduce_(1, likely, x.gather(1, likely) + torch.rand(n, 24, generator=g, device=DEV) * 12, "amax")
         if case["masked"]:
             x.masked_fill_(torch.rand(n, v, generator=g, device=DEV) < 0.95, -math.inf)
-            x.scatter_(1, likely, torch.rand(n, 24, generator=g, device=DEV) * 8)
+            x.scatter_reduce_(1, likely, torch.rand(n, 24, generator=g, device=DEV) * 8, "amax", include_self=False)
         # mostly tokens that the model holds for likely, as a text has them
         tokens = torch.where(torch.rand(n, generator=g, device=DEV) < 0.7, likely[:, 0],
                              torch.randint(v, (n,), generator=g, device=DEV))
