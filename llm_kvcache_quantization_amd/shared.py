@@ -15,7 +15,8 @@ from __future__ import annotations
 
 import ctypes
 import functools
-from typing import Optional, Sequence, Tuple, Union
+from bisect import bisect_left
+from typing import Dict, List, Optional, Sequence, Tuple, Union
 
 import torch
 from torch import Tensor
@@ -69,6 +70,22 @@ class PagePools:
         self._blocks = (C.PagePool * len(rows))(*rows)
         self._at = ctypes.addressof(self._blocks)
 
+    @functools.cached_property
+    def _grids(self) -> Tuple[Dict[Tuple[int, int], List[int]], List[int]]:
+        """Where the tensors' pages begin, to find those that two tensors have in common: of each (page stride, address of a page
+        modulo it) the tensors' first pages as multiples of the stride, rising; and the addresses of those that repeat one page."""
+        grids: Dict[Tuple[int, int], List[int]] = {}
+        fixed = []
+        for t in self.tensors:
+            at, step = t.data_ptr(), t.stride(0) * t.element_size()
+            if step:
+                grids.setdefault((step, at % step), []).append(at // step)
+            else:
+                fixed.append(at)
+        for firsts in grids.values():
+            firsts.sort()
+        return grids, fixed
+
 
 @functools.lru_cache(maxsize=256)
 def _scratch(info: Tuple[int, ...], cols: int, size: int, rows: int, heads: int, q_heads: int) -> int:
@@ -85,12 +102,42 @@ def _scratch(info: Tuple[int, ...], cols: int, size: int, rows: int, heads: int,
 Pages = Union[Tensor, Sequence[int]]
 
 
-def _page_numbers(x: Pages, name: str, pages: int, device: torch.device) -> Tensor:
+def _apart(pools: PagePools, src: Optional[List[int]], to: PagePools, dst: List[int]) -> None:
+    """Refuses pages that are written twice, or written and read (`src` None: not known here)."""
+    written = set(dst)
+    if len(written) < len(dst):
+        raise ValueError("no page may be written twice")
+    if not written:
+        return
+    low, high = min(written), max(written)
+    (reads, fixed), (writes, _) = pools._grids, to._grids
+    for grid, firsts in writes.items():
+        for i, a in enumerate(firsts):  # page d of a tensor is page d - k of one that begins k pages behind it
+            for b in firsts[i + 1 :]:
+                if b - a > high - low:
+                    break
+                # (a tensor that the pools name twice is written twice, with the same)
+                if (b > a or to is not pools) and any(d + b - a in written for d in dst):
+                    raise ValueError("no page may be written twice: tensors that are written share their memory")
+        if not src:
+            continue
+        least, most = low - max(src), high - min(src)
+        for r in reads.get(grid, ()):  # page s of a tensor is page s + r - w of one that begins at w
+            for w in firsts[bisect_left(firsts, r - most) :]:
+                if r - w < least:
+                    break
+                if any(s + r - w in written for s in src):
+                    raise ValueError("no page may be written by one pair and read by another")
+        for at in fixed:
+            if at % grid[0] == grid[1] and any(at // grid[0] - w in written for w in firsts):
+                raise ValueError("no page may be written by one pair and read by another")
+
+
+def _page_numbers(x: Union[Tensor, List[int]], name: str, pages: int, device: torch.device) -> Tensor:
     if isinstance(x, Tensor):
         if x.ndim != 1:
             raise ValueError(f"{name} must be [n], got {tuple(x.shape)}")
         return _i32(x, name, x.shape[0], device)
-    x = [int(v) for v in x]
     if any(not 0 <= v < pages for v in x):
         raise ValueError(f"{name} must be pages of the pool, 0 to {pages - 1}")
     return torch.tensor(x, dtype=torch.int32, device=device)
@@ -103,6 +150,8 @@ def copy_paged(pools: Union[PagePools, Sequence[Tensor]], src: Pages, dst: Pages
 
     ``src`` and ``dst`` [n] are integer tensors, or whole numbers from the host, which are checked; of tensors, pairs with a
     page that is not there are left out.  No page may be written by two pairs, or written by one and read by another.
+    (Of numbers from the host that is refused too, where pages are the same because the pools' tensors and those of
+    ``into`` are the same or slices of one another's pages; memory that is cut into pages in two ways is not looked for.)
     ``into`` has the pools' heads, page size, row sizes and types; its number of pages may differ.
     """
     pools = pools if isinstance(pools, PagePools) else PagePools(pools)
@@ -115,10 +164,11 @@ def copy_paged(pools: Union[PagePools, Sequence[Tensor]], src: Pages, dst: Pages
     if pools._grad or to._grad or forward_ad._current_level >= 0:
         _no_grad(*pools.tensors, *to.tensors)
     device = pools.device
-    if not isinstance(src, Tensor) and not isinstance(dst, Tensor):
-        src, dst = list(src), list(dst)
-        if len(set(dst)) < len(dst) or to is pools and not set(dst).isdisjoint(src):
-            raise ValueError("no page may be written twice, or written and read")
+    if not isinstance(src, Tensor):
+        src = [int(v) for v in src]
+    if not isinstance(dst, Tensor):
+        dst = [int(v) for v in dst]
+        _apart(pools, None if isinstance(src, Tensor) else src, to, dst)
     src, dst = _page_numbers(src, "src", pools.num_pages, device), _page_numbers(dst, "dst", to.num_pages, device)
     n = src.shape[0]
     if dst.shape[0] != n:
