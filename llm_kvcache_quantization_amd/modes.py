@@ -612,6 +612,16 @@ def _columns(scores) -> dict:
     return {name: [getattr(s, name) for s in scores] for name in scores[0]._fields if getattr(scores[0], name) is not None}
 
 
+def _draw(logits: torch.Tensor, temperature: float, generator: torch.Generator) -> torch.Tensor:
+    """A token of each row of logits at `temperature` (0: the likeliest): the first of independent exponential arrivals at rates p;
+    of logits that are NaN any token, where multinomial's check would end the process."""
+    if temperature == 0:
+        return logits.argmax(dim=-1)
+    x = logits.float()
+    p = torch.softmax((x - x.amax(dim=-1, keepdim=True)) / temperature, dim=-1)  # x / temperature alone may pass fp32
+    return (p / torch.empty_like(p).exponential_(generator=generator)).argmax(dim=-1)
+
+
 def sample_from_ids(model, tokenizer, input_ids: torch.Tensor, num_samples: int = 1, max_new_tokens: int = 128,
                     temperature: float = 1.0, seed: int = 1234, top_logprobs: int = 0,
                     kv_dtype: Optional[torch.dtype] = None, group_size: int = 32, page_size: int = 64,
@@ -666,13 +676,7 @@ def sample_from_ids(model, tokenizer, input_ids: torch.Tensor, num_samples: int 
                 cache.fork([b for b in range(batch) for _ in range(num_samples)])
             alive, where = list(range(rows)), slice(None)  # rows of the batch, and the same as an index
             for t in range(max_new_tokens):
-                if temperature > 0:
-                    # the first of independent exponential arrivals at rates p; of logits that are NaN any token, where
-                    # multinomial's check would end the process
-                    p = torch.softmax(logits.float() / temperature, dim=-1)
-                    token = (p / torch.empty_like(p).exponential_(generator=generator)).argmax(dim=-1)
-                else:
-                    token = logits.argmax(dim=-1)
+                token = _draw(logits, temperature, generator)
                 ids[where, t] = token
                 scores = token_logprobs(logits, token, top_logprobs, temperature=temperature if temperature > 0 else 1.0)
                 for name, x in kept.items():

@@ -1,0 +1,51 @@
+"""The draw of sample_from_ids: temperatures down to the coldest, rows without numbers, and how often each token comes."""
+import math
+
+import pytest
+import torch
+
+from llm_kvcache_quantization_amd.modes import _draw
+
+
+def draw(x, temperature, seed=1, device="cpu"):
+    return _draw(x.to(device), temperature, torch.Generator(device=device).manual_seed(seed)).cpu()
+
+
+@pytest.mark.parametrize("temperature", [1.0000001e-30, 1e-29, 1e-20, 1e-3])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+def test_cold_draws_are_the_likeliest(temperature, dtype):
+    """Logits of several thousand, of either sign, with one that leads by 32 and more: 32000 temperatures."""
+    x, best = leading(4096.0, dtype)
+    assert torch.equal(draw(x, temperature), best)
+
+
+@pytest.mark.parametrize("dtype,top,temperature", [(torch.float32, 2.0 ** 33, 1e-29), (torch.bfloat16, 2.0 ** 40, 1e-29),
+                                                   (torch.bfloat16, 2.0 ** 127, 0.125), (torch.float32, 2.0 ** 127, 0.1)])
+def test_logits_whose_quotient_passes_fp32(dtype, top, temperature):
+    x, best = leading(top, dtype)
+    assert torch.equal(draw(x, temperature), best)
+
+
+def leading(top, dtype):
+    """Rows of whole multiples of top / 512, of which one is above all others: some rows all positive or none, some masked."""
+    g = torch.Generator().manual_seed(2)
+    x = torch.randint(-100, 100, (64, 211), generator=g).float()
+    best = torch.randint(211, (64,), generator=g)
+    x[1::4] -= 112
+    x[2::4] += 112
+    x = x / 256 * (top / 2)
+    x[3::4, :7] = -math.inf
+    others = x.scatter(1, best[:, None], -math.inf).amax(1)
+    x.scatter_(1, best[:, None], (others + top / 64)[:, None])
+    return x.to(dtype), best
+
+
+def test_rows_without_numbers_draw_a_token():
+    x = torch.zeros(4, 211)
+    x[0] = math.nan
+    x[1] = -math.inf
+    x[2, 5] = math.inf
+    x[3, 5] = math.nan
+    for t in (0.0, 1e-29, 1.0, 1e29):
+        got = draw(x, t)
+        assert ((got >= 0) & (got < 211)).all()
