@@ -49,3 +49,32 @@ def test_rows_without_numbers_draw_a_token():
     for t in (0.0, 1e-29, 1.0, 1e29):
         got = draw(x, t)
         assert ((got >= 0) & (got < 211)).all()
+
+
+def chi_square(seen, p):
+    """(sum of (seen - n p)^2 / n p, its degrees of freedom); tokens expected fewer than 50 times are counted with the last of
+    the others."""
+    want, order = (seen.sum() * p).sort(descending=True)
+    seen, cells = seen[order], int((want >= 50).sum())
+    seen, want = (torch.cat([x[: cells - 1], x[cells - 1 :].sum(0, keepdim=True)]) for x in (seen, want))
+    return float(((seen - want) ** 2 / want).sum()), cells - 1
+
+
+@pytest.mark.parametrize("temperature", [0.3, 1.0, 1.7, 1e29])
+@pytest.mark.parametrize("device,n", [("cpu", 1 << 16), pytest.param("cuda:0", 1 << 20, marks=pytest.mark.gpu)])
+def test_every_token_comes_as_often_as_its_probability_says(device, n, temperature):
+    """A chi-square of k degrees of freedom is above k + 2 sqrt(20 k) + 40 with a probability below e^-20.  (A draw from a third
+    of 211 tokens alike would have 2 n, one that never draws one of them n / 211.)"""
+    logits = torch.randn(211, generator=torch.Generator().manual_seed(3)) * 1.5
+    p = torch.softmax(logits.double() / temperature, 0)
+    seen = torch.bincount(draw(logits.expand(n, -1), temperature, 5, device), minlength=211).double()
+    value, k = chi_square(seen, p)
+    assert value <= k + 2 * math.sqrt(20 * k) + 40, (value, k)
+
+
+def test_the_chi_square_sees_a_wrong_draw():
+    p = torch.softmax(torch.randn(211, generator=torch.Generator().manual_seed(3)).double(), 0)
+    n = 1 << 16
+    for wrong in (lambda x: x % 70, lambda x: torch.where(x == 100, 101, x)):
+        value, k = chi_square(torch.bincount(wrong(torch.multinomial(p, n, replacement=True, generator=torch.Generator().manual_seed(1))), minlength=211).double(), p)
+        assert value > k + 2 * math.sqrt(20 * k) + 40
