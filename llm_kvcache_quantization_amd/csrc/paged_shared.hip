@@ -608,8 +608,8 @@ __global__ __launch_bounds__(kThreads, 2) void shared_decode_kernel(ShArgs a) {
     load_v(t + 1, p1, ok1, v2);
     p = pages_of(pc, s, min(t + 2, t1 - 1));
     if constexpr (std::is_same<T, TB16>::value) {
-      // bf16 values in fp16: exact once the column's largest is scaled to [1, 2) by a power of two (what lies 2^24
-      // and more below it loses bits that are below the sum's)
+      // bf16 values in fp16, the column's largest scaled to [2^14, 2^15) by a power of two: those down to 2^-31 of that power
+      // are exact, and smaller ones off by at most 2^-39 of it (fp16's least step is 2^-24)
       float top = 0.f;
 #pragma unroll
       for (int kk = 0; kk < 8; ++kk)
@@ -618,7 +618,7 @@ __global__ __launch_bounds__(kThreads, 2) void shared_decode_kernel(ShArgs a) {
           top = fmaxf(top, fmaxf(fabsf(TB16::to_f((uint16_t)q[kk][j])), fabsf(TB16::to_f((uint16_t)(q[kk][j] >> 16)))));
       top = fmaxf(top, xor32(top));
       int ex = (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127;
-      if (ex == 128 || ex == -127) ex = 0;  // Inf or NaN stays what it is; zero or a subnormal is 0
+      ex = ex == 128 || ex == -127 ? 0 : max(ex - 14, -126);  // Inf or NaN stays what it is; zero or a subnormal is 0
       const float g = ldexpf(1.f, -ex);
       scale = ldexpf(scale, ex);
 #pragma unroll
