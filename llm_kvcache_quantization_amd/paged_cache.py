@@ -515,14 +515,12 @@ class PagedKVCache(_EngineBase):
         used = list(dict.fromkeys(page for row in self._rows for page in row if page >= 0))
         if self.num_pages is not None or len(used) == self._total:
             return
-        if not used:
-            self._pools, self._free, self._total, self._handle = [None] * self.num_layers, [], 0, None
-            return
         old = [x for pool in self._pools if pool is not None for x in pool if x is not None]
         pools = [None if pool is None else tuple(None if x is None else x.new_empty((len(used), *x.shape[1:])) for x in pool)
                  for pool in self._pools]
-        handle = PagePools([x for pool in pools if pool is not None for x in pool if x is not None])
-        copy_paged(old, used, range(len(used)), into=handle)
+        handle = PagePools([x for pool in pools if pool is not None for x in pool if x is not None]) if used else None
+        if used:
+            copy_paged(old, used, range(len(used)), into=handle)
         place = {page: i for i, page in enumerate(used)}
         self._pools, self._handle, self._total, self._free = pools, handle, len(used), []
         self._rows = [[place.get(page, -1) for page in row] for row in self._rows]
