@@ -258,15 +258,18 @@ class PagedKVCache(_EngineBase):
                     out.append((b, i))
         return out
 
+    def _page_pools(self) -> PagePools:
+        if self._handle is None:
+            self._handle = PagePools([x for pool in self._pools if pool is not None for x in pool if x is not None])
+        return self._handle
+
     def _copy(self, places: List[Tuple[int, int]], device) -> None:
         """Copies pages of places that are about to be written, of all layers, and puts the copies there."""
         new = self._free[len(self._free) - len(places) :]
         most = [max(x) for x in zip(*[h for h in self._held if h])]  # slots that any layer holds
         lens = [min(self.page_size, max(most[b] - i * self.page_size, 0)) for b, i in places]
-        if self._handle is None:
-            self._handle = PagePools([x for pool in self._pools if pool is not None for x in pool if x is not None])
         t = torch.tensor([[self._rows[b][i] for b, i in places], new, lens, *zip(*places)], dtype=torch.int32, device=device)
-        copy_paged(self._handle, t[0], t[1], t[2])
+        copy_paged(self._page_pools(), t[0], t[1], t[2])
         table = self._table
         if table is not None:  # another tensor: calls on other streams may still read the one that was
             table = table.index_put((t[3], t[4]), t[1]) if table.numel() >= _PATCHED else None
@@ -510,22 +513,27 @@ class PagedKVCache(_EngineBase):
         self._lens = {}
 
     def compact(self) -> None:
-        """Moves what is held into pools of no more pages than that takes, and frees the others' memory.  A cache of a fixed
-        ``num_pages`` keeps its pools."""
-        used = list(dict.fromkeys(page for row in self._rows for page in row if page >= 0))
-        if self.num_pages is not None or len(used) == self._total:
+        """Moves what is held into pools of no more pages than that takes, and frees the others' memory: layer by layer, with room
+        for one layer's new pool.  (Where there is not even that, the cache goes on with what it holds, and the next call gives the
+        rest back.)  A cache of a fixed ``num_pages`` keeps its pools."""
+        if self.num_pages is not None:
             return
-        old = [x for pool in self._pools if pool is not None for x in pool if x is not None]
-        pools = [None if pool is None else tuple(None if x is None else x.new_empty((len(used), *x.shape[1:])) for x in pool)
-                 for pool in self._pools]
-        handle = PagePools([x for pool in pools if pool is not None for x in pool if x is not None]) if used else None
-        if used:
-            copy_paged(old, used, range(len(used)), into=handle)
-        place = {page: i for i, page in enumerate(used)}
-        self._pools, self._handle, self._total, self._free = pools, handle, len(used), []
-        self._rows = [[place.get(page, -1) for page in row] for row in self._rows]
-        self._refs = {place[page]: n for page, n in self._refs.items()}
-        self._table = None
+        used = {page for row in self._rows for page in row if page >= 0}
+        n = len(used)
+        if n < self._total:
+            # within the pools first, in all layers alike: from there on each can shrink by itself, or fail to
+            high = sorted(page for page in used if page >= n)
+            place = dict(zip(high, (page for page in range(n) if page not in used)))
+            if place:
+                copy_paged(self._page_pools(), list(place), list(place.values()))
+            self._rows = [[place.get(page, page) for page in row] for row in self._rows]
+            self._refs = {place.get(page, page): count for page, count in self._refs.items()}
+            self._pools = [None if pool is None else tuple(None if x is None else x[:n] for x in pool) for pool in self._pools]
+            self._total, self._free, self._table, self._handle = n, [], None, None
+        for i, pool in enumerate(self._pools):
+            if pool is not None and any(x is not None and x.untyped_storage().nbytes() > x.nbytes for x in pool):
+                self._handle = None
+                self._pools[i] = tuple(None if x is None else x.clone() for x in pool)
 
     def _prefix(self, layer_id: int, q_heads: int, device) -> Optional[SharedPrefix]:
         """How the sequences share their first tokens, where that is worth an attention of its own."""

@@ -38,3 +38,36 @@ def test_a_cache_that_holds_nothing(dtype, pages):
         out = c.append_decode_attn(layer, q.squeeze(2), k, v, SM)
         want = c.get_kv(layer)[1].repeat_interleave(6, 1).squeeze(2)  # of one token: its V
         assert torch.equal(out, want.to(dtype))
+
+
+@pytest.mark.parametrize("pages", [F16, torch.int8])
+def test_memory(pages):
+    """Most pages are held: the call needs room for one layer's new pool beside the old ones, and gives back the rest; what
+    is held is the same, bit for bit."""
+    K = _k()
+    g = torch.Generator().manual_seed(2)
+    layers, page = 6, 64
+    c = K.PagedKVCache(layers, device=DEV, dtype=pages, page_size=page)
+    for layer in range(layers):
+        k, v = (randn(4, 4, 900, D, dtype=F16, g=g) for _ in range(2))
+        c.append(layer, k, v, lens=[900, 100, 850, 700])
+    c.fork([2, 0, 3, 0])
+    before = [c.get_kv(layer) for layer in range(layers)]
+    k = v = None
+    total = c.get_memory_mb() * 2 ** 20
+    used = len({p for row in c._rows for p in row})
+    one = total / c._total * used / layers
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    base = torch.cuda.memory_allocated()
+    c.compact()
+    peak = torch.cuda.max_memory_allocated() - base
+    left = torch.cuda.memory_allocated() - base
+    assert c.get_memory_mb() * 2 ** 20 == pytest.approx(one * layers)
+    assert peak <= one + 2 ** 20 and left <= one * layers - total + 2 ** 20, (peak, left, one)
+    for layer in range(layers):
+        for a, b in zip(before[layer], c.get_kv(layer)):
+            assert torch.equal(a, b)
+    out = c.append_decode_attn(0, *(randn(4, n, 1, D, dtype=F16, g=g).squeeze(2) if n == 12 else randn(4, n, 1, D, dtype=F16, g=g)
+                                    for n in (12, 4, 4)), SM)
+    assert not out.isnan().any()
