@@ -40,7 +40,7 @@ typedef struct kvq_token_logprobs_params {
   int32_t top;                /* at most vocab and KVQ_LOGPROBS_MAX_TOP */
   int32_t logits_type;
   int32_t tokens64;           /* tokens are int64 */
-  float inv_temperature;      /* positive */
+  float inv_temperature;      /* 1e-30 to 1e30 */
   int32_t reserved;           /* 0 */
 } kvq_token_logprobs_params;
 int kvq_token_logprobs(const kvq_token_logprobs_params* p, kvq_stream_t stream);

@@ -476,7 +476,9 @@ int check(const kvq_token_logprobs_params* p) {
   if (p->rows < 0 || p->vocab < 1) return fail(KVQ_ERR_INVALID, "token logprobs: rows must not be negative and vocab positive");
   if (p->logits_type < KVQ_LOGITS_F16 || p->logits_type > KVQ_LOGITS_F32) return fail(KVQ_ERR_INVALID, "token logprobs: unknown type");
   if (p->top < 0 || p->top > kTop || p->top > p->vocab) return fail(KVQ_ERR_INVALID, "token logprobs: top must be 0 to 32 and at most vocab");
-  if (!(p->inv_temperature > 0.f) || !(p->inv_temperature < 1e30f)) return fail(KVQ_ERR_INVALID, "token logprobs: inv_temperature must be positive and finite");
+  // hotter, the sum of (x - m) e passes fp32: x - m still has a weight up to 100 T, and there are 2^28 of them
+  if (!(p->inv_temperature >= 0.999e-30f) || !(p->inv_temperature <= 1.001e30f))
+    return fail(KVQ_ERR_INVALID, "token logprobs: inv_temperature must be 1e-30 to 1e30");
   if (p->vocab > (1 << 28)) return fail(KVQ_ERR_UNSUPPORTED, "token logprobs: more than 2^28 tokens");
   if (p->rows * parts_of(*p) >= (1 << 24)) return fail(KVQ_ERR_UNSUPPORTED, "token logprobs: too many rows");
   return KVQ_OK;

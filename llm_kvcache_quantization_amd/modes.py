@@ -39,7 +39,7 @@ import torch
 from .cache import (FP16KVCache, INT4KVCache, INT8KVCache, KIVIStyleKVCache, MixedKVCache,
                     RoleAwareAllocatorKVCache, RoleAwareAsymKVCache, load_per_layer_bits_from_policy)
 from .paged_cache import PagedKVCache
-from .scoring import MAX_TOP, token_logprobs
+from .scoring import COLDEST, HOTTEST, MAX_TOP, token_logprobs
 
 # src/engine/generate_loop.py:44-46
 _FUSED_KV_MODES = frozenset({"int8_fused", "int8_ours", "int4_fused", "int4_ours", "int4_ours_mixed"})
@@ -635,8 +635,8 @@ def sample_from_ids(model, tokenizer, input_ids: torch.Tensor, num_samples: int 
 
     if num_samples < 1 or max_new_tokens < 1:
         raise ValueError(f"num_samples and max_new_tokens must be positive, got {num_samples} and {max_new_tokens}")
-    if not (temperature == 0 or 1e-30 < temperature < 1e30):  # what token_logprobs takes
-        raise ValueError(f"temperature must be 0 or positive and finite, got {temperature}")
+    if not (temperature == 0 or COLDEST <= temperature <= HOTTEST):
+        raise ValueError(f"temperature must be 0 or {COLDEST} to {HOTTEST}, got {temperature}")
     if not 0 <= top_logprobs <= MAX_TOP:
         raise ValueError(f"top_logprobs must be 0 to {MAX_TOP}, got {top_logprobs}")
     if not isinstance(input_ids, torch.Tensor):

@@ -18,6 +18,7 @@ from . import _capi as C
 from .paged import _INTEGERS, _call, _no_grad, _packer
 
 MAX_TOP = 32
+COLDEST, HOTTEST = 1e-30, 1e30  # temperatures: in fp32 with their inverse, and sums of differences that still have a weight too
 _TYPES = {torch.float16: C.KVQ_LOGITS_F16, torch.bfloat16: C.KVQ_LOGITS_BF16, torch.float32: C.KVQ_LOGITS_F32}
 _LOGPROBS = _packer(C.TokenLogprobsParams)
 
@@ -47,8 +48,9 @@ def token_logprobs(logits: Tensor, tokens: Optional[Tensor] = None, top: int = 0
     * ``top_tokens`` int64 and ``top_logprobs`` fp32 [..., top]: the ``top`` likeliest tokens (at most 32) and their log
       p, the lower token first among equal logits, NaN logits below all others.
 
-    Sums are fp32.  -Inf logits have probability 0; a row whose softmax is none (a NaN, a +Inf, nothing but -Inf) has
-    NaN for its log probabilities and entropy.
+    Sums are fp32; ``temperature`` is 1e-30 to 1e30.  -Inf logits, and those further below the row's largest than fp32
+    goes, have probability 0; a row whose softmax is none (a NaN, a +Inf, nothing but -Inf) has NaN for its log
+    probabilities and entropy.
     """
     if logits.ndim < 1 or not logits.is_cuda or logits.dtype not in _TYPES:
         raise ValueError(f"logits must be fp16, bf16 or fp32 [..., V] on a GPU, got {logits.dtype} {tuple(logits.shape)} on {logits.device}")
@@ -57,9 +59,8 @@ def token_logprobs(logits: Tensor, tokens: Optional[Tensor] = None, top: int = 0
         raise ValueError("logits must have at least one token")
     if not 0 <= top <= min(MAX_TOP, vocab):
         raise ValueError(f"top must be 0 to {min(MAX_TOP, vocab)}, got {top}")
-    inverse = 1.0 / temperature if temperature > 0 else 0.0
-    if not 0 < inverse < 1e30:
-        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    if not COLDEST <= temperature <= HOTTEST:
+        raise ValueError(f"temperature must be {COLDEST} to {HOTTEST}, got {temperature}")
     if tokens is not None:
         if tokens.shape != shape or tokens.dtype not in _INTEGERS:
             raise ValueError(f"tokens must be integers {tuple(shape)}, one for each row of logits, got {tokens.dtype} {tuple(tokens.shape)}")
@@ -89,5 +90,5 @@ def token_logprobs(logits: Tensor, tokens: Optional[Tensor] = None, top: int = 0
         x.data_ptr(), step, 0 if tokens is None else tokens.data_ptr(), 0 if tokens is None else logprobs.data_ptr(),
         entropy.data_ptr(), best.data_ptr() if top else 0, ids.data_ptr() if top else 0,
         0 if scratch is None else scratch.data_ptr(), nbytes, rows, vocab, top, _TYPES[x.dtype],
-        tokens is not None and tokens.dtype == torch.int64, inverse, 0), device)
+        tokens is not None and tokens.dtype == torch.int64, 1.0 / temperature, 0), device)
     return out

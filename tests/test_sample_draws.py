@@ -1,4 +1,5 @@
 """The draw of sample_from_ids: temperatures down to the coldest, rows without numbers, and how often each token comes."""
+import ctypes
 import math
 
 import pytest
@@ -24,6 +25,26 @@ def test_cold_draws_are_the_likeliest(temperature, dtype):
 def test_logits_whose_quotient_passes_fp32(dtype, top, temperature):
     x, best = leading(top, dtype)
     assert torch.equal(draw(x, temperature), best)
+
+
+def test_temperatures_that_are_taken():
+    """The same from 1e-30 to 1e30 everywhere: sample_from_ids looks before the prompt runs, kvq_token_logprobs at the inverse in
+    fp32 (rows of 0: nothing is launched)."""
+    from llm_kvcache_quantization_amd import sample_from_ids
+    from test_shared_cpu import _lib, _logprobs
+
+    C, L = _lib()
+    ends = [1e-30, math.nextafter(1e-30, 1), 1.00000002e-30, 1.0, 9.9999998e29, math.nextafter(1e30, 0), 1e30]
+    for t in ends:
+        assert L.kvq_token_logprobs(ctypes.byref(_logprobs(C, rows=0, inv_temperature=1.0 / t)), None) == 0, t
+    for t in (0.99e-30, 1.01e30, 1e37):
+        assert L.kvq_token_logprobs(ctypes.byref(_logprobs(C, rows=0, inv_temperature=1.0 / t)), None) == 1, t
+        with pytest.raises(ValueError, match="temperature"):
+            sample_from_ids(None, None, torch.zeros(1, 4, dtype=torch.long), temperature=t)
+    if not torch.cuda.is_available():
+        for t in ends:
+            with pytest.raises(RuntimeError, match="GPU"):
+                sample_from_ids(None, None, torch.zeros(1, 4, dtype=torch.long), temperature=t)
 
 
 def leading(top, dtype):
