@@ -64,7 +64,8 @@ struct AttnTile {
     return sc;
   }
 
-  // P of 32 keys, in 16 bits, from the scores times mul; returns this lane's sum of it.
+  // P of 32 keys from the scores times mul; returns this lane's sum of it.  P is rounded to 16 bits for the product with V,
+  // as the matrix instructions take it (kUp keeps faint ones); the sum is of the unrounded.
   __device__ __forceinline__ float exps(const float16v& sc, float mul, u32x4 (&pb)[2]) const {
     const float mm = -(m == kNegInf ? 0.f : m);
     float s0 = 0.f, s1 = 0.f;

@@ -462,7 +462,9 @@ struct Shared : AttnTile<M> {
       if (!full) mask(sc, s, scale, key0, ok, u);
       const float before = m;
       this->add_sum(this->exps(sc, mul, pb[i]), sc, mul, pb[i]);
-      if (i == 1 && __any(m != before)) {  // the first half's P stand at the maximum before this one
+      // The first half's P stand at the maximum before this one, in 16 bits, and are rounded once more: 2^-11 of a token's
+      // weight again, in tiles that raise the maximum.  In fp32 they would take 8 registers more; groups of 32 hold 250 of 256.
+      if (i == 1 && __any(m != before)) {
         const float f = fast_exp2(before - shift_of(m));
 #pragma unroll
         for (int x = 0; x < 2; ++x)

@@ -8,6 +8,8 @@
 // 105 us, 5.9 TB/s (12 us more with one instruction a logit more, and the likeliest by counting).  Few rows are split over
 // work-groups, whose parts a second launch joins: 32 rows of 151936 with 20 of the likeliest 10 and 4.5 us, a chain of
 // latencies (one row of 32000, in one launch, 8).
+// Exponentials are the hardware's exp2, of an argument rounded as a difference and as a product: relative errors of 0.7 to
+// 1.1e-7 (rows of 32000, one a call) and 0.8e-7 (2047 of 152064), where fp32 with the library's has 0.3 to 0.9e-7 and 0.8e-7.
 //
 // The likeliest: the pass leaves the maximum of every 32 logits that a lane takes (of 64 and more in long rows) in LDS.  The
 // top-th largest of 64 groups' maxima is a bar that at least `top` logits reach; only the 32s that reach it are read
