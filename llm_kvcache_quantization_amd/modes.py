@@ -40,6 +40,7 @@ from .cache import (FP16KVCache, INT4KVCache, INT8KVCache, KIVIStyleKVCache, Mix
                     RoleAwareAllocatorKVCache, RoleAwareAsymKVCache, load_per_layer_bits_from_policy)
 from .paged_cache import PagedKVCache
 from .scoring import COLDEST, HOTTEST, MAX_TOP, token_logprobs
+from .shared import MAX_ROWS
 
 # src/engine/generate_loop.py:44-46
 _FUSED_KV_MODES = frozenset({"int8_fused", "int8_ours", "int4_fused", "int4_ours", "int4_ours_mixed"})
@@ -627,10 +628,10 @@ def sample_from_ids(model, tokenizer, input_ids: torch.Tensor, num_samples: int 
                     kv_dtype: Optional[torch.dtype] = None, group_size: int = 32, page_size: int = 64,
                     num_pages: Optional[int] = None, inv_tau: Optional[torch.Tensor] = None,
                     stop_on_eos: bool = True) -> SampleBatchOutput:
-    """``num_samples`` continuations of each of the prompts input_ids [B, S] (of one length), drawn at ``temperature`` (0: the
-    likeliest token, in all samples alike), over a :class:`PagedKVCache` of ``kv_dtype`` pages (default: the model's type; torch.int8 with
-    scales per ``group_size``).  The prompts run once; their samples share the pages and attend them together.  A sample
-    ends with its eos and leaves the batch."""
+    """``num_samples`` continuations of each of the prompts input_ids [B, S] (of one length; B * num_samples at most 4096), drawn
+    at ``temperature`` (1e-30 to 1e30, or 0: the likeliest token, in all samples alike), over a :class:`PagedKVCache` of
+    ``kv_dtype`` pages (default: the model's type; torch.int8 with scales per ``group_size``).  The prompts run once; their
+    samples share the pages and attend them together.  A sample ends with its eos and leaves the batch."""
     from .patch import INT8CacheWrapperContainer, apply_int8_fused_patch, remove_int8_fused_patch
 
     if num_samples < 1 or max_new_tokens < 1:
@@ -643,6 +644,8 @@ def sample_from_ids(model, tokenizer, input_ids: torch.Tensor, num_samples: int 
         raise TypeError(f"input_ids must be a torch.Tensor, got {type(input_ids)}")
     if input_ids.ndim != 2 or 0 in input_ids.shape:
         raise ValueError(f"input_ids must be non-empty [B, S], got {tuple(input_ids.shape)}")
+    if input_ids.shape[0] * num_samples > MAX_ROWS and max_new_tokens > 1:
+        raise ValueError(f"B * num_samples must be at most {MAX_ROWS}, got {input_ids.shape[0]} * {num_samples}")
     if not torch.cuda.is_available():
         raise RuntimeError("CUDA is required for generation. Please run on a GPU-enabled server.")
     dev = model.device

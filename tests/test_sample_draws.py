@@ -99,3 +99,16 @@ def test_the_chi_square_sees_a_wrong_draw():
     for wrong in (lambda x: x % 70, lambda x: torch.where(x == 100, 101, x)):
         value, k = chi_square(torch.bincount(wrong(torch.multinomial(p, n, replacement=True, generator=torch.Generator().manual_seed(1))), minlength=211).double(), p)
         assert value > k + 2 * math.sqrt(20 * k) + 40
+
+
+def test_more_rows_than_a_step_takes_are_refused_before_the_prompt_runs():
+    from llm_kvcache_quantization_amd import sample_from_ids
+
+    for batch, n in ((1, 4097), (2, 2049), (4097, 1)):
+        with pytest.raises(ValueError, match="4096"):
+            sample_from_ids(None, None, torch.zeros(batch, 4, dtype=torch.long), num_samples=n, max_new_tokens=2)
+    if not torch.cuda.is_available():  # no step comes after the first token
+        with pytest.raises(RuntimeError, match="GPU"):
+            sample_from_ids(None, None, torch.zeros(1, 4, dtype=torch.long), num_samples=4097, max_new_tokens=1)
+        with pytest.raises(RuntimeError, match="GPU"):
+            sample_from_ids(None, None, torch.zeros(2, 4, dtype=torch.long), num_samples=2048)
