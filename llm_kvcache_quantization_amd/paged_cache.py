@@ -514,8 +514,8 @@ class PagedKVCache(_EngineBase):
 
     def compact(self) -> None:
         """Moves what is held into pools of no more pages than that takes, and frees the others' memory: layer by layer, with room
-        for one layer's new pool.  (Where there is not even that, the cache goes on with what it holds, and the next call gives the
-        rest back.)  A cache of a fixed ``num_pages`` keeps its pools."""
+        for one layer's new pool.  (Where there is not even that it raises, the cache goes on with what it holds, and the next call
+        gives the rest back.)  A cache of a fixed ``num_pages`` keeps its pools."""
         if self.num_pages is not None:
             return
         used = {page for row in self._rows for page in row if page >= 0}

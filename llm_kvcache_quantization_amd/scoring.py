@@ -18,7 +18,7 @@ from . import _capi as C
 from .paged import _INTEGERS, _call, _no_grad, _packer
 
 MAX_TOP = 32
-COLDEST, HOTTEST = 1e-30, 1e30  # temperatures: in fp32 with their inverse, and sums of differences that still have a weight too
+COLDEST, HOTTEST = 1e-30, 1e30  # temperatures: they, their inverses and the entropy's sums lie in fp32
 _TYPES = {torch.float16: C.KVQ_LOGITS_F16, torch.bfloat16: C.KVQ_LOGITS_BF16, torch.float32: C.KVQ_LOGITS_F32}
 _LOGPROBS = _packer(C.TokenLogprobsParams)
 
